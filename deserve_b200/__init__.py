@@ -9,9 +9,10 @@ from .context import FlashDecodeCtx, FlashForwardCtx, FlashPrefillCtx, ForwardCt
 from .kvcache import (ChunkHandle, ChunkPool, CopiedPinnedMemory, CpuChunkPool, CpuPagePool, GpuPagePool,
                       KVCacheManager, KVConfig, PagedKVCache, PagePool, PageTableAllocator, PageTableHandle,
                       PinnedKVCache, PinnedMemory, VirtualPagedKVCache, VirtualPagePool, check_page_ownership)
-from .ops import (BatchDecodeWithPagedKVCacheWrapper, BatchPrefillWithPagedKVCacheWrapper, append_paged_kv_cache,
-                  apply_rope, apply_rope_inplace, greedy_sample, paged_decode, paged_prefill, rmsnorm,
-                  rope_append_paged_kv_cache, silu_mul)
+from .ops import (BatchChunkWithPagedKVCacheWrapper, BatchDecodeWithPagedKVCacheWrapper,
+                  BatchPrefillWithPagedKVCacheWrapper, append_paged_kv_cache, apply_rope, apply_rope_inplace,
+                  greedy_sample, paged_chunk_attention, paged_decode, paged_prefill, rmsnorm,
+                  rope_append_paged_kv_cache, sample_top_p, silu_mul, verify_draft)
 from .engine import (BatchDecode, BatchPrefill, BatchResult, KVStage, MicroBatchProcessor, RingPipeline, StageProcessor,
                      StepRequest, make_ring_links)
 from .model import LlamaStage, ModelArgs

@@ -83,6 +83,15 @@ _SIGNATURES = {
     "dsv_paged_prefill": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                   c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                   c_float, c_int, c_void_p]),
+    "dsv_chunk_plan": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64,
+                               _p64, _p64]),
+    "dsv_paged_chunk_attention": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                          c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                          c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p]),
+    "dsv_sample_top_p": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_int64, c_int, c_void_p]),
+    "dsv_verify_draft": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                 c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
     "dsv_pack_pages": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int, c_int,
                                c_void_p, c_void_p]),
     "dsv_unpack_pages": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64,

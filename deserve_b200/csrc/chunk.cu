@@ -1,0 +1,488 @@
+// Attention of a few new tokens per request (the drafted tokens of a speculative step, a short
+// continuation) over the paged cache, with the kv axis split over CTAs.
+//
+//   out[r, h] = sum_t softmax_t(q[r, h] . K[t, h / G] * sm_scale) V[t, h / G],   t <= len_i - n_i + j
+//
+// for row j of request i. The work of a batch is K/V traffic: every row of the cache is needed once,
+// whatever the number of new tokens, so the plan cuts requests along the kv axis until all SMs
+// stream, and a merge kernel folds the partial (max, sum, output) states. An item of the plan is
+// (request, q tile, page range): the tile's tokens and the G q heads of a kv head are stacked into
+// rows (row = token * G + head), so one pass over a K/V tile serves all of them.
+#include <algorithm>
+#include <functional>
+#include <vector>
+
+#include "common.cuh"
+
+namespace dsv {
+namespace {
+
+constexpr int32_t kChunkMagic = 0x44534331;  // "DSC1"
+// header: magic, items, merge rows, q tokens per tile, batch, offset of the items, offset of the merge
+// rows, q heads, kv heads, head_dim, partial rows, page size, dtype, nnz, 2 unused
+constexpr int kPlanHeader = 16;
+constexpr int kItemInts = 8;  // request, first q token, q tokens, first page, end page, partial row or -1, 2 unused
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct ChunkParams {
+  const void* q;
+  const void* pages;
+  const int32_t* qo_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_indptr;
+  const int32_t* kv_last_page_len;
+  void* out;
+  float* lse;
+  const int32_t* items;
+  float* part_o;   // [partial rows][Hq][D]
+  float* part_ml;  // [partial rows][Hq][2]
+  int64_t q_stride, out_stride, page_stride;  // elements
+  int n_q_heads, n_kv_heads, head_dim, page_size, num_pages, nnz;
+  float scale_log2;
+  int* status;
+};
+
+// What a CTA knows about its item after the bounds checks.
+struct Item {
+  int q_row0;    // first q row (global) of the tile
+  int nq;        // tokens of the tile
+  int n_rows;    // nq * G
+  int ip0;       // first entry of the request's page list
+  int tok_begin, tok_end;  // kv tokens [begin, end) of this part
+  int limit0;    // last kv position the tile's first token sees
+  int slot;      // first partial row, -1: write the result
+};
+
+__device__ __forceinline__ bool load_item(const ChunkParams& p, int index, Item& it) {
+  const int32_t* raw = p.items + (int64_t)index * kItemInts;
+  const int4 a = __ldg(reinterpret_cast<const int4*>(raw));
+  const int2 b = __ldg(reinterpret_cast<const int2*>(raw + 4));
+  const int req = a.x, q0 = a.y, nq = a.z, pb = a.w, pe = b.x;
+  const int q_begin = __ldg(p.qo_indptr + req), n_new = __ldg(p.qo_indptr + req + 1) - q_begin;
+  const int ip0 = __ldg(p.kv_indptr + req), n_pages = __ldg(p.kv_indptr + req + 1) - ip0;
+  if (q0 < 0 || nq < 1 || q0 + nq > n_new || q_begin < 0 || q_begin + n_new > p.nnz || pb < 0 || pe > n_pages || pb > pe)
+    return false;
+  const int kv_len = n_pages > 0 ? (n_pages - 1) * p.page_size + __ldg(p.kv_last_page_len + req) : 0;
+  it.q_row0 = q_begin + q0;
+  it.nq = nq;
+  it.n_rows = nq * (p.n_q_heads / p.n_kv_heads);
+  it.ip0 = ip0;
+  it.limit0 = kv_len - n_new + q0;
+  it.tok_begin = pb * p.page_size;
+  // what lies behind the last token's limit is not needed by any row of the tile
+  it.tok_end = max(it.tok_begin, min(min(pe * p.page_size, kv_len), it.limit0 + nq));
+  it.slot = b.y;
+  return true;
+}
+
+// ---- the general kernel: every type, head_dim, page size and pool stride --------------------------
+// CTA of 128 threads: 16 rows of one kv head, 8 threads a row. 32 kv tokens at a time are widened to
+// fp32 in shared memory; a thread computes 4 of its row's 32 scores, the row's softmax runs over the 8
+// lanes, and the thread keeps head_dim / 8 elements of the row's output in registers. fp32
+// multiply-adds bound it: it serves fp32 caches and shapes that the tensor-core kernel does not take.
+constexpr int kSimpleThreads = 128, kSimpleRows = 16, kSimpleTok = 32;
+
+template <typename T, int DMAX>
+__global__ void __launch_bounds__(kSimpleThreads)
+chunk_simple_kernel(const ChunkParams p, int row_blocks) {
+  constexpr int N = Vec16<T>::N;
+  constexpr int NV = DMAX / 32;  // float4 of the output per thread
+  constexpr int LD = DMAX + 4;   // row pitch: float4 loads of 8 lanes x 4 rows fall in different banks
+  extern __shared__ __align__(16) float sm[];
+  float* sq = sm;                             // [16][LD]
+  float* sk = sq + kSimpleRows * LD;          // [32][LD]
+  float* sv = sk + kSimpleTok * LD;           // [32][LD]
+  float* sp = sv + kSimpleTok * LD;           // [16][33]
+  const int G = p.n_q_heads / p.n_kv_heads, D = p.head_dim;
+  const int tid = threadIdx.x;
+  int b = blockIdx.x;
+  const int rb = b % row_blocks;
+  b /= row_blocks;
+  const int kv_head = b % p.n_kv_heads;
+  Item it;
+  if (!load_item(p, b / p.n_kv_heads, it)) {
+    if (tid == 0) record_status(p.status, ST_BAD_PLAN);
+    return;
+  }
+  const int row0 = rb * kSimpleRows;
+  if (row0 >= it.n_rows) return;
+  const int row = tid >> 3, c = tid & 7;
+  const int r = row0 + row;
+  const bool live = r < it.n_rows;
+  const int tok = live ? r / G : 0, head = live ? r % G : 0;
+  const int limit = it.limit0 + tok;
+
+  const int vec = D / N;  // 16-byte vectors of a head row
+  const T* q = reinterpret_cast<const T*>(p.q);
+  for (int x = tid; x < kSimpleRows * vec; x += kSimpleThreads) {
+    const int rr = x / vec, v = x % vec, gr = row0 + rr;
+    float f[N];
+    if (gr < it.n_rows) {
+      Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4*>(q + (int64_t)(it.q_row0 + gr / G) * p.q_stride +
+                                                           (int64_t)(kv_head * G + gr % G) * D) + v), f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) sq[rr * LD + v * N + e] = f[e] * p.scale_log2;
+  }
+  float m = -INFINITY, l = 0.f;
+  float4 o[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+
+  const T* pages = reinterpret_cast<const T*>(p.pages);
+  const int64_t half = (int64_t)p.page_size * p.n_kv_heads * D;
+  for (int t0 = it.tok_begin; t0 < it.tok_end; t0 += kSimpleTok) {
+    const int n = min(kSimpleTok, it.tok_end - t0);
+    __syncthreads();  // the previous tile is no longer read
+    for (int x = tid; x < 2 * kSimpleTok * vec; x += kSimpleThreads) {
+      const int kv = x / (kSimpleTok * vec), y = x % (kSimpleTok * vec), tt = y / vec, v = y % vec;
+      float f[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = 0.f;
+      if (tt < n) {
+        const int t = t0 + tt;
+        int page = __ldg(p.kv_indices + it.ip0 + t / p.page_size);
+        if (page < 0 || page >= p.num_pages) {
+          record_status(p.status, ST_BAD_PAGE_ID);
+          page = 0;
+        }
+        Vec16<T>::unpack(ld_stream16(pages + (int64_t)page * p.page_stride + kv * half +
+                                     ((int64_t)(t % p.page_size) * p.n_kv_heads + kv_head) * D + v * N), f);
+      }
+      float* dst = (kv ? sv : sk) + tt * LD + v * N;
+#pragma unroll
+      for (int e = 0; e < N; ++e) dst[e] = f[e];
+    }
+    __syncthreads();
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < D; d += 4) {
+      const float4 a = *reinterpret_cast<const float4*>(sq + row * LD + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 k = *reinterpret_cast<const float4*>(sk + (c + 8 * i) * LD + d);
+        s[i] = fmaf(a.x, k.x, fmaf(a.y, k.y, fmaf(a.z, k.z, fmaf(a.w, k.w, s[i]))));
+      }
+    }
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = t0 + c + 8 * i;
+      if (t >= it.tok_end || t > limit || !live) s[i] = -INFINITY;
+      mx = fmaxf(mx, s[i]);
+    }
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+    const float off = mx == -INFINITY ? 0.f : mx;  // a row that has seen nothing yet
+    const float keep = exp2f(m - off);
+    m = mx;
+    l *= keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = exp2f(s[i] - off);
+      l += s[i];
+      sp[row * 33 + c + 8 * i] = s[i];
+    }
+    __syncwarp();  // a row's 8 threads are in one warp
+#pragma unroll
+    for (int i = 0; i < NV; ++i) { o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep; }
+    // only what the row sees: a later token's V may hold anything, 0 * inf included
+    const int seen = live ? min(n, limit - t0 + 1) : 0;
+    for (int tt = 0; tt < seen; ++tt) {
+      const float w = sp[row * 33 + tt];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int d = (i * 8 + c) * 4;
+        if (d < D) {
+          const float4 v = *reinterpret_cast<const float4*>(sv + tt * LD + d);
+          o[i].x = fmaf(w, v.x, o[i].x); o[i].y = fmaf(w, v.y, o[i].y);
+          o[i].z = fmaf(w, v.z, o[i].z); o[i].w = fmaf(w, v.w, o[i].w);
+        }
+      }
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int x = 1; x < 8; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  if (!live) return;
+  const int qh = kv_head * G + head;
+  if (it.slot < 0) {
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(it.q_row0 + tok) * p.out_stride + (int64_t)qh * D;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int d = (i * 8 + c) * 4;
+      if (d < D) {
+        dst[d] = from_f32<T>(o[i].x * inv); dst[d + 1] = from_f32<T>(o[i].y * inv);
+        dst[d + 2] = from_f32<T>(o[i].z * inv); dst[d + 3] = from_f32<T>(o[i].w * inv);
+      }
+    }
+    if (p.lse != nullptr && c == 0)
+      p.lse[(int64_t)(it.q_row0 + tok) * p.n_q_heads + qh] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  } else {
+    const int64_t at = (int64_t)(it.slot + tok) * p.n_q_heads + qh;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int d = (i * 8 + c) * 4;
+      if (d < D) *reinterpret_cast<float4*>(p.part_o + at * D + d) = o[i];
+    }
+    if (c == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l);
+  }
+}
+
+// ---- merge of the parts of a split tile -----------------------------------------------------------
+// One warp per (split q row, q head). merge row: {q row, first partial row, parts, partial rows per part}.
+template <typename T>
+__global__ void __launch_bounds__(256)
+chunk_merge_kernel(const int4* __restrict__ rows, int n_rows, const float* __restrict__ part_o,
+                   const float* __restrict__ part_ml, T* __restrict__ out, float* __restrict__ lse, int64_t out_stride,
+                   int n_q_heads, int head_dim) {
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= (int64_t)n_rows * n_q_heads) return;
+  const int4 mr = __ldg(rows + unit / n_q_heads);
+  const int qh = (int)(unit % n_q_heads);
+  const int64_t first = (int64_t)mr.y * n_q_heads + qh, step = (int64_t)mr.w * n_q_heads;
+  float mx = -INFINITY;
+  for (int s = lane; s < mr.z; s += 32) mx = fmaxf(mx, part_ml[(first + s * step) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float off = mx == -INFINITY ? 0.f : mx;
+  float lsum = 0.f;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};  // head_dim <= 256
+  for (int s0 = 0; s0 < mr.z; s0 += 32) {
+    const int n = min(32, mr.z - s0);
+    float w = 0.f;
+    if (lane < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(part_ml + (first + (s0 + lane) * step) * 2);
+      w = exp2f(ml.x - off);
+      lsum += ml.y * w;
+    }
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      const float4* po = reinterpret_cast<const float4*>(part_o + (first + (s0 + s) * step) * head_dim);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if ((lane + 32 * k) * 4 < head_dim) {
+          const float4 v = __ldg(po + lane + 32 * k);
+          acc[k].x = fmaf(ws, v.x, acc[k].x); acc[k].y = fmaf(ws, v.y, acc[k].y);
+          acc[k].z = fmaf(ws, v.z, acc[k].z); acc[k].w = fmaf(ws, v.w, acc[k].w);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
+  const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+  T* dst = out + (int64_t)mr.x * out_stride + (int64_t)qh * head_dim;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = (lane + 32 * k) * 4;
+    if (d < head_dim) {
+      dst[d] = from_f32<T>(acc[k].x * inv); dst[d + 1] = from_f32<T>(acc[k].y * inv);
+      dst[d + 2] = from_f32<T>(acc[k].z * inv); dst[d + 3] = from_f32<T>(acc[k].w * inv);
+    }
+  }
+  if (lse != nullptr && lane == 0)
+    lse[(int64_t)mr.x * n_q_heads + qh] = lsum > 0.f ? (mx + log2f(lsum)) * kLn2 : -INFINITY;
+}
+
+template <typename T, int DMAX>
+cudaError_t launch_simple(const ChunkParams& p, int n_items, int tile_tokens, cudaStream_t st) {
+  const int row_blocks = (tile_tokens * (p.n_q_heads / p.n_kv_heads) + kSimpleRows - 1) / kSimpleRows;
+  const int64_t grid = (int64_t)n_items * p.n_kv_heads * row_blocks;
+  const size_t smem = ((size_t)(kSimpleRows + 2 * kSimpleTok) * (DMAX + 4) + kSimpleRows * 33) * sizeof(float);
+  auto kernel = chunk_simple_kernel<T, DMAX>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<(unsigned)grid, kSimpleThreads, smem, st>>>(p, row_blocks);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_simple_d(const ChunkParams& p, int n_items, int tile_tokens, cudaStream_t st) {
+  if (p.head_dim <= 64) return launch_simple<T, 64>(p, n_items, tile_tokens, st);
+  if (p.head_dim <= 128) return launch_simple<T, 128>(p, n_items, tile_tokens, st);
+  return launch_simple<T, 256>(p, n_items, tile_tokens, st);
+}
+
+}  // namespace
+}  // namespace dsv
+
+extern "C" {
+
+int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int batch, int n_q_heads,
+                   int n_kv_heads, int head_dim, int page_size, int dtype, int sm_count, int32_t* plan_host,
+                   int64_t plan_capacity_i32, int64_t* plan_used_i32, int64_t* workspace_bytes) {
+  using namespace dsv;
+  DSV_REQUIRE(qo_indptr_host && kv_indptr_host && plan_host && plan_used_i32 && workspace_bytes,
+              "chunk_plan: null pointer argument");
+  DSV_REQUIRE(batch >= 0, "chunk_plan: negative batch");
+  DSV_REQUIRE(dtype_ok(dtype), "chunk_plan: unknown dtype %d", dtype);
+  DSV_REQUIRE(n_q_heads > 0 && n_kv_heads > 0 && n_q_heads % n_kv_heads == 0,
+              "chunk_plan: n_q_heads (%d) must be a positive multiple of n_kv_heads (%d)", n_q_heads, n_kv_heads);
+  DSV_REQUIRE(head_dim > 0 && head_dim % 8 == 0 && head_dim <= 256, "chunk_plan: head_dim %d must be a multiple of 8, at most 256",
+              head_dim);
+  DSV_REQUIRE(page_size > 0, "chunk_plan: page_size must be positive");
+  if (sm_count <= 0) sm_count = 148;
+  const int G = n_q_heads / n_kv_heads;
+  const int tile = std::max(1, kSimpleRows / G);
+
+  struct Tile { int req, q0, nq, pages; };
+  std::vector<Tile> tiles;
+  int64_t total_pages = 0;
+  int max_pages = 0;
+  DSV_REQUIRE(qo_indptr_host[0] == 0 && kv_indptr_host[0] >= 0, "chunk_plan: indptr must begin at 0");
+  for (int i = 0; i < batch; ++i) {
+    const int n = qo_indptr_host[i + 1] - qo_indptr_host[i], np = kv_indptr_host[i + 1] - kv_indptr_host[i];
+    DSV_REQUIRE(n >= 0 && np >= 0, "chunk_plan: indptr not monotone at %d", i);
+    DSV_REQUIRE((int64_t)np * page_size < (1ll << 31), "chunk_plan: request %d is longer than 2^31 tokens", i);
+    for (int q0 = 0; q0 < n; q0 += tile) {
+      const int nq = std::min(tile, n - q0);
+      // pages that the tile's last token can see if the last page is full (the kernel knows its true length)
+      const int64_t seen = (int64_t)np * page_size - n + q0 + nq;
+      const int pages = (int)std::max<int64_t>(0, std::min<int64_t>(np, (seen + page_size - 1) / page_size));
+      tiles.push_back({i, q0, nq, pages});
+      total_pages += pages;
+      max_pages = std::max(max_pages, pages);
+    }
+  }
+  // Chunk length: the smallest that keeps the CTA count within 4 per SM, at least 256 tokens.
+  const int64_t target = std::max<int64_t>((int64_t)4 * sm_count / n_kv_heads, (int64_t)tiles.size());
+  const int min_chunk = std::max(1, 256 / page_size);
+  auto count_items = [&](int c) {
+    int64_t k = 0;
+    for (const Tile& t : tiles) k += std::max(1, (t.pages + c - 1) / c);
+    return k;
+  };
+  int lo = min_chunk, hi = std::max(min_chunk, max_pages);
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (count_items(mid) <= target) hi = mid; else lo = mid + 1;
+  }
+  const int chunk = lo;
+  const int64_t n_items = count_items(chunk);
+  int64_t merge_rows = 0, part_rows = 0;
+  for (const Tile& t : tiles) {
+    const int64_t parts = std::max(1, (t.pages + chunk - 1) / chunk);
+    if (parts > 1) { merge_rows += t.nq; part_rows += parts * t.nq; }
+  }
+  const int64_t need = kPlanHeader + kItemInts * n_items + 4 * merge_rows;
+  *plan_used_i32 = need;
+  *workspace_bytes = part_rows * n_q_heads * (head_dim + 2) * (int64_t)sizeof(float);
+  if (need > plan_capacity_i32)
+    return fail(DSV_E_WORKSPACE, "chunk_plan: plan needs %lld int32, capacity %lld", (long long)need,
+                (long long)plan_capacity_i32);
+  DSV_REQUIRE(part_rows < (1ll << 31) && n_items * n_kv_heads < (1ll << 31), "chunk_plan: too many partial states");
+  struct Out { int len; int32_t v[6]; };
+  std::vector<Out> items;
+  items.reserve((size_t)n_items);
+  int32_t* merge = plan_host + kPlanHeader + kItemInts * n_items;
+  int64_t at_merge = 0, at_part = 0;
+  for (const Tile& t : tiles) {
+    const int parts = std::max(1, (t.pages + chunk - 1) / chunk);
+    const int base = t.pages / parts, extra = t.pages % parts;
+    int at = 0;
+    for (int s = 0; s < parts; ++s) {
+      const int len = base + (s < extra ? 1 : 0);
+      items.push_back({len, {t.req, t.q0, t.nq, at, at + len, parts > 1 ? (int32_t)(at_part + (int64_t)s * t.nq) : -1}});
+      at += len;
+    }
+    if (parts > 1) {
+      for (int j = 0; j < t.nq; ++j) {
+        int32_t* m = merge + 4 * at_merge++;
+        m[0] = qo_indptr_host[t.req] + t.q0 + j; m[1] = (int32_t)(at_part + j); m[2] = parts; m[3] = t.nq;
+      }
+      at_part += (int64_t)parts * t.nq;
+    }
+  }
+  std::stable_sort(items.begin(), items.end(), [](const Out& a, const Out& b) { return a.len > b.len; });  // longest first
+  for (int k = 0; k < kPlanHeader; ++k) plan_host[k] = 0;
+  plan_host[0] = kChunkMagic; plan_host[1] = (int32_t)n_items; plan_host[2] = (int32_t)merge_rows; plan_host[3] = tile;
+  plan_host[4] = batch; plan_host[5] = kPlanHeader; plan_host[6] = (int32_t)(kPlanHeader + kItemInts * n_items);
+  plan_host[7] = n_q_heads; plan_host[8] = n_kv_heads; plan_host[9] = head_dim; plan_host[10] = (int32_t)part_rows;
+  plan_host[11] = page_size; plan_host[12] = dtype; plan_host[13] = batch > 0 ? qo_indptr_host[batch] : 0;
+  for (int64_t k = 0; k < n_items; ++k) {
+    int32_t* it = plan_host + kPlanHeader + kItemInts * k;
+    for (int j = 0; j < 6; ++j) it[j] = items[k].v[j];
+    it[6] = it[7] = 0;
+  }
+  return DSV_OK;
+}
+
+int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t* qo_indptr, const void* pages_layer,
+                              int64_t page_stride, int64_t num_pages, const int32_t* kv_indices,
+                              const int32_t* kv_indptr, const int32_t* kv_last_page_len, void* out,
+                              int64_t out_stride_tok, float* lse, const int32_t* plan_host, const int32_t* plan_dev,
+                              void* workspace, int64_t workspace_bytes, int batch, int nnz, int n_q_heads,
+                              int n_kv_heads, int head_dim, int page_size, int dtype, float sm_scale, void* stream) {
+  using namespace dsv;
+  DSV_REQUIRE(dtype_ok(dtype), "chunk: unknown dtype %d", dtype);
+  DSV_REQUIRE(batch >= 0 && nnz >= 0, "chunk: negative batch or nnz");
+  if (batch == 0 || nnz == 0) return DSV_OK;
+  DSV_REQUIRE(q && qo_indptr && pages_layer && kv_indptr && kv_last_page_len && out && plan_host && plan_dev,
+              "chunk: null pointer argument");
+  DSV_REQUIRE(n_q_heads > 0 && n_kv_heads > 0 && n_q_heads % n_kv_heads == 0, "chunk: bad head counts");
+  DSV_REQUIRE(head_dim > 0 && head_dim % 8 == 0 && head_dim <= 256, "chunk: head_dim %d must be a multiple of 8, at most 256",
+              head_dim);
+  DSV_REQUIRE(page_size > 0, "chunk: page_size must be positive");
+  DSV_REQUIRE(num_pages > 0 && num_pages < (1ll << 30), "chunk: num_pages (%lld) out of range", (long long)num_pages);
+  DSV_REQUIRE(plan_host[0] == kChunkMagic && plan_host[4] == batch && plan_host[7] == n_q_heads &&
+                  plan_host[8] == n_kv_heads && plan_host[9] == head_dim && plan_host[11] == page_size && plan_host[12] == dtype,
+              "chunk: plan does not belong to this call");
+  DSV_REQUIRE(nnz >= plan_host[13], "chunk: the plan covers %d rows, q has %d", plan_host[13], nnz);
+  const int n_items = plan_host[1], merge_rows = plan_host[2];
+  const int64_t part_rows = plan_host[10];
+  DSV_REQUIRE(n_items >= 0 && merge_rows >= 0 && part_rows >= 0 && plan_host[3] > 0, "chunk: corrupt plan");
+  if (n_items == 0) return DSV_OK;
+  DSV_REQUIRE(kv_indices != nullptr, "chunk: null pointer argument");
+  const int es = elem_size(dtype);
+  DSV_REQUIRE(aligned16(q) && aligned16(pages_layer) && aligned16(out) && (q_stride_tok * es) % 16 == 0 &&
+                  (out_stride_tok * es) % 16 == 0 && (page_stride * es) % 16 == 0,
+              "chunk: pointers and strides must be 16-byte aligned");
+  DSV_REQUIRE(q_stride_tok >= (int64_t)n_q_heads * head_dim && out_stride_tok >= (int64_t)n_q_heads * head_dim,
+              "chunk: token stride smaller than a row");
+  DSV_REQUIRE(page_stride >= (int64_t)2 * page_size * n_kv_heads * head_dim, "chunk: page_stride smaller than one page");
+  const int64_t ws_need = part_rows * n_q_heads * (head_dim + 2) * (int64_t)sizeof(float);
+  if (ws_need > 0 && (workspace == nullptr || workspace_bytes < ws_need))
+    return fail(DSV_E_WORKSPACE, "chunk: workspace needs %lld bytes, got %lld", (long long)ws_need, (long long)workspace_bytes);
+  DSV_REQUIRE(ws_need == 0 || aligned16(workspace), "chunk: workspace must be 16-byte aligned");
+  ChunkParams p;
+  p.q = q; p.pages = pages_layer; p.qo_indptr = qo_indptr; p.kv_indices = kv_indices; p.kv_indptr = kv_indptr;
+  p.kv_last_page_len = kv_last_page_len; p.out = out; p.lse = lse; p.items = plan_dev + plan_host[5];
+  DSV_REQUIRE(aligned16(p.items) && aligned16(plan_dev + plan_host[6]), "chunk: device plan must be 16-byte aligned");
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + part_rows * n_q_heads * head_dim;
+  p.q_stride = q_stride_tok; p.out_stride = out_stride_tok; p.page_stride = page_stride;
+  p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads; p.head_dim = head_dim; p.page_size = page_size;
+  p.num_pages = (int)num_pages; p.nnz = nnz; p.scale_log2 = sm_scale * kLog2e; p.status = device_status_ptr();
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  switch (dtype) {
+    case DSV_F32: e = launch_simple_d<float>(p, n_items, plan_host[3], st); break;
+    case DSV_F16: e = launch_simple_d<__half>(p, n_items, plan_host[3], st); break;
+    default: e = launch_simple_d<__nv_bfloat16>(p, n_items, plan_host[3], st);
+  }
+  if (e != cudaSuccess) return fail(DSV_E_CUDA, "chunk launch failed: %s", cudaGetErrorString(e));
+  if (merge_rows > 0) {
+    const int4* rows = reinterpret_cast<const int4*>(plan_dev + plan_host[6]);
+    const unsigned grid = (unsigned)(((int64_t)merge_rows * n_q_heads + 7) / 8);
+    switch (dtype) {
+      case DSV_F32:
+        chunk_merge_kernel<float><<<grid, 256, 0, st>>>(rows, merge_rows, p.part_o, p.part_ml, (float*)out, lse, out_stride_tok, n_q_heads, head_dim);
+        break;
+      case DSV_F16:
+        chunk_merge_kernel<__half><<<grid, 256, 0, st>>>(rows, merge_rows, p.part_o, p.part_ml, (__half*)out, lse, out_stride_tok, n_q_heads, head_dim);
+        break;
+      default:
+        chunk_merge_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(rows, merge_rows, p.part_o, p.part_ml, (__nv_bfloat16*)out, lse, out_stride_tok, n_q_heads, head_dim);
+    }
+    DSV_CUDA(cudaGetLastError());
+  }
+  return DSV_OK;
+}
+
+}  // extern "C"

@@ -7,6 +7,7 @@ All tensors must live on a CUDA device; there is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -24,6 +25,22 @@ def _i32_dev(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype != torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor")
     return t
+
+
+def _same_device(what: str, first: torch.Tensor, *others) -> None:
+    _lib.require_cuda(first)
+    for t in others:
+        if t is not None and t.device != first.device:
+            _lib.require_cuda(t)
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def _device_of(t: torch.Tensor):
+    """Context in which the tensor's device is the current one (kernels launch on the current device)."""
+    return _NO_SWITCH if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_NO_SWITCH = contextlib.nullcontext()
 
 
 def _row_stride(t: torch.Tensor, heads: int, dim: int, name: str) -> int:
@@ -392,6 +409,126 @@ class BatchPrefillWithPagedKVCacheWrapper:
         self._dec = None
 
 
+def chunk_plan_capacity(nnz: int, batch: int, sm_count: int = 148) -> int:
+    """int32 entries that a chunk plan for `nnz` new tokens of `batch` requests can need."""
+    return 16 + 8 * (4 * sm_count + 2 * (nnz + batch)) + 4 * nnz
+
+
+def make_chunk_plan(qo_indptr_host: np.ndarray, kv_indptr_host: np.ndarray, n_q_heads: int, n_kv_heads: int,
+                    head_dim: int, page_size: int, dtype: torch.dtype, sm_count: int,
+                    plan_out: np.ndarray) -> tuple[int, int]:
+    """Fill plan_out (int32) with the (request, q tile, page range) work items; returns (int32
+    entries used, device workspace bytes needed)."""
+    qo = np.ascontiguousarray(qo_indptr_host, dtype=np.int32)
+    kv = np.ascontiguousarray(kv_indptr_host, dtype=np.int32)
+    if len(qo) != len(kv) or len(qo) == 0:
+        raise ValueError("chunk_plan: qo_indptr and kv_indptr must both have batch + 1 entries")
+    used, ws = ctypes.c_int64(), ctypes.c_int64()
+    _lib.check(_lib.lib.dsv_chunk_plan(
+        qo.ctypes.data, kv.ctypes.data, len(qo) - 1, n_q_heads, n_kv_heads, head_dim, page_size, _lib.dtype_code(dtype),
+        sm_count, plan_out.ctypes.data, plan_out.size, ctypes.byref(used), ctypes.byref(ws)))
+    return used.value, ws.value
+
+
+def paged_chunk_attention(q: torch.Tensor, qo_indptr: torch.Tensor, paged_kv_cache: torch.Tensor,
+                          kv_indices: torch.Tensor, kv_indptr: torch.Tensor, kv_last_page_len: torch.Tensor,
+                          plan_host: np.ndarray, plan_dev: torch.Tensor, workspace: torch.Tensor | None,
+                          out: torch.Tensor | None = None, sm_scale: float | None = None,
+                          lse: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of a few new tokens per request over the paged cache, the kv axis split over the
+    GPU. Functional form: every buffer explicit. Rows behind the last request are left as they are; lse,
+    if given ([nnz, n_q_heads] fp32), receives the natural-log sum-exp of the scaled scores."""
+    _same_device("chunk attention", q, qo_indptr, paged_kv_cache, kv_indices, kv_indptr, kv_last_page_len, plan_dev,
+                 workspace, out, lse)
+    ps, hkv, d, page_stride = _pages_view(paged_kv_cache)
+    if q.dtype != paged_kv_cache.dtype or (out is not None and out.dtype != q.dtype):
+        raise ValueError("chunk attention: dtypes of q, out and the pages differ")
+    nnz, hq, batch = q.shape[0], q.shape[1], kv_last_page_len.shape[0]
+    qs = _row_stride(q, hq, d, "q")
+    if out is None:
+        out = torch.empty((nnz, hq, d), dtype=q.dtype, device=q.device)
+    os_ = _row_stride(out, hq, d, "out")
+    if out.shape[0] != nnz:
+        raise ValueError("chunk attention: out must have as many rows as q")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (nnz, hq) or not lse.is_contiguous()):
+        raise ValueError(f"chunk attention: lse must be a contiguous float32 tensor [{nnz}, {hq}]")
+    if qo_indptr.shape[0] != batch + 1 or kv_indptr.shape[0] != batch + 1:
+        raise ValueError("chunk attention: qo_indptr and kv_indptr must have batch + 1 entries")
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(d)
+    with _device_of(q):
+        _lib.check(_lib.lib.dsv_paged_chunk_attention(
+            q.data_ptr(), qs, _i32_dev(qo_indptr, "qo_indptr").data_ptr(), paged_kv_cache.data_ptr(), page_stride,
+            paged_kv_cache.shape[0], _i32_dev(kv_indices, "kv_indices").data_ptr(),
+            _i32_dev(kv_indptr, "kv_indptr").data_ptr(), _i32_dev(kv_last_page_len, "kv_last_page_len").data_ptr(),
+            out.data_ptr(), os_, _lib.ptr(lse), plan_host.ctypes.data, _i32_dev(plan_dev, "plan_dev").data_ptr(),
+            _lib.ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), batch, nnz, hq,
+            hkv, d, ps, _lib.dtype_code(q.dtype), float(sm_scale), _lib.current_stream_ptr(q.device)))
+    _lib.LAUNCHES[0] += int(plan_host[1] > 0) + int(plan_host[2] > 0)  # the attention kernel, the merge of split tiles
+    return out
+
+
+class BatchChunkWithPagedKVCacheWrapper:
+    """begin_forward / forward / end_forward object of a step that feeds a few tokens per request (the
+    last token and its drafts), beside the decode and prefill wrappers. `workspace_buffer` is a uint8
+    device tensor owned by the caller: its head holds the device copy of the plan, the rest the split-KV
+    partial states. Two wrappers (or two captured graphs) that may run at the same time need two buffers."""
+
+    _PLAN_BYTES = 1 << 20
+
+    def __init__(self, workspace_buffer: torch.Tensor, kv_layout: str = "NHD"):
+        _lib.require_cuda(workspace_buffer)
+        if kv_layout != "NHD":
+            raise ValueError("only the NHD page layout of the reference is implemented")
+        if workspace_buffer.dtype != torch.uint8 or workspace_buffer.numel() < 2 * self._PLAN_BYTES:
+            raise ValueError("workspace_buffer must be a uint8 tensor of at least 2 MiB")
+        self._ws = workspace_buffer
+        self._sm_count = _lib.device_info()[0]
+        self._plan_host: np.ndarray | None = None
+        self._desc = None
+
+    def begin_forward(self, qo_indptr: torch.Tensor, paged_kv_indptr: torch.Tensor, paged_kv_indices: torch.Tensor,
+                      paged_kv_last_page_len: torch.Tensor, num_qo_heads: int, num_kv_heads: int, head_dim: int,
+                      page_size: int, data_type=torch.float16, *, qo_indptr_host: np.ndarray | None = None,
+                      kv_indptr_host: np.ndarray | None = None) -> None:
+        """Plan the batch. The *_host arrays (same values as the device tensors) avoid device->host copies."""
+        if qo_indptr_host is None:
+            qo_indptr_host = qo_indptr.cpu().numpy()
+        if kv_indptr_host is None:
+            kv_indptr_host = paged_kv_indptr.cpu().numpy()
+        cap = chunk_plan_capacity(int(qo_indptr_host[-1]), len(qo_indptr_host) - 1, self._sm_count)
+        pinned, slot = _pinned_ring("chunk_plan").take(cap)
+        plan = pinned.numpy()
+        used, ws_bytes = make_chunk_plan(qo_indptr_host, kv_indptr_host, num_qo_heads, num_kv_heads, head_dim, page_size,
+                                         data_type if isinstance(data_type, torch.dtype) else torch.float16,
+                                         self._sm_count, plan)
+        if used * 4 > self._PLAN_BYTES:
+            raise _lib.DeserveKVError(f"chunk plan for {int(qo_indptr_host[-1])} tokens does not fit the workspace head")
+        if ws_bytes > self._ws.numel() - self._PLAN_BYTES:
+            raise _lib.DeserveKVError(f"workspace_buffer too small: split-KV partials need {ws_bytes} bytes")
+        self._ws[: used * 4].view(torch.int32).copy_(pinned[:used], non_blocking=True)
+        _pinned_ring("chunk_plan").done(slot)
+        _COUNTERS["h2d_bytes"] += used * 4
+        self._plan_host = plan[:16].copy()  # the header is all that a call reads on the host
+        self._plan_dev, self._partials = self._ws[: self._PLAN_BYTES].view(torch.int32), self._ws[self._PLAN_BYTES :]
+        self._desc = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, num_qo_heads, head_dim)
+
+    def forward(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, causal: bool = True, sm_scale: float | None = None,
+                out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
+        if self._desc is None:
+            raise RuntimeError("forward() called outside begin_forward()/end_forward()")
+        if not causal:
+            raise ValueError("chunk attention is causal: a row sees the cache up to its own position")
+        qo, kv_indptr, kv_indices, last, hq, d = self._desc
+        if q.dim() == 2:
+            q = q.view(-1, hq, d)
+        return paged_chunk_attention(q, qo, paged_kv_cache, kv_indices, kv_indptr, last, self._plan_host, self._plan_dev,
+                                     self._partials, out, sm_scale, lse)
+
+    def end_forward(self) -> None:
+        self._desc = None
+
+
 def rope_append_paged_kv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, indptr: torch.Tensor,
                                offsets: torch.Tensor, paged_kv_cache: torch.Tensor, kv_indices: torch.Tensor,
                                kv_indptr: torch.Tensor, kv_last_page_len: torch.Tensor,
@@ -454,3 +591,83 @@ def greedy_sample(logits: torch.Tensor) -> torch.Tensor:
                                           _lib.current_stream_ptr(logits.device)))
     _lib.LAUNCHES[0] += 1
     return out
+
+
+def _f32_rows(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor [{n}]")
+    return t
+
+
+def _rows_of(t: torch.Tensor, name: str) -> int:
+    """Row stride (elements) of a [rows, vocab] tensor with dense rows."""
+    if t.dim() != 2 or t.shape[1] == 0 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name} must be [rows, vocab] with dense rows")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def sample_top_p(logits: torch.Tensor, temperature: torch.Tensor, top_p: torch.Tensor, uniform: torch.Tensor,
+                 probs: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """int32 tokens drawn from every row of [rows, vocab] logits. temperature, top_p and uniform (in [0, 1),
+    one random number per row) are float32 [rows]; a row with temperature <= 0 takes the argmax. The nucleus
+    is the shortest prefix of the tokens by probability (lower index first among equals) whose mass exceeds
+    top_p; the draw walks it in index order. probs, if given ([rows, vocab] float32), receives the kept,
+    renormalised probabilities: what verify_draft takes as draft_probs."""
+    _same_device("sample_top_p", logits, temperature, top_p, uniform, probs, out)
+    stride = _rows_of(logits, "sample_top_p: logits")
+    rows, vocab = logits.shape
+    for t, name in ((temperature, "temperature"), (top_p, "top_p"), (uniform, "uniform")):
+        _f32_rows(t, rows, f"sample_top_p: {name}")
+    probs_stride = 0
+    if probs is not None:
+        probs_stride = _rows_of(probs, "sample_top_p: probs")
+        if probs.dtype != torch.float32 or probs.shape != logits.shape:
+            raise ValueError(f"sample_top_p: probs must be float32 {tuple(logits.shape)}")
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    elif out.dtype != torch.int32 or out.shape != (rows,) or not out.is_contiguous():
+        raise ValueError(f"sample_top_p: out must be a contiguous int32 tensor [{rows}]")
+    with _device_of(logits):
+        _lib.check(_lib.lib.dsv_sample_top_p(
+            logits.data_ptr(), stride, rows, vocab, temperature.data_ptr(), top_p.data_ptr(), uniform.data_ptr(),
+            out.data_ptr(), _lib.ptr(probs), probs_stride, _lib.dtype_code(logits.dtype),
+            _lib.current_stream_ptr(logits.device)))
+    _lib.LAUNCHES[0] += int(rows > 0)
+    return out
+
+
+def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, indptr: torch.Tensor, uniform: torch.Tensor,
+                 temperature: torch.Tensor, top_p: torch.Tensor,
+                 draft_probs: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Verification of drafted tokens against the target's distribution. Request i owns the rows
+    indptr[i]..indptr[i+1) of a step: `tokens` (int32 [nnz]) are its last token and its drafts as they were
+    fed in, row r of `logits` ([nnz, vocab]) is the target's answer behind tokens[r]. The draft behind row r
+    is accepted when uniform[r] * q(x) < p(x); p is the row's nucleus distribution under temperature[i] and
+    top_p[i], q row r of draft_probs ([nnz, vocab] float32, the distribution the draft was drawn from) or,
+    without draft_probs, 1 at the draft. Returns int32 [batch] tensors (accepted drafts, next token); the next
+    token is drawn from max(p - q, 0) of the first rejected row, or from p of the last row, with the uniform
+    number of the request's last row. A request without rows gets (0, -1)."""
+    _same_device("verify_draft", logits, tokens, indptr, uniform, temperature, top_p, draft_probs)
+    stride = _rows_of(logits, "verify_draft: logits")
+    nnz, vocab = logits.shape
+    batch = indptr.shape[0] - 1
+    if indptr.dim() != 1 or batch < 0 or tokens.shape != (nnz,):
+        raise ValueError("verify_draft: indptr must have batch + 1 entries and tokens one per row of logits")
+    _f32_rows(uniform, nnz, "verify_draft: uniform")
+    _f32_rows(temperature, batch, "verify_draft: temperature")
+    _f32_rows(top_p, batch, "verify_draft: top_p")
+    draft_stride = 0
+    if draft_probs is not None:
+        draft_stride = _rows_of(draft_probs, "verify_draft: draft_probs")
+        if draft_probs.dtype != torch.float32 or draft_probs.shape != logits.shape:
+            raise ValueError(f"verify_draft: draft_probs must be float32 {tuple(logits.shape)}")
+    accepted, following = torch.empty((2, batch), dtype=torch.int32, device=logits.device).unbind(0)
+    workspace = torch.empty(nnz, dtype=torch.uint8, device=logits.device)
+    with _device_of(logits):
+        _lib.check(_lib.lib.dsv_verify_draft(
+            logits.data_ptr(), stride, nnz, vocab, _i32_dev(tokens, "tokens").data_ptr(),
+            _i32_dev(indptr, "indptr").data_ptr(), batch, uniform.data_ptr(), temperature.data_ptr(), top_p.data_ptr(),
+            _lib.ptr(draft_probs), draft_stride, workspace.data_ptr(), nnz, accepted.data_ptr(), following.data_ptr(),
+            _lib.dtype_code(logits.dtype), _lib.current_stream_ptr(logits.device)))
+    _lib.LAUNCHES[0] += int(nnz > 0) + 1 if batch > 0 else 0
+    return accepted, following

@@ -142,6 +142,48 @@ int dsv_greedy_sample(const void* logits, int64_t row_stride, int rows, int voca
                       int32_t* tokens, int dtype, void* stream);
 
 /*
+ * Temperature / top-p sampling of every row of logits, the temperature > 0 branch of
+ * deserve_worker/layer_storage.py:219-253 for a whole batch, with the random numbers
+ * given. Row r has weights w_v = exp((l_v - max l) / temperature[r]); entries are ranked
+ * by value, the lower index first among equals; v is kept when the weights ranked before
+ * it sum to at most top_p[r] times the whole sum (top_p >= 1, or NaN: all are kept; the
+ * first entry always is). tokens[r] is the first kept v in INDEX order whose running sum
+ * of kept weights exceeds uniform[r] (in [0, 1)) times the kept sum. temperature[r] <= 0
+ * (or NaN): the argmax, lowest index among equals. NaN and -inf entries are no tokens; a
+ * row without any gives token 0. probs (optional, may be NULL): [rows, vocab] fp32, the
+ * kept weights over their sum, 0 elsewhere (one at the argmax for a greedy row, all 0 for
+ * a row without tokens). Weights and sums are 64-bit (weights below 2^-45 of the largest
+ * cannot be drawn), so the token does not depend on the launch. vocab <= 2^18
+ * (DSV_E_UNSUPPORTED above). Row strides in elements, any alignment of a row.
+ */
+int dsv_sample_top_p(const void* logits, int64_t row_stride, int rows, int vocab,
+                     const float* temperature, const float* top_p, const float* uniform,
+                     int32_t* tokens, float* probs, int64_t probs_stride, int dtype, void* stream);
+
+/*
+ * Verification of drafted tokens (speculative decoding). It has no counterpart in the
+ * reference. The step's rows are ragged: request i owns rows indptr[i]..indptr[i+1)
+ * (DEVICE int32, batch + 1 entries), the tokens fed in are its last token and its
+ * drafted tokens, tokens[indptr[i]] and on, and logits row r is the target's answer
+ * behind tokens[r]. With p the kept, renormalised probabilities of dsv_sample_top_p under
+ * temperature[i] and top_p[i] (per REQUEST; temperature <= 0: one at the argmax) and q =
+ * draft_probs[r, :] (fp32, the distribution that tokens[r + 1] was drawn from; NULL: drafts
+ * without a distribution, q = 1 at the draft), the draft behind row r is accepted when
+ * uniform[r] * q[x] < p[x], x = tokens[r + 1]. accepted[i] counts the accepted prefix;
+ * next_tokens[i] is drawn, with the uniform number of the request's LAST row, from
+ * max(p - q, 0) of the first rejected row (from p where nothing is left) or from p of
+ * the last row when every draft was accepted: first index in ascending order whose running
+ * sum exceeds u times the whole. A request without rows gets accepted 0 and token -1; a
+ * draft outside [0, vocab) is rejected. Rows behind indptr[batch] are not read.
+ * workspace: device scratch of nnz bytes; may be NULL when nnz is 0.
+ */
+int dsv_verify_draft(const void* logits, int64_t row_stride, int nnz, int vocab,
+                     const int32_t* tokens, const int32_t* indptr, int batch, const float* uniform,
+                     const float* temperature, const float* top_p, const float* draft_probs,
+                     int64_t draft_stride, uint8_t* workspace, int64_t workspace_bytes,
+                     int32_t* accepted, int32_t* next_tokens, int dtype, void* stream);
+
+/*
  * Host-side planning of the split-KV schedule for paged decode attention.
  * Replaces BatchDecodeWithPagedKVCacheWrapper.begin_forward(...) at
  * deserve_worker/execution/exec.py:184-192. Pure host arithmetic: reads
@@ -222,6 +264,43 @@ int dsv_paged_prefill(const void* q, int64_t q_stride_tok, const int32_t* qo_ind
                       const int32_t* plan_host, const int32_t* plan_dev, int batch, int nnz,
                       int n_q_heads, int n_kv_heads, int head_dim, int page_size, int dtype,
                       float sm_scale, int causal, void* stream);
+
+/*
+ * Host-side planning of attention of a few new tokens per request over the paged cache
+ * (dsv_paged_chunk_attention). Reads qo_indptr_host[batch+1] and kv_indptr_host[batch+1]
+ * (HOST memory), cuts every request into q tiles and the page list of a tile into parts
+ * so that the whole GPU streams K/V, and writes the int32 plan (opaque: a header, eight
+ * integers per item, four per q row whose tile was split) with its size and the bytes of
+ * device workspace that the partial states need. Pure host arithmetic. sm_count <= 0
+ * means 148. One plan serves all layers of a step.
+ */
+int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int batch,
+                   int n_q_heads, int n_kv_heads, int head_dim, int page_size, int dtype,
+                   int sm_count, int32_t* plan_host, int64_t plan_capacity_i32,
+                   int64_t* plan_used_i32, int64_t* workspace_bytes);
+
+/*
+ * Causal attention of a few new tokens per request (drafted tokens that are verified, a
+ * short continuation) over one layer's pages, the kv axis split over the GPU. q row j (of
+ * n_i) of request i sees kv positions <= len_i - n_i + j. It computes what
+ * dsv_paged_prefill does, for the batches that kernel is not made for: it keeps the GPU
+ * busy with ONE request, takes fp32, any head_dim that is a multiple of 8 up to 256, any
+ * page size, GQA group and page stride, and returns the log-sum-exp. A row that sees
+ * nothing (len_i - n_i + j < 0) gets output 0 and lse -inf. Rows of q / out / lse behind
+ * qo_indptr[batch] are neither read nor written. out may not alias q. lse (optional, may
+ * be NULL): [nnz, n_q_heads] natural-log sum-exp of the scaled scores. plan_host /
+ * plan_dev: the same plan on the host (header) and on the device; workspace: device
+ * scratch of the size that the plan reported. A replayed CUDA graph may change the
+ * contents of q, pages, kv_indices and kv_last_page_len, not the plan's page counts.
+ */
+int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t* qo_indptr,
+                              const void* pages_layer, int64_t page_stride, int64_t num_pages,
+                              const int32_t* kv_indices, const int32_t* kv_indptr,
+                              const int32_t* kv_last_page_len, void* out, int64_t out_stride_tok,
+                              float* lse, const int32_t* plan_host, const int32_t* plan_dev,
+                              void* workspace, int64_t workspace_bytes, int batch, int nnz,
+                              int n_q_heads, int n_kv_heads, int head_dim, int page_size,
+                              int dtype, float sm_scale, void* stream);
 
 /*
  * dsv_paged_decode for callers that cannot allocate device memory. It has no

@@ -9,7 +9,7 @@
 // (request, q tile, page range): the tile's tokens and the G q heads of a kv head are stacked into
 // rows (row = token * G + head), so one pass over a K/V tile serves all of them.
 #include <algorithm>
-#include <functional>
+#include <type_traits>
 #include <vector>
 
 #include "common.cuh"
@@ -19,7 +19,8 @@ namespace {
 
 constexpr int32_t kChunkMagic = 0x44534331;  // "DSC1"
 // header: magic, items, merge rows, q tokens per tile, batch, offset of the items, offset of the merge
-// rows, q heads, kv heads, head_dim, partial rows, page size, dtype, nnz, 2 unused
+// rows, q heads, kv heads, head_dim, partial rows, page size, dtype, nnz, 16-row blocks of a tile for the
+// tensor-core kernel (0: the shape is not for it), 1 unused
 constexpr int kPlanHeader = 16;
 constexpr int kItemInts = 8;  // request, first q token, q tokens, first page, end page, partial row or -1, 2 unused
 constexpr float kLog2e = 1.4426950408889634f;
@@ -75,6 +76,12 @@ __device__ __forceinline__ bool load_item(const ChunkParams& p, int index, Item&
   it.slot = b.y;
   return true;
 }
+
+}  // namespace
+}  // namespace dsv
+#include "chunk_tma.cuh"
+namespace dsv {
+namespace {
 
 // ---- the general kernel: every type, head_dim, page size and pool stride --------------------------
 // CTA of 128 threads: 16 rows of one kv head, 8 threads a row. 32 kv tokens at a time are widened to
@@ -302,6 +309,29 @@ cudaError_t launch_simple(const ChunkParams& p, int n_items, int tile_tokens, cu
   kernel<<<(unsigned)grid, kSimpleThreads, smem, st>>>(p, row_blocks);
   return cudaGetLastError();
 }
+int ilog2_exact(int x) {  // log2 of a power of two, -1 otherwise
+  if (x <= 0 || (x & (x - 1)) != 0) return -1;
+  int l = 0;
+  while ((1 << l) < x) ++l;
+  return l;
+}
+// kv heads of a CTA of the tensor-core kernel: 8 warps over heads and row blocks
+int heads_per_cta(int n_kv_heads, int row_blocks) {
+  int hb = 8 / row_blocks;
+  while (hb > 1 && n_kv_heads % hb != 0) hb >>= 1;
+  return hb;
+}
+
+template <typename T, int D>
+cudaError_t launch_tma(const CUtensorMap& map, const ChunkParams& p, const chunk_tma::Split& sp, int n_items, cudaStream_t st) {
+  const size_t smem = (size_t)512 * D * chunk_tma::kStages + 1024 + 64;
+  auto kernel = chunk_tma::chunk_tma_kernel<T, D>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<(unsigned)(n_items * (p.n_kv_heads >> sp.hb_log2)), chunk_tma::kThreads, smem, st>>>(map, p, sp);
+  return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t launch_simple_d(const ChunkParams& p, int n_items, int tile_tokens, cudaStream_t st) {
   if (p.head_dim <= 64) return launch_simple<T, 64>(p, n_items, tile_tokens, st);
@@ -329,7 +359,20 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
   DSV_REQUIRE(page_size > 0, "chunk_plan: page_size must be positive");
   if (sm_count <= 0) sm_count = 148;
   const int G = n_q_heads / n_kv_heads;
-  const int tile = std::max(1, kSimpleRows / G);
+  // Rows of a q tile: all new tokens of a request where they fit, so that its K/V is read once. The
+  // tensor-core kernel takes up to 128 rows (8 warps of 16).
+  const bool tensor = dtype != DSV_F32 && (head_dim == 64 || head_dim == 128) && G <= 128 && ilog2_exact(page_size) >= 3;
+  int most = 0;
+  for (int i = 0; i < batch; ++i) most = std::max(most, qo_indptr_host[i + 1] - qo_indptr_host[i]);
+  int row_blocks = 0;
+  if (tensor) {
+    row_blocks = 1;
+    while (row_blocks < 8 && (int64_t)row_blocks * 16 < (int64_t)most * G) row_blocks *= 2;
+    while (row_blocks * 16 < G) row_blocks *= 2;
+  }
+  const int tile = std::max(1, (tensor ? row_blocks * 16 : kSimpleRows) / G);
+  const int ctas_per_item = tensor ? n_kv_heads / heads_per_cta(n_kv_heads, row_blocks)
+                                   : n_kv_heads * ((tile * G + kSimpleRows - 1) / kSimpleRows);
 
   struct Tile { int req, q0, nq, pages; };
   std::vector<Tile> tiles;
@@ -350,20 +393,42 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
       max_pages = std::max(max_pages, pages);
     }
   }
-  // Chunk length: the smallest that keeps the CTA count within 4 per SM, at least 256 tokens.
-  const int64_t target = std::max<int64_t>((int64_t)4 * sm_count / n_kv_heads, (int64_t)tiles.size());
-  const int min_chunk = std::max(1, 256 / page_size);
+  // Part length: compared on a model of the launch. A CTA costs the bytes it streams plus a fixed
+  // overhead (fill and drain of its ring, q, the partial state), a launch that splits anything a merge.
+  // CTAs fill `slots` at a time; the last round is half empty on average.
   auto count_items = [&](int c) {
     int64_t k = 0;
     for (const Tile& t : tiles) k += std::max(1, (t.pages + c - 1) / c);
     return k;
   };
-  int lo = min_chunk, hi = std::max(min_chunk, max_pages);
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (count_items(mid) <= target) hi = mid; else lo = mid + 1;
+  const double page_cost = (double)2 * page_size * n_kv_heads * head_dim * elem_size(dtype) / ctas_per_item;
+  const double overhead = 128.0 * 1024, merge_cost = 192.0 * 1024;
+  const int64_t slots = (int64_t)sm_count * (tensor ? 1 : 4);
+  const int64_t most_items = std::max<int64_t>((int64_t)4 * sm_count, (int64_t)tiles.size());
+  const int min_chunk = std::max(1, 64 / page_size);
+  int chunk = std::max(min_chunk, max_pages);
+  double best = -1.0;
+  auto consider = [&](int64_t c64) {
+    const int c = (int)std::min<int64_t>(std::max<int64_t>(c64, min_chunk), std::max(min_chunk, max_pages));
+    const int64_t k = count_items(c);
+    if (k > most_items) return;
+    const int64_t ctas = k * ctas_per_item;
+    const double longest = std::min(c, max_pages) * page_cost + overhead;
+    double cost = ctas <= slots ? longest
+                                : std::max(longest, ((double)total_pages * ctas_per_item * page_cost + (double)ctas * overhead) / (double)slots) + 0.5 * longest;
+    if (k > (int64_t)tiles.size()) cost += merge_cost;
+    if (best < 0.0 || cost < best) { best = cost; chunk = c; }
+  };
+  if (!tiles.empty()) {
+    for (int parts = 1; parts <= 8; ++parts) consider((max_pages + parts - 1) / parts);
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+      const int64_t c = (total_pages * ctas_per_item + rounds * slots - 1) / (rounds * slots);
+      consider(c);
+      consider(c + std::max<int64_t>(1, c / 16));
+      consider(c + std::max<int64_t>(1, c / 6));
+      consider(c + std::max<int64_t>(1, c / 3));
+    }
   }
-  const int chunk = lo;
   const int64_t n_items = count_items(chunk);
   int64_t merge_rows = 0, part_rows = 0;
   for (const Tile& t : tiles) {
@@ -376,7 +441,7 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
   if (need > plan_capacity_i32)
     return fail(DSV_E_WORKSPACE, "chunk_plan: plan needs %lld int32, capacity %lld", (long long)need,
                 (long long)plan_capacity_i32);
-  DSV_REQUIRE(part_rows < (1ll << 31) && n_items * n_kv_heads < (1ll << 31), "chunk_plan: too many partial states");
+  DSV_REQUIRE(part_rows < (1ll << 31) && n_items * std::max(n_kv_heads * 8, ctas_per_item) < (1ll << 31), "chunk_plan: too many partial states");
   struct Out { int len; int32_t v[6]; };
   std::vector<Out> items;
   items.reserve((size_t)n_items);
@@ -405,6 +470,7 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
   plan_host[4] = batch; plan_host[5] = kPlanHeader; plan_host[6] = (int32_t)(kPlanHeader + kItemInts * n_items);
   plan_host[7] = n_q_heads; plan_host[8] = n_kv_heads; plan_host[9] = head_dim; plan_host[10] = (int32_t)part_rows;
   plan_host[11] = page_size; plan_host[12] = dtype; plan_host[13] = batch > 0 ? qo_indptr_host[batch] : 0;
+  plan_host[14] = row_blocks;
   for (int64_t k = 0; k < n_items; ++k) {
     int32_t* it = plan_host + kPlanHeader + kItemInts * k;
     for (int j = 0; j < 6; ++j) it[j] = items[k].v[j];
@@ -461,7 +527,22 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
   p.num_pages = (int)num_pages; p.nnz = nnz; p.scale_log2 = sm_scale * kLog2e; p.status = device_status_ptr();
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
-  switch (dtype) {
+  const int row_blocks = plan_host[14];
+  DSV_REQUIRE(row_blocks >= 0 && row_blocks <= 8, "chunk: corrupt plan");
+  chunk_tma::Split sp = {};
+  CUtensorMap map;
+  bool tensor = row_blocks > 0 && page_stride == (int64_t)2 * page_size * n_kv_heads * head_dim;
+  if (tensor) {
+    const int hb = heads_per_cta(n_kv_heads, row_blocks);
+    sp.hb_log2 = ilog2_exact(hb); sp.rw_log2 = ilog2_exact(row_blocks); sp.ps_log2 = ilog2_exact(page_size);
+    tensor = chunk_tma::make_tensor_map(&map, pages_layer, num_pages, page_size, n_kv_heads, head_dim, hb, dtype == DSV_BF16);
+  }
+  if (tensor) {
+    if (dtype == DSV_F16)
+      e = head_dim == 128 ? launch_tma<__half, 128>(map, p, sp, n_items, st) : launch_tma<__half, 64>(map, p, sp, n_items, st);
+    else
+      e = head_dim == 128 ? launch_tma<__nv_bfloat16, 128>(map, p, sp, n_items, st) : launch_tma<__nv_bfloat16, 64>(map, p, sp, n_items, st);
+  } else switch (dtype) {
     case DSV_F32: e = launch_simple_d<float>(p, n_items, plan_host[3], st); break;
     case DSV_F16: e = launch_simple_d<__half>(p, n_items, plan_host[3], st); break;
     default: e = launch_simple_d<__nv_bfloat16>(p, n_items, plan_host[3], st);

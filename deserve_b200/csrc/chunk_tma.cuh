@@ -1,0 +1,452 @@
+// Chunk attention for 16-bit K/V on the tensor cores (mma.sync), K/V staged by TMA.
+//
+// A CTA owns one item of the plan for `hb` kv heads: 8 consumer warps and a producer warp, 1 CTA per SM,
+// a 3-deep ring of 512 * D bytes per stage (128 (head, token) rows of K and of V). The warps are split over
+// heads first, then over 16-row blocks of the tile (rw of them), then over 16-token groups of a stage:
+// hb * rw * ts = 8. A K/V tile is read from HBM once for all rows; each row block reads it from shared
+// memory again, which costs rw * 23 bytes per clock and SM at full HBM speed, of 128 available.
+// Per 16 tokens and 16 rows: S = Q K^T as 16 mma.sync.m16n8k16, causal / length mask where a row's limit
+// falls into the group, online softmax on the fragments, O += P V as 16 more.
+#pragma once
+
+#include <cuda.h>
+
+namespace dsv {
+namespace chunk_tma {
+
+constexpr int kConsumerWarps = 8;
+constexpr int kConsumerThreads = kConsumerWarps * 32;
+constexpr int kThreads = kConsumerThreads + 32;
+constexpr int kStages = 3;
+constexpr int kSpinLimit = 1 << 21;
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+// Bounded wait: false (and a status code) when the phase never completes.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* status) {
+  for (int i = 0; i < kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (i > (1 << 16)) __nanosleep(64);  // back off only when the wait is clearly not a normal one
+  }
+  record_status(status, ST_WAIT_TIMEOUT);
+  return false;
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n" ::
+          "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+// The halves of a pair that are no finite numbers (an exponent of all ones), as a mask.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return ((w & E) == E ? 0x0000ffffu : 0u) | (((w >> 16) & E) == E ? 0xffff0000u : 0u);
+}
+__device__ __forceinline__ float ex2(float x) {  // 2^x on the special-function unit; ex2(-inf) = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct Split {
+  int hb_log2, rw_log2, ps_log2;  // kv heads of a CTA, 16-row blocks of a tile, page size
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, const Split sp) {
+  constexpr int DH = D / 64;            // 64-element halves of head_dim
+  constexpr int KSTEPS = D / 16;
+  constexpr int HALF = 128 * D * 2;     // K (or V) part of a stage
+  constexpr int STAGE = 2 * HALF;
+
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;  // swizzle atoms are 1024-byte aligned
+  unsigned char* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t bar_full = smem_base + kStages * STAGE;  // kStages x 8 bytes
+  const uint32_t bar_empty = bar_full + kStages * 8;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int hb_log = sp.hb_log2, hb = 1 << hb_log;
+  const int rw = 1 << sp.rw_log2, ts = kConsumerWarps >> (hb_log + sp.rw_log2);
+  const int ng = kConsumerWarps >> hb_log, ttok = 16 * ng;  // 16-token groups and tokens of a stage
+  const int ps_log = sp.ps_log2, ps = 1 << ps_log;
+  const int bt_log = min(ps_log, 4), bt = 1 << bt_log;      // tokens per TMA box
+  const int bpg = 16 >> bt_log;                               // boxes per 16-token group
+  const int box_bytes = DH * hb * bt * 128;
+  const int G = p.n_q_heads / p.n_kv_heads;
+  const int n_groups = p.n_kv_heads >> hb_log;
+  const int kv_group = blockIdx.x % n_groups;                 // the kv heads of an item are adjacent CTAs
+
+  Item it;
+  if (!load_item(p, blockIdx.x / n_groups, it)) {
+    if (tid == 0) record_status(p.status, ST_BAD_PLAN);
+    return;
+  }
+  const int n_tiles = (it.tok_end - it.tok_begin + ttok - 1) / ttok;
+  const int live_blocks = min(rw, (it.n_rows + 15) >> 4);
+
+  if (tid == 0) {
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, live_blocks * hb * ts);  // warps without a live row take no part
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  __syncthreads();
+
+  // ============================ producer warp ============================================
+  if (warp == kConsumerWarps) {
+    const int32_t* idx = p.kv_indices + it.ip0;
+    const int n_boxes = ng * bpg;  // boxes per tile and per K/V half (<= 16)
+    for (int tile = 0; tile < n_tiles; ++tile) {
+      const int s = tile % kStages;
+      const int tok0 = it.tok_begin + tile * ttok + lane * bt;  // first token of this lane's box
+      const bool mine = lane < n_boxes && tok0 < it.tok_end;
+      int page = 0;
+      if (mine) {
+        page = __ldg(idx + (tok0 >> ps_log));
+        if (page < 0 || page >= p.num_pages) {
+          record_status(p.status, ST_BAD_PAGE_ID);
+          page = 0;
+        }
+      }
+      if (tile >= kStages) {
+        if (!mbar_wait(bar_empty + 8 * s, ((tile / kStages) - 1) & 1, p.status)) return;
+      }
+      const unsigned live = __ballot_sync(0xffffffffu, mine);
+      if (lane == 0) mbar_expect_tx(bar_full + 8 * s, (uint32_t)(__popc(live) * 2 * box_bytes));
+      __syncwarp();
+      if (mine) {
+        const uint32_t dst = smem_base + s * STAGE + lane * box_bytes;
+        const int in_page = tok0 & (ps - 1);
+        tma_load_5d(dst, &tmap, bar_full + 8 * s, 0, in_page, kv_group * hb, 0, 2 * page);
+        tma_load_5d(dst + HALF, &tmap, bar_full + 8 * s, 0, in_page, kv_group * hb, 0, 2 * page + 1);
+      }
+    }
+    return;
+  }
+
+  // ============================ consumer warps ===========================================
+  const int g = lane >> 2, tg = lane & 3;
+  const int head_local = warp & (hb - 1), block = (warp >> hb_log) & (rw - 1), sub = warp >> (hb_log + sp.rw_log2);
+  const int kv_head = kv_group * hb + head_local;
+  const int r0 = block * 16 + g, r1 = r0 + 8;  // this lane's rows
+  const int t_r0 = r0 / G, t_r1 = r1 / G;
+  // last kv position that a row sees in this part; -1 for rows that are not there
+  const int lim0 = r0 < it.n_rows ? min(it.limit0 + t_r0, it.tok_end - 1) : -1;
+  const int lim1 = r1 < it.n_rows ? min(it.limit0 + t_r1, it.tok_end - 1) : -1;
+  const int lim_first = min(it.limit0 + (block * 16) / G, it.tok_end - 1);  // smallest limit of the block's live rows
+  const int lim_last = min(it.limit0 + min(block * 16 + 15, it.n_rows - 1) / G, it.tok_end - 1);
+
+  uint32_t qa[KSTEPS][4];
+  {
+    const T* q0 = reinterpret_cast<const T*>(p.q) + (int64_t)(it.q_row0 + t_r0) * p.q_stride + (int64_t)(kv_head * G + r0 % G) * D;
+    const T* q1 = reinterpret_cast<const T*>(p.q) + (int64_t)(it.q_row0 + t_r1) * p.q_stride + (int64_t)(kv_head * G + r1 % G) * D;
+    const bool a0 = r0 < it.n_rows, a1 = r1 < it.n_rows;
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      const int d0 = kk * 16 + tg * 2;
+      qa[kk][0] = a0 ? *reinterpret_cast<const uint32_t*>(q0 + d0) : 0u;
+      qa[kk][2] = a0 ? *reinterpret_cast<const uint32_t*>(q0 + d0 + 8) : 0u;
+      qa[kk][1] = a1 ? *reinterpret_cast<const uint32_t*>(q1 + d0) : 0u;
+      qa[kk][3] = a1 ? *reinterpret_cast<const uint32_t*>(q1 + d0 + 8) : 0u;
+    }
+  }
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  const float sc = p.scale_log2;
+
+  // Row (128 bytes) of token tl of a 16-token group, head head_local, half dh, inside the group:
+  //   ((box * DH + dh) * hb + head_local) * bt + token_in_box, box = tl >> bt_log.
+  // ldmatrix lane roles: K matrices (tok lo, c), (tok lo, c+1), (tok hi, c), (tok hi, c+1);
+  //                      V matrices (tok lo, c), (tok hi, c), (tok lo, c+1), (tok hi, c+1).
+  const int lr = lane & 7, lm = lane >> 3;
+  const int k_tl = lr + ((lm >> 1) << 3), k_cx = lm & 1;
+  const int v_tl = lr + ((lm & 1) << 3), v_cx = lm >> 1;
+  auto row_of = [&](int tl, int dh) { return (((tl >> bt_log) * DH + dh) * hb + head_local) * bt + (tl & (bt - 1)); };
+  int k_row[DH], v_row[DH];
+#pragma unroll
+  for (int dh = 0; dh < DH; ++dh) {
+    k_row[dh] = row_of(k_tl, dh);
+    v_row[dh] = row_of(v_tl, dh);
+  }
+
+  bool ok = true;
+  if (block < live_blocks) {
+    for (int tile = 0; tile < n_tiles; ++tile) {
+      const int s = tile % kStages;
+      if (!mbar_wait(bar_full + 8 * s, (tile / kStages) & 1, p.status)) {
+        ok = false;
+        break;
+      }
+      for (int grp = sub; grp < ng; grp += ts) {
+        const int wt0 = it.tok_begin + tile * ttok + 16 * grp;
+        if (wt0 > lim_last) break;  // nothing here that a row of this block sees
+        const uint32_t kbase = smem_base + s * STAGE + (uint32_t)(grp * bpg * box_bytes);
+        const uint32_t vbase = kbase + HALF;
+        const bool masked = wt0 + 15 > lim_first;
+        bool poisoned = false;  // V of a token that some row does not see is not a number
+        if (masked) {
+          unsigned char* vg = smem + (vbase - smem_base);
+          const int live = it.tok_end - wt0;
+          if (live < 16) {
+            // whole boxes were brought: tokens past the end hold whatever the pool holds there. Clear them in
+            // V so that 0 * garbage cannot produce a NaN (every warp that reads them writes the same zeros).
+            for (int x = lane; x < (16 - live) * DH * 8; x += 32) {
+              const int ch = x & 7, dh = (x >> 3) % DH, tl = live + (x >> 3) / DH;
+              *reinterpret_cast<uint4*>(vg + row_of(tl, dh) * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
+            }
+            __syncwarp();
+          }
+          for (int x = lane; x < 16 * DH * 8; x += 32) {
+            const int ch = x & 7, dh = (x >> 3) % DH, tl = (x >> 3) / DH;
+            const uint4 v = *reinterpret_cast<const uint4*>(vg + row_of(tl, dh) * 128 + ch * 16);
+            poisoned |= (not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w)) != 0;
+          }
+          poisoned = __any_sync(0xffffffffu, poisoned);
+        }
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) {
+          const int cidx = 2 * kk + k_cx, row = k_row[cidx >> 3];
+          uint32_t b[4];
+          ldmatrix_x4(b, kbase + row * 128 + (((cidx & 7) ^ (row & 7)) << 4));
+          mma16816<T>(s0, qa[kk], b[0], b[1]);
+          mma16816<T>(s1, qa[kk], b[2], b[3]);
+        }
+        if (masked) {
+          const int c0 = wt0 + 2 * tg;
+          if (c0 > lim0) s0[0] = -INFINITY;
+          if (c0 + 1 > lim0) s0[1] = -INFINITY;
+          if (c0 + 8 > lim0) s1[0] = -INFINITY;
+          if (c0 + 9 > lim0) s1[1] = -INFINITY;
+          if (c0 > lim1) s0[2] = -INFINITY;
+          if (c0 + 1 > lim1) s0[3] = -INFINITY;
+          if (c0 + 8 > lim1) s1[2] = -INFINITY;
+          if (c0 + 9 > lim1) s1[3] = -INFINITY;
+        }
+        float mx0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1]));
+        float mx1 = fmaxf(fmaxf(s0[2], s0[3]), fmaxf(s1[2], s1[3]));
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+        const float mn0 = fmaxf(m0, mx0 * sc), mn1 = fmaxf(m1, mx1 * sc);
+        const float off0 = mn0 == -INFINITY ? 0.f : mn0, off1 = mn1 == -INFINITY ? 0.f : mn1;
+        if (__any_sync(0xffffffffu, mn0 > m0 || mn1 > m1)) {  // rescale only when a row maximum moved
+          const float f0 = ex2(m0 - off0), f1 = ex2(m1 - off1);
+          l0 *= f0;
+          l1 *= f1;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
+        }
+        m0 = mn0;
+        m1 = mn1;
+        const float p00 = ex2(fmaf(s0[0], sc, -off0)), p01 = ex2(fmaf(s0[1], sc, -off0));
+        const float p10 = ex2(fmaf(s1[0], sc, -off0)), p11 = ex2(fmaf(s1[1], sc, -off0));
+        const float q00 = ex2(fmaf(s0[2], sc, -off1)), q01 = ex2(fmaf(s0[3], sc, -off1));
+        const float q10 = ex2(fmaf(s1[2], sc, -off1)), q11 = ex2(fmaf(s1[3], sc, -off1));
+        l0 += (p00 + p01) + (p10 + p11);
+        l1 += (q00 + q01) + (q10 + q11);
+        // P is rounded to the 16-bit type of V, as the tensor core needs it; the sum l is not
+        uint32_t pa[4] = {pack2<T>(p00, p01), pack2<T>(q00, q01), pack2<T>(p10, p11), pack2<T>(q10, q11)};
+#pragma unroll
+        for (int jn = 0; jn < D / 16; ++jn) {
+          const int cidx = 2 * jn + v_cx, row = v_row[cidx >> 3];
+          uint32_t v[4];
+          ldmatrix_x4_trans(v, vbase + row * 128 + (((cidx & 7) ^ (row & 7)) << 4));
+          if (poisoned) {  // a zero weight must not meet an infinity: such values are added below
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] &= ~not_finite<T>(v[i]);
+          }
+          mma16816<T>(o[2 * jn], pa, v[0], v[1]);
+          mma16816<T>(o[2 * jn + 1], pa, v[2], v[3]);
+        }
+        if (poisoned) {  // the rest, token by token, only into the rows that see it
+          for (int tl = 0; tl < 16; ++tl) {
+            const int from = g * 4 + ((tl & 7) >> 1);
+            const float2 w0 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[0] : pa[2], from));
+            const float2 w1 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[1] : pa[3], from));
+            const float a = (tl & 1) ? w0.y : w0.x, b = (tl & 1) ? w1.y : w1.x;
+            const bool see0 = wt0 + tl <= lim0, see1 = wt0 + tl <= lim1;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+              const int d = j * 8 + tg * 2, row = row_of(tl, d >> 6);
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + (vbase - smem_base) + row * 128 +
+                                                                    ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2);
+              const uint32_t odd = not_finite<T>(w);
+              const float2 v = unpack2<T>(w);
+              if (odd & 0xffffu) {
+                if (see0) o[j][0] = fmaf(a, v.x, o[j][0]);
+                if (see1) o[j][2] = fmaf(b, v.x, o[j][2]);
+              }
+              if (odd >> 16) {
+                if (see0) o[j][1] = fmaf(a, v.y, o[j][1]);
+                if (see1) o[j][3] = fmaf(b, v.y, o[j][3]);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_empty + 8 * s);  // this warp is done with the stage
+    }
+  }
+  if (!ok) return;
+
+  l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+  l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+  l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+  l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+
+  // ---- merge the warps that share rows and write, through shared memory ---------------------
+  // every issued copy has been waited for above (by a warp with live rows), so the ring is free
+  asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumerThreads) : "memory");
+  constexpr int LD = D + 4;
+  float* sc_o = reinterpret_cast<float*>(smem);        // [warp][16][LD]
+  float* sc_ml = sc_o + kConsumerWarps * 16 * LD;      // [warp][16][2]
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j) {
+    *reinterpret_cast<float2*>(&sc_o[(warp * 16 + g) * LD + j * 8 + tg * 2]) = make_float2(o[j][0], o[j][1]);
+    *reinterpret_cast<float2*>(&sc_o[(warp * 16 + g + 8) * LD + j * 8 + tg * 2]) = make_float2(o[j][2], o[j][3]);
+  }
+  if (tg == 0) {
+    *reinterpret_cast<float2*>(&sc_ml[(warp * 16 + g) * 2]) = make_float2(m0, l0);
+    *reinterpret_cast<float2*>(&sc_ml[(warp * 16 + g + 8) * 2]) = make_float2(m1, l1);
+  }
+  asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumerThreads) : "memory");
+
+  // four consecutive elements of a row per thread
+  const int quads = D / 4;
+  for (int x = tid; x < hb * it.n_rows * quads; x += kConsumerThreads) {
+    const int d = (x % quads) * 4, y = x / quads, r = y % it.n_rows, hl = y / it.n_rows;
+    const int w0 = hl + ((r >> 4) << hb_log), step = 1 << (hb_log + sp.rw_log2);
+    float mx = -INFINITY;
+    for (int s2 = 0; s2 < ts; ++s2) mx = fmaxf(mx, sc_ml[((w0 + s2 * step) * 16 + (r & 15)) * 2]);
+    const float off = mx == -INFINITY ? 0.f : mx;
+    float lsum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s2 = 0; s2 < ts; ++s2) {
+      const int at = (w0 + s2 * step) * 16 + (r & 15);
+      const float a = ex2(sc_ml[at * 2] - off);
+      lsum = fmaf(sc_ml[at * 2 + 1], a, lsum);
+      const float4 v = *reinterpret_cast<const float4*>(&sc_o[at * LD + d]);
+      acc.x = fmaf(v.x, a, acc.x); acc.y = fmaf(v.y, a, acc.y);
+      acc.z = fmaf(v.z, a, acc.z); acc.w = fmaf(v.w, a, acc.w);
+    }
+    const int tok = r / G, qh = (kv_group * hb + hl) * G + r % G;
+    if (it.slot < 0) {
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(it.q_row0 + tok) * p.out_stride + (int64_t)qh * D + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+      if (p.lse != nullptr && d == 0)
+        p.lse[(int64_t)(it.q_row0 + tok) * p.n_q_heads + qh] = lsum == 0.f ? -INFINITY : (mx + log2f(lsum)) * kLn2;
+    } else {
+      const int64_t at = (int64_t)(it.slot + tok) * p.n_q_heads + qh;
+      *reinterpret_cast<float4*>(p.part_o + at * D + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mx, lsum);
+    }
+  }
+}
+
+// ---- host: the tensor map of one layer's pages ----------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_tiled_fn() {
+  static EncodeTiledFn fn = []() -> EncodeTiledFn {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  return fn;
+}
+
+// (64 elements, token in page, kv head, 64-element half of head_dim, 2 * page + {K, V}): one box is the
+// [16 tokens x hb heads x head_dim] slab of a page's K or V, token-major per head, 128-byte swizzled.
+inline bool make_tensor_map(CUtensorMap* map, const void* pages_layer, int64_t num_pages, int page_size, int n_kv_heads,
+                            int head_dim, int hb, bool bf16) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t half_stride = (cuuint64_t)page_size * n_kv_heads * head_dim * 2;
+  const cuuint64_t dims[5] = {64, (cuuint64_t)page_size, (cuuint64_t)n_kv_heads, (cuuint64_t)(head_dim / 64), (cuuint64_t)(2 * num_pages)};
+  const cuuint64_t strides[4] = {(cuuint64_t)n_kv_heads * head_dim * 2, (cuuint64_t)head_dim * 2, 128, half_stride};
+  const cuuint32_t box[5] = {64, (cuuint32_t)(page_size < 16 ? page_size : 16), (cuuint32_t)hb, (cuuint32_t)(head_dim / 64), 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+            const_cast<void*>(pages_layer), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace chunk_tma
+}  // namespace dsv

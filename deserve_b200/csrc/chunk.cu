@@ -241,61 +241,73 @@ chunk_simple_kernel(const ChunkParams p, int row_blocks) {
 }
 
 // ---- merge of the parts of a split tile -----------------------------------------------------------
-// One warp per (split q row, q head). merge row: {q row, first partial row, parts, partial rows per part}.
+// One CTA per (split q row, q head): its 8 warps take the parts round robin, 4 in flight each, and are
+// joined in shared memory. merge row: {q row, first partial row, parts, partial rows per part}.
+// (One warp per row and head took 11 us for the 74 parts of a 64k-token request, a chain of 19 loads.)
+constexpr int kMergeWarps = 8;
+
 template <typename T>
-__global__ void __launch_bounds__(256)
-chunk_merge_kernel(const int4* __restrict__ rows, int n_rows, const float* __restrict__ part_o,
-                   const float* __restrict__ part_ml, T* __restrict__ out, float* __restrict__ lse, int64_t out_stride,
-                   int n_q_heads, int head_dim) {
-  const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit >= (int64_t)n_rows * n_q_heads) return;
-  const int4 mr = __ldg(rows + unit / n_q_heads);
-  const int qh = (int)(unit % n_q_heads);
+__global__ void __launch_bounds__(kMergeWarps * 32)
+chunk_merge_kernel(const int4* __restrict__ rows, const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                   T* __restrict__ out, float* __restrict__ lse, int64_t out_stride, int n_q_heads, int head_dim) {
+  __shared__ float4 s_acc[kMergeWarps][64];  // head_dim <= 256
+  __shared__ float s_m[kMergeWarps], s_l[kMergeWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4 mr = __ldg(rows + blockIdx.x / n_q_heads);
+  const int qh = (int)(blockIdx.x % n_q_heads);
   const int64_t first = (int64_t)mr.y * n_q_heads + qh, step = (int64_t)mr.w * n_q_heads;
-  float mx = -INFINITY;
-  for (int s = lane; s < mr.z; s += 32) mx = fmaxf(mx, part_ml[(first + s * step) * 2]);
+  float m = -INFINITY, l = 0.f;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int s0 = warp; s0 < mr.z; s0 += 4 * kMergeWarps) {
+    float2 ml[4];
+    float4 v[4][2];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const float off = mx == -INFINITY ? 0.f : mx;
-  float lsum = 0.f;
-  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};  // head_dim <= 256
-  for (int s0 = 0; s0 < mr.z; s0 += 32) {
-    const int n = min(32, mr.z - s0);
-    float w = 0.f;
-    if (lane < n) {
-      const float2 ml = *reinterpret_cast<const float2*>(part_ml + (first + (s0 + lane) * step) * 2);
-      w = exp2f(ml.x - off);
-      lsum += ml.y * w;
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i * kMergeWarps;
+      ml[i] = make_float2(-INFINITY, 0.f);
+      v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s < mr.z) {
+        ml[i] = __ldg(reinterpret_cast<const float2*>(part_ml + (first + s * step) * 2));
+        const float4* po = reinterpret_cast<const float4*>(part_o + (first + s * step) * head_dim);
+        if (lane * 4 < head_dim) v[i][0] = __ldg(po + lane);
+        if (lane * 4 + 128 < head_dim) v[i][1] = __ldg(po + lane + 32);
+      }
     }
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      const float4* po = reinterpret_cast<const float4*>(part_o + (first + (s0 + s) * step) * head_dim);
+    const float mx = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+    const float off = mx == -INFINITY ? 0.f : mx;
+    const float keep = exp2f(m - off);
+    m = mx;
+    l *= keep;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) { acc[k].x *= keep; acc[k].y *= keep; acc[k].z *= keep; acc[k].w *= keep; }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float w = exp2f(ml[i].x - off);
+      l = fmaf(ml[i].y, w, l);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if ((lane + 32 * k) * 4 < head_dim) {
-          const float4 v = __ldg(po + lane + 32 * k);
-          acc[k].x = fmaf(ws, v.x, acc[k].x); acc[k].y = fmaf(ws, v.y, acc[k].y);
-          acc[k].z = fmaf(ws, v.z, acc[k].z); acc[k].w = fmaf(ws, v.w, acc[k].w);
-        }
+        acc[k].x = fmaf(w, v[i][k].x, acc[k].x); acc[k].y = fmaf(w, v[i][k].y, acc[k].y);
+        acc[k].z = fmaf(w, v[i][k].z, acc[k].z); acc[k].w = fmaf(w, v[i][k].w, acc[k].w);
       }
     }
   }
+  s_acc[warp][lane] = acc[0];
+  s_acc[warp][lane + 32] = acc[1];
+  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+  __syncthreads();
+  const int d = threadIdx.x;
+  float mx = -INFINITY, lsum = 0.f, res = 0.f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
-  const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-  T* dst = out + (int64_t)mr.x * out_stride + (int64_t)qh * head_dim;
+  for (int w = 0; w < kMergeWarps; ++w) mx = fmaxf(mx, s_m[w]);
+  const float off = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int d = (lane + 32 * k) * 4;
-    if (d < head_dim) {
-      dst[d] = from_f32<T>(acc[k].x * inv); dst[d + 1] = from_f32<T>(acc[k].y * inv);
-      dst[d + 2] = from_f32<T>(acc[k].z * inv); dst[d + 3] = from_f32<T>(acc[k].w * inv);
-    }
+  for (int w = 0; w < kMergeWarps; ++w) {
+    const float a = exp2f(s_m[w] - off);
+    lsum = fmaf(s_l[w], a, lsum);
+    res = fmaf(reinterpret_cast<const float*>(s_acc[w])[d], a, res);
   }
-  if (lse != nullptr && lane == 0)
-    lse[(int64_t)mr.x * n_q_heads + qh] = lsum > 0.f ? (mx + log2f(lsum)) * kLn2 : -INFINITY;
+  if (d < head_dim) out[(int64_t)mr.x * out_stride + (int64_t)qh * head_dim + d] = from_f32<T>(lsum == 0.f ? 0.f : res / lsum);
+  if (lse != nullptr && d == 0) lse[(int64_t)mr.x * n_q_heads + qh] = lsum == 0.f ? -INFINITY : (mx + log2f(lsum)) * kLn2;
 }
 
 template <typename T, int DMAX>
@@ -441,7 +453,8 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
   if (need > plan_capacity_i32)
     return fail(DSV_E_WORKSPACE, "chunk_plan: plan needs %lld int32, capacity %lld", (long long)need,
                 (long long)plan_capacity_i32);
-  DSV_REQUIRE(part_rows < (1ll << 31) && n_items * std::max(n_kv_heads * 8, ctas_per_item) < (1ll << 31), "chunk_plan: too many partial states");
+  DSV_REQUIRE(part_rows < (1ll << 31) && n_items * std::max(n_kv_heads * 8, ctas_per_item) < (1ll << 31) &&
+                  merge_rows * n_q_heads < (1ll << 31), "chunk_plan: too many partial states");
   struct Out { int len; int32_t v[6]; };
   std::vector<Out> items;
   items.reserve((size_t)n_items);
@@ -534,7 +547,7 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
   bool tensor = row_blocks > 0 && page_stride == (int64_t)2 * page_size * n_kv_heads * head_dim;
   if (tensor) {
     const int hb = heads_per_cta(n_kv_heads, row_blocks);
-    sp.hb_log2 = ilog2_exact(hb); sp.rw_log2 = ilog2_exact(row_blocks); sp.ps_log2 = ilog2_exact(page_size);
+    sp.hb_log2 = ilog2_exact(hb); sp.ps_log2 = ilog2_exact(page_size);
     tensor = chunk_tma::make_tensor_map(&map, pages_layer, num_pages, page_size, n_kv_heads, head_dim, hb, dtype == DSV_BF16);
   }
   if (tensor) {
@@ -550,16 +563,16 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
   if (e != cudaSuccess) return fail(DSV_E_CUDA, "chunk launch failed: %s", cudaGetErrorString(e));
   if (merge_rows > 0) {
     const int4* rows = reinterpret_cast<const int4*>(plan_dev + plan_host[6]);
-    const unsigned grid = (unsigned)(((int64_t)merge_rows * n_q_heads + 7) / 8);
+    const unsigned grid = (unsigned)merge_rows * (unsigned)n_q_heads;
     switch (dtype) {
       case DSV_F32:
-        chunk_merge_kernel<float><<<grid, 256, 0, st>>>(rows, merge_rows, p.part_o, p.part_ml, (float*)out, lse, out_stride_tok, n_q_heads, head_dim);
+        chunk_merge_kernel<float><<<grid, kMergeWarps * 32, 0, st>>>(rows, p.part_o, p.part_ml, (float*)out, lse, out_stride_tok, n_q_heads, head_dim);
         break;
       case DSV_F16:
-        chunk_merge_kernel<__half><<<grid, 256, 0, st>>>(rows, merge_rows, p.part_o, p.part_ml, (__half*)out, lse, out_stride_tok, n_q_heads, head_dim);
+        chunk_merge_kernel<__half><<<grid, kMergeWarps * 32, 0, st>>>(rows, p.part_o, p.part_ml, (__half*)out, lse, out_stride_tok, n_q_heads, head_dim);
         break;
       default:
-        chunk_merge_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(rows, merge_rows, p.part_o, p.part_ml, (__nv_bfloat16*)out, lse, out_stride_tok, n_q_heads, head_dim);
+        chunk_merge_kernel<__nv_bfloat16><<<grid, kMergeWarps * 32, 0, st>>>(rows, p.part_o, p.part_ml, (__nv_bfloat16*)out, lse, out_stride_tok, n_q_heads, head_dim);
     }
     DSV_CUDA(cudaGetLastError());
   }

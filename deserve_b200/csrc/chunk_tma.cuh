@@ -2,7 +2,7 @@
 //
 // A CTA owns one item of the plan for `hb` kv heads: 8 consumer warps and a producer warp, 1 CTA per SM,
 // a 3-deep ring of 512 * D bytes per stage (128 (head, token) rows of K and of V). The warps are split over
-// heads first, then over 16-row blocks of the tile (rw of them), then over 16-token groups of a stage:
+// heads first, then over the item's 16-row blocks (rw of them), then over 16-token groups of a stage (ts):
 // hb * rw * ts = 8. A K/V tile is read from HBM once for all rows; each row block reads it from shared
 // memory again, which costs rw * 23 bytes per clock and SM at full HBM speed, of 128 available.
 // Per 16 tokens and 16 rows: S = Q K^T as 16 mma.sync.m16n8k16, causal / length mask where a row's limit
@@ -19,6 +19,7 @@ constexpr int kConsumerThreads = kConsumerWarps * 32;
 constexpr int kThreads = kConsumerThreads + 32;
 constexpr int kStages = 3;
 constexpr int kSpinLimit = 1 << 21;
+constexpr float kGrow = 8.f;  // log2 units
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
@@ -110,7 +111,7 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x on the special-function 
 }
 
 struct Split {
-  int hb_log2, rw_log2, ps_log2;  // kv heads of a CTA, 16-row blocks of a tile, page size
+  int hb_log2, ps_log2;  // kv heads of a CTA, page size
 };
 
 template <typename T, int D>
@@ -129,7 +130,6 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hb_log = sp.hb_log2, hb = 1 << hb_log;
-  const int rw = 1 << sp.rw_log2, ts = kConsumerWarps >> (hb_log + sp.rw_log2);
   const int ng = kConsumerWarps >> hb_log, ttok = 16 * ng;  // 16-token groups and tokens of a stage
   const int ps_log = sp.ps_log2, ps = 1 << ps_log;
   const int bt_log = min(ps_log, 4), bt = 1 << bt_log;      // tokens per TMA box
@@ -145,7 +145,11 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
     return;
   }
   const int n_tiles = (it.tok_end - it.tok_begin + ttok - 1) / ttok;
-  const int live_blocks = min(rw, (it.n_rows + 15) >> 4);
+  // The item's own row blocks (a request with one new token needs one, whatever the plan's tile holds):
+  // the warps that are left over split the 16-token groups of a stage. A warp has rw groups per stage.
+  const int live_blocks = (it.n_rows + 15) >> 4;
+  const int rw_log = live_blocks <= 1 ? 0 : live_blocks <= 2 ? 1 : live_blocks <= 4 ? 2 : 3;
+  const int rw = 1 << rw_log, ts = kConsumerWarps >> (hb_log + rw_log);
 
   if (tid == 0) {
 #pragma unroll
@@ -191,7 +195,7 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
 
   // ============================ consumer warps ===========================================
   const int g = lane >> 2, tg = lane & 3;
-  const int head_local = warp & (hb - 1), block = (warp >> hb_log) & (rw - 1), sub = warp >> (hb_log + sp.rw_log2);
+  const int head_local = warp & (hb - 1), block = (warp >> hb_log) & (rw - 1), sub = warp >> (hb_log + rw_log);
   const int kv_head = kv_group * hb + head_local;
   const int r0 = block * 16 + g, r1 = r0 + 8;  // this lane's rows
   const int t_r0 = r0 / G, t_r1 = r1 / G;
@@ -230,12 +234,146 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
   const int k_tl = lr + ((lm >> 1) << 3), k_cx = lm & 1;
   const int v_tl = lr + ((lm & 1) << 3), v_cx = lm >> 1;
   auto row_of = [&](int tl, int dh) { return (((tl >> bt_log) * DH + dh) * hb + head_local) * bt + (tl & (bt - 1)); };
-  int k_row[DH], v_row[DH];
+  // Offset of this lane's first 16-byte chunk; the chunk index enters by XOR (128-byte swizzle), and chunk 2 k + cx
+  // differs from chunk cx in the bits of 32 k, so a step's addresses are offset ^ (32 k).
+  uint32_t k_off[DH], v_off[DH];
 #pragma unroll
   for (int dh = 0; dh < DH; ++dh) {
-    k_row[dh] = row_of(k_tl, dh);
-    v_row[dh] = row_of(v_tl, dh);
+    const int kr = row_of(k_tl, dh), vr = row_of(v_tl, dh);
+    k_off[dh] = kr * 128 + ((k_cx ^ (kr & 7)) << 4);
+    v_off[dh] = HALF + vr * 128 + ((v_cx ^ (vr & 7)) << 4);
   }
+
+  // One step: NG groups of 16 tokens (32 where a warp has more than one group: four independent chains
+  // of S products, one maximum and one rescale test for all).
+  auto step = [&](auto ng_tag, const int stage, const int grp, const int wt0) {
+    constexpr int NG = decltype(ng_tag)::value;
+    const uint32_t kbase = smem_base + stage * STAGE + (uint32_t)(grp * bpg * box_bytes);
+    const uint32_t vbase = kbase + HALF;
+    const uint32_t group_bytes = (uint32_t)(bpg * box_bytes);
+    const bool masked = wt0 + 16 * NG - 1 > lim_first;
+    bool poisoned = false;  // V of a token that some row does not see is not a number
+    if (masked) {
+      unsigned char* vg = smem + (vbase - smem_base);
+      const int live = it.tok_end - wt0;
+      if (live < 16 * NG) {
+        // whole boxes were brought (or none): tokens past the end hold whatever was there. Clear them in V so
+        // that 0 * garbage cannot produce a NaN (every warp that reads them writes the same zeros).
+        for (int x = lane; x < (16 * NG - live) * DH * 8; x += 32) {
+          const int ch = x & 7, dh = (x >> 3) % DH, tl = live + (x >> 3) / DH;
+          *reinterpret_cast<uint4*>(vg + (tl >> 4) * group_bytes + row_of(tl & 15, dh) * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+      }
+      for (int x = lane; x < 16 * NG * DH * 8; x += 32) {
+        const int ch = x & 7, dh = (x >> 3) % DH, tl = (x >> 3) / DH;
+        const uint4 v = *reinterpret_cast<const uint4*>(vg + (tl >> 4) * group_bytes + row_of(tl & 15, dh) * 128 + ch * 16);
+        poisoned |= (not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w)) != 0;
+      }
+      poisoned = __any_sync(0xffffffffu, poisoned);
+    }
+    float s[2 * NG][4];  // [8-token column block][row g: 2 tokens, row g + 8: 2 tokens]
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        uint32_t b[4];
+        ldmatrix_x4(b, (kbase + i * group_bytes + k_off[kk >> 2]) ^ ((kk & 3) << 5));
+        mma16816<T>(s[2 * i], qa[kk], b[0], b[1]);
+        mma16816<T>(s[2 * i + 1], qa[kk], b[2], b[3]);
+      }
+    }
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 2 * NG; ++i) {
+        const int c = wt0 + 8 * i + 2 * tg;
+        if (c > lim0) s[i][0] = -INFINITY;
+        if (c + 1 > lim0) s[i][1] = -INFINITY;
+        if (c > lim1) s[i][2] = -INFINITY;
+        if (c + 1 > lim1) s[i][3] = -INFINITY;
+      }
+    }
+    float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i) {
+      mx0 = fmaxf(mx0, fmaxf(s[i][0], s[i][1]));
+      mx1 = fmaxf(mx1, fmaxf(s[i][2], s[i][3]));
+    }
+    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+    // The reference maximum moves only when a row maximum outgrew it by 2^8 (P stays below 2^8, its rounding is
+    // relative), so O is rescaled a few times per request instead of at every new maximum.
+    const float t0m = mx0 * sc, t1m = mx1 * sc;
+    const bool grow0 = t0m > m0 + kGrow || (m0 == -INFINITY && t0m > m0), grow1 = t1m > m1 + kGrow || (m1 == -INFINITY && t1m > m1);
+    if (__any_sync(0xffffffffu, grow0 || grow1)) {
+      const float f0 = grow0 ? ex2(m0 - t0m) : 1.f, f1 = grow1 ? ex2(m1 - t1m) : 1.f;
+      m0 = grow0 ? t0m : m0;
+      m1 = grow1 ? t1m : m1;
+      l0 *= f0;
+      l1 *= f1;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
+    }
+    const float off0 = m0 == -INFINITY ? 0.f : -m0, off1 = m1 == -INFINITY ? 0.f : -m1;
+    // P is rounded to the 16-bit type of V, as the tensor core needs it; the sum l is not
+    uint32_t pa[NG][4];
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i) {
+      const float a = ex2(fmaf(s[i][0], sc, off0)), b = ex2(fmaf(s[i][1], sc, off0));
+      const float c = ex2(fmaf(s[i][2], sc, off1)), d = ex2(fmaf(s[i][3], sc, off1));
+      l0 += a + b;
+      l1 += c + d;
+      pa[i >> 1][(i & 1) * 2] = pack2<T>(a, b);
+      pa[i >> 1][(i & 1) * 2 + 1] = pack2<T>(c, d);
+    }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+#pragma unroll
+      for (int jn = 0; jn < D / 16; ++jn) {
+        uint32_t v[4];
+        ldmatrix_x4_trans(v, (kbase + i * group_bytes + v_off[jn >> 2]) ^ ((jn & 3) << 5));
+        if (poisoned) {  // a zero weight must not meet an infinity: such values are added below
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] &= ~not_finite<T>(v[k]);
+        }
+        mma16816<T>(o[2 * jn], pa[i], v[0], v[1]);
+        mma16816<T>(o[2 * jn + 1], pa[i], v[2], v[3]);
+      }
+    }
+    if (poisoned) {  // the rest, token by token, only into the rows that see it
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+#pragma unroll 1
+        for (int tl = 0; tl < 16; ++tl) {
+          const int from = g * 4 + ((tl & 7) >> 1);
+          const float2 w0 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[i][0] : pa[i][2], from));
+          const float2 w1 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[i][1] : pa[i][3], from));
+          const float a = (tl & 1) ? w0.y : w0.x, b = (tl & 1) ? w1.y : w1.x;
+          const bool see0 = wt0 + 16 * i + tl <= lim0, see1 = wt0 + 16 * i + tl <= lim1;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            const int d = j * 8 + tg * 2, row = row_of(tl, d >> 6);
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + (vbase - smem_base) + i * group_bytes + row * 128 +
+                                                                  ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2);
+            const uint32_t odd = not_finite<T>(w);
+            const float2 v = unpack2<T>(w);
+            if (odd & 0xffffu) {
+              if (see0) o[j][0] = fmaf(a, v.x, o[j][0]);
+              if (see1) o[j][2] = fmaf(b, v.x, o[j][2]);
+            }
+            if (odd >> 16) {
+              if (see0) o[j][1] = fmaf(a, v.y, o[j][1]);
+              if (see1) o[j][3] = fmaf(b, v.y, o[j][3]);
+            }
+          }
+        }
+      }
+    }
+  };
 
   bool ok = true;
   if (block < live_blocks) {
@@ -245,114 +383,13 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
         ok = false;
         break;
       }
-      for (int grp = sub; grp < ng; grp += ts) {
-        const int wt0 = it.tok_begin + tile * ttok + 16 * grp;
-        if (wt0 > lim_last) break;  // nothing here that a row of this block sees
-        const uint32_t kbase = smem_base + s * STAGE + (uint32_t)(grp * bpg * box_bytes);
-        const uint32_t vbase = kbase + HALF;
-        const bool masked = wt0 + 15 > lim_first;
-        bool poisoned = false;  // V of a token that some row does not see is not a number
-        if (masked) {
-          unsigned char* vg = smem + (vbase - smem_base);
-          const int live = it.tok_end - wt0;
-          if (live < 16) {
-            // whole boxes were brought: tokens past the end hold whatever the pool holds there. Clear them in
-            // V so that 0 * garbage cannot produce a NaN (every warp that reads them writes the same zeros).
-            for (int x = lane; x < (16 - live) * DH * 8; x += 32) {
-              const int ch = x & 7, dh = (x >> 3) % DH, tl = live + (x >> 3) / DH;
-              *reinterpret_cast<uint4*>(vg + row_of(tl, dh) * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
-            }
-            __syncwarp();
-          }
-          for (int x = lane; x < 16 * DH * 8; x += 32) {
-            const int ch = x & 7, dh = (x >> 3) % DH, tl = (x >> 3) / DH;
-            const uint4 v = *reinterpret_cast<const uint4*>(vg + row_of(tl, dh) * 128 + ch * 16);
-            poisoned |= (not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w)) != 0;
-          }
-          poisoned = __any_sync(0xffffffffu, poisoned);
-        }
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) {
-          const int cidx = 2 * kk + k_cx, row = k_row[cidx >> 3];
-          uint32_t b[4];
-          ldmatrix_x4(b, kbase + row * 128 + (((cidx & 7) ^ (row & 7)) << 4));
-          mma16816<T>(s0, qa[kk], b[0], b[1]);
-          mma16816<T>(s1, qa[kk], b[2], b[3]);
-        }
-        if (masked) {
-          const int c0 = wt0 + 2 * tg;
-          if (c0 > lim0) s0[0] = -INFINITY;
-          if (c0 + 1 > lim0) s0[1] = -INFINITY;
-          if (c0 + 8 > lim0) s1[0] = -INFINITY;
-          if (c0 + 9 > lim0) s1[1] = -INFINITY;
-          if (c0 > lim1) s0[2] = -INFINITY;
-          if (c0 + 1 > lim1) s0[3] = -INFINITY;
-          if (c0 + 8 > lim1) s1[2] = -INFINITY;
-          if (c0 + 9 > lim1) s1[3] = -INFINITY;
-        }
-        float mx0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1]));
-        float mx1 = fmaxf(fmaxf(s0[2], s0[3]), fmaxf(s1[2], s1[3]));
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-        const float mn0 = fmaxf(m0, mx0 * sc), mn1 = fmaxf(m1, mx1 * sc);
-        const float off0 = mn0 == -INFINITY ? 0.f : mn0, off1 = mn1 == -INFINITY ? 0.f : mn1;
-        if (__any_sync(0xffffffffu, mn0 > m0 || mn1 > m1)) {  // rescale only when a row maximum moved
-          const float f0 = ex2(m0 - off0), f1 = ex2(m1 - off1);
-          l0 *= f0;
-          l1 *= f1;
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
-        }
-        m0 = mn0;
-        m1 = mn1;
-        const float p00 = ex2(fmaf(s0[0], sc, -off0)), p01 = ex2(fmaf(s0[1], sc, -off0));
-        const float p10 = ex2(fmaf(s1[0], sc, -off0)), p11 = ex2(fmaf(s1[1], sc, -off0));
-        const float q00 = ex2(fmaf(s0[2], sc, -off1)), q01 = ex2(fmaf(s0[3], sc, -off1));
-        const float q10 = ex2(fmaf(s1[2], sc, -off1)), q11 = ex2(fmaf(s1[3], sc, -off1));
-        l0 += (p00 + p01) + (p10 + p11);
-        l1 += (q00 + q01) + (q10 + q11);
-        // P is rounded to the 16-bit type of V, as the tensor core needs it; the sum l is not
-        uint32_t pa[4] = {pack2<T>(p00, p01), pack2<T>(q00, q01), pack2<T>(p10, p11), pack2<T>(q10, q11)};
-#pragma unroll
-        for (int jn = 0; jn < D / 16; ++jn) {
-          const int cidx = 2 * jn + v_cx, row = v_row[cidx >> 3];
-          uint32_t v[4];
-          ldmatrix_x4_trans(v, vbase + row * 128 + (((cidx & 7) ^ (row & 7)) << 4));
-          if (poisoned) {  // a zero weight must not meet an infinity: such values are added below
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] &= ~not_finite<T>(v[i]);
-          }
-          mma16816<T>(o[2 * jn], pa, v[0], v[1]);
-          mma16816<T>(o[2 * jn + 1], pa, v[2], v[3]);
-        }
-        if (poisoned) {  // the rest, token by token, only into the rows that see it
-          for (int tl = 0; tl < 16; ++tl) {
-            const int from = g * 4 + ((tl & 7) >> 1);
-            const float2 w0 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[0] : pa[2], from));
-            const float2 w1 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[1] : pa[3], from));
-            const float a = (tl & 1) ? w0.y : w0.x, b = (tl & 1) ? w1.y : w1.x;
-            const bool see0 = wt0 + tl <= lim0, see1 = wt0 + tl <= lim1;
-#pragma unroll
-            for (int j = 0; j < D / 8; ++j) {
-              const int d = j * 8 + tg * 2, row = row_of(tl, d >> 6);
-              const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + (vbase - smem_base) + row * 128 +
-                                                                    ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2);
-              const uint32_t odd = not_finite<T>(w);
-              const float2 v = unpack2<T>(w);
-              if (odd & 0xffffu) {
-                if (see0) o[j][0] = fmaf(a, v.x, o[j][0]);
-                if (see1) o[j][2] = fmaf(b, v.x, o[j][2]);
-              }
-              if (odd >> 16) {
-                if (see0) o[j][1] = fmaf(a, v.y, o[j][1]);
-                if (see1) o[j][3] = fmaf(b, v.y, o[j][3]);
-              }
-            }
-          }
-        }
+      // this warp's groups of the stage: [sub * rw, sub * rw + rw); nothing behind lim_last is seen by its rows
+      const int t0 = it.tok_begin + tile * ttok + 16 * (sub << rw_log);
+      if (rw == 1) {
+        if (t0 <= lim_last) step(std::integral_constant<int, 1>{}, s, sub, t0);
+      } else {
+        for (int i = 0; i < rw && t0 + 16 * i <= lim_last; i += 2)
+          step(std::integral_constant<int, 2>{}, s, (sub << rw_log) + i, t0 + 16 * i);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_empty + 8 * s);  // this warp is done with the stage
@@ -386,7 +423,7 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
   const int quads = D / 4;
   for (int x = tid; x < hb * it.n_rows * quads; x += kConsumerThreads) {
     const int d = (x % quads) * 4, y = x / quads, r = y % it.n_rows, hl = y / it.n_rows;
-    const int w0 = hl + ((r >> 4) << hb_log), step = 1 << (hb_log + sp.rw_log2);
+    const int w0 = hl + ((r >> 4) << hb_log), step = 1 << (hb_log + rw_log);
     float mx = -INFINITY;
     for (int s2 = 0; s2 < ts; ++s2) mx = fmaxf(mx, sc_ml[((w0 + s2 * step) * 16 + (r & 15)) * 2]);
     const float off = mx == -INFINITY ? 0.f : mx;

@@ -19,8 +19,7 @@ namespace {
 
 constexpr int32_t kChunkMagic = 0x44534331;  // "DSC1"
 // header: magic, items, merge rows, q tokens per tile, batch, offset of the items, offset of the merge
-// rows, q heads, kv heads, head_dim, partial rows, page size, dtype, nnz, 16-row blocks of a tile for the
-// tensor-core kernel (0: the shape is not for it), 1 unused
+// rows, q heads, kv heads, head_dim, partial rows, page size, dtype, nnz, kernel, most parts of a tile
 constexpr int kPlanHeader = 16;
 constexpr int kItemInts = 8;  // request, first q token, q tokens, first page, end page, partial row or -1, 2 unused
 constexpr float kLog2e = 1.4426950408889634f;
@@ -80,6 +79,7 @@ __device__ __forceinline__ bool load_item(const ChunkParams& p, int index, Item&
 }  // namespace
 }  // namespace dsv
 #include "chunk_tma.cuh"
+#include "chunk_tc.cuh"
 namespace dsv {
 namespace {
 
@@ -241,29 +241,32 @@ chunk_simple_kernel(const ChunkParams p, int row_blocks) {
 }
 
 // ---- merge of the parts of a split tile -----------------------------------------------------------
-// One CTA per (split q row, q head): its 8 warps take the parts round robin, 4 in flight each, and are
-// joined in shared memory. merge row: {q row, first partial row, parts, partial rows per part}.
-// (One warp per row and head took 11 us for the 74 parts of a 64k-token request, a chain of 19 loads.)
-constexpr int kMergeWarps = 8;
+// W warps per (split q row, q head) take its parts round robin, 4 in flight each, and are joined in shared
+// memory. merge row: {q row, first partial row, parts, partial rows per part}. W = 8 when some row has more
+// than 8 parts (one warp took 11 us for the 74 parts of a 64k-token request, a chain of 19 loads), else 1
+// (8 warps for the 2 parts of each of 37,000 rows took 40 us longer).
+constexpr int kMergeThreads = 256;
 
-template <typename T>
-__global__ void __launch_bounds__(kMergeWarps * 32)
-chunk_merge_kernel(const int4* __restrict__ rows, const float* __restrict__ part_o, const float* __restrict__ part_ml,
+template <typename T, int W>
+__global__ void __launch_bounds__(kMergeThreads)
+chunk_merge_kernel(const int4* __restrict__ rows, int units, const float* __restrict__ part_o, const float* __restrict__ part_ml,
                    T* __restrict__ out, float* __restrict__ lse, int64_t out_stride, int n_q_heads, int head_dim) {
-  __shared__ float4 s_acc[kMergeWarps][64];  // head_dim <= 256
-  __shared__ float s_m[kMergeWarps], s_l[kMergeWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int4 mr = __ldg(rows + blockIdx.x / n_q_heads);
-  const int qh = (int)(blockIdx.x % n_q_heads);
+  constexpr int U = kMergeThreads / 32 / W;  // units of a CTA
+  __shared__ float4 s_acc[U][W][64];  // head_dim <= 256
+  __shared__ float s_m[U][W], s_l[U][W];
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % W, sub = (threadIdx.x >> 5) / W;
+  const int unit = min((int)blockIdx.x * U + sub, units - 1);  // the last CTA may do a unit twice
+  const int4 mr = __ldg(rows + unit / n_q_heads);
+  const int qh = unit % n_q_heads;
   const int64_t first = (int64_t)mr.y * n_q_heads + qh, step = (int64_t)mr.w * n_q_heads;
   float m = -INFINITY, l = 0.f;
   float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-  for (int s0 = warp; s0 < mr.z; s0 += 4 * kMergeWarps) {
+  for (int s0 = warp; s0 < mr.z; s0 += 4 * W) {
     float2 ml[4];
     float4 v[4][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int s = s0 + i * kMergeWarps;
+      const int s = s0 + i * W;
       ml[i] = make_float2(-INFINITY, 0.f);
       v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (s < mr.z) {
@@ -291,23 +294,32 @@ chunk_merge_kernel(const int4* __restrict__ rows, const float* __restrict__ part
       }
     }
   }
-  s_acc[warp][lane] = acc[0];
-  s_acc[warp][lane + 32] = acc[1];
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+  s_acc[sub][warp][lane] = acc[0];
+  s_acc[sub][warp][lane + 32] = acc[1];
+  if (lane == 0) { s_m[sub][warp] = m; s_l[sub][warp] = l; }
   __syncthreads();
-  const int d = threadIdx.x;
-  float mx = -INFINITY, lsum = 0.f, res = 0.f;
+  float mx = -INFINITY, lsum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) mx = fmaxf(mx, s_m[w]);
+  for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[sub][w]);
   const float off = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) {
-    const float a = exp2f(s_m[w] - off);
-    lsum = fmaf(s_l[w], a, lsum);
-    res = fmaf(reinterpret_cast<const float*>(s_acc[w])[d], a, res);
+  for (int w = 0; w < W; ++w) lsum = fmaf(s_l[sub][w], exp2f(s_m[sub][w] - off), lsum);
+  for (int d = warp * 32 + lane; d < head_dim; d += W * 32) {
+    float res = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) res = fmaf(reinterpret_cast<const float*>(s_acc[sub][w])[d], exp2f(s_m[sub][w] - off), res);
+    out[(int64_t)mr.x * out_stride + (int64_t)qh * head_dim + d] = from_f32<T>(lsum == 0.f ? 0.f : res / lsum);
   }
-  if (d < head_dim) out[(int64_t)mr.x * out_stride + (int64_t)qh * head_dim + d] = from_f32<T>(lsum == 0.f ? 0.f : res / lsum);
-  if (lse != nullptr && d == 0) lse[(int64_t)mr.x * n_q_heads + qh] = lsum == 0.f ? -INFINITY : (mx + log2f(lsum)) * kLn2;
+  if (lse != nullptr && warp == 0 && lane == 0)
+    lse[(int64_t)mr.x * n_q_heads + qh] = lsum == 0.f ? -INFINITY : (mx + log2f(lsum)) * kLn2;
+}
+
+template <typename T>
+void launch_merge(const int4* rows, int units, bool many, const ChunkParams& p, cudaStream_t st) {
+  if (many)
+    chunk_merge_kernel<T, 8><<<units, kMergeThreads, 0, st>>>(rows, units, p.part_o, p.part_ml, (T*)p.out, p.lse, p.out_stride, p.n_q_heads, p.head_dim);
+  else
+    chunk_merge_kernel<T, 1><<<(units + 7) / 8, kMergeThreads, 0, st>>>(rows, units, p.part_o, p.part_ml, (T*)p.out, p.lse, p.out_stride, p.n_q_heads, p.head_dim);
 }
 
 template <typename T, int DMAX>
@@ -327,9 +339,10 @@ int ilog2_exact(int x) {  // log2 of a power of two, -1 otherwise
   while ((1 << l) < x) ++l;
   return l;
 }
-// kv heads of a CTA of the tensor-core kernel: 8 warps over heads and row blocks
-int heads_per_cta(int n_kv_heads, int row_blocks) {
-  int hb = 8 / row_blocks;
+enum : int { kSimple = 0, kMma = 1, kTc = 2 };  // kernel of a plan
+// kv heads of a CTA of the mma.sync kernel
+int heads_per_cta(int n_kv_heads) {
+  int hb = 8;
   while (hb > 1 && n_kv_heads % hb != 0) hb >>= 1;
   return hb;
 }
@@ -342,6 +355,21 @@ cudaError_t launch_tma(const CUtensorMap& map, const ChunkParams& p, const chunk
   if (e != cudaSuccess) return e;
   kernel<<<(unsigned)(n_items * (p.n_kv_heads >> sp.hb_log2)), chunk_tma::kThreads, smem, st>>>(map, p, sp);
   return cudaGetLastError();
+}
+
+template <typename T, int D, bool MERGED>
+cudaError_t launch_tc(const chunk_tc::Maps& m, const ChunkParams& p, int ps_log2, int n_items, cudaStream_t st) {
+  const size_t smem = (size_t)2 * 128 * D * 2 + (size_t)(2 + chunk_tc::kVStages) * chunk_tc::kBN * D * 2 + 256 + 1024;
+  auto kernel = chunk_tc::chunk_tc_kernel<T, D, MERGED>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<(unsigned)(n_items * p.n_kv_heads), chunk_tc::kThreads, smem, st>>>(m.q, m.k, m.v, p, ps_log2);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_tc_d(const chunk_tc::Maps& m, const ChunkParams& p, int ps_log2, int n_items, cudaStream_t st) {
+  if (p.head_dim == 64) return launch_tc<T, 64, false>(m, p, ps_log2, n_items, st);
+  return p.page_size >= 16 ? launch_tc<T, 128, true>(m, p, ps_log2, n_items, st) : launch_tc<T, 128, false>(m, p, ps_log2, n_items, st);
 }
 
 template <typename T>
@@ -371,20 +399,15 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
   DSV_REQUIRE(page_size > 0, "chunk_plan: page_size must be positive");
   if (sm_count <= 0) sm_count = 148;
   const int G = n_q_heads / n_kv_heads;
-  // Rows of a q tile: all new tokens of a request where they fit, so that its K/V is read once. The
-  // tensor-core kernel takes up to 128 rows (8 warps of 16).
+  // Rows of a q tile: all new tokens of a request where they fit, so that its K/V is read once.
   const bool tensor = dtype != DSV_F32 && (head_dim == 64 || head_dim == 128) && G <= 128 && ilog2_exact(page_size) >= 3;
   int most = 0;
   for (int i = 0; i < batch; ++i) most = std::max(most, qo_indptr_host[i + 1] - qo_indptr_host[i]);
-  int row_blocks = 0;
-  if (tensor) {
-    row_blocks = 1;
-    while (row_blocks < 8 && (int64_t)row_blocks * 16 < (int64_t)most * G) row_blocks *= 2;
-    while (row_blocks * 16 < G) row_blocks *= 2;
-  }
-  const int tile = std::max(1, (tensor ? row_blocks * 16 : kSimpleRows) / G);
-  const int ctas_per_item = tensor ? n_kv_heads / heads_per_cta(n_kv_heads, row_blocks)
-                                   : n_kv_heads * ((tile * G + kSimpleRows - 1) / kSimpleRows);
+  // up to 16 rows: mma.sync, all heads of a page in one CTA; more: tcgen05, one kv head per CTA
+  const int kind = !tensor ? kSimple : (int64_t)most * G <= 16 ? kMma : kTc;
+  const int tile = std::max(1, kind == kMma ? 16 / G : kind == kTc ? (most > 128 / G ? 2 * (128 / G) : 128 / G) : kSimpleRows / G);
+  const int ctas_per_item = kind == kMma ? n_kv_heads / heads_per_cta(n_kv_heads)
+                            : kind == kTc ? n_kv_heads : n_kv_heads * ((tile * G + kSimpleRows - 1) / kSimpleRows);
 
   struct Tile { int req, q0, nq, pages; };
   std::vector<Tile> tiles;
@@ -414,10 +437,12 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
     return k;
   };
   const double page_cost = (double)2 * page_size * n_kv_heads * head_dim * elem_size(dtype) / ctas_per_item;
-  const double overhead = 128.0 * 1024, merge_cost = 192.0 * 1024;
-  const int64_t slots = (int64_t)sm_count * (tensor ? 1 : 4);
+  // in bytes of streaming; the general kernel is bound by arithmetic: there a CTA's cost is counted in tokens
+  const double unit = kind == kSimple ? page_cost / page_size * 32 : 128.0 * 1024;
+  const double overhead = unit, merge_cost = 1.5 * unit;
+  const int64_t slots = (int64_t)sm_count * (kind == kSimple ? 4 : 1);
   const int64_t most_items = std::max<int64_t>((int64_t)4 * sm_count, (int64_t)tiles.size());
-  const int min_chunk = std::max(1, 64 / page_size);
+  const int min_chunk = std::max(1, (kind == kSimple ? 32 : 128) / page_size);
   int chunk = std::max(min_chunk, max_pages);
   double best = -1.0;
   auto consider = [&](int64_t c64) {
@@ -442,9 +467,10 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
     }
   }
   const int64_t n_items = count_items(chunk);
-  int64_t merge_rows = 0, part_rows = 0;
+  int64_t merge_rows = 0, part_rows = 0, most_parts = 0;
   for (const Tile& t : tiles) {
     const int64_t parts = std::max(1, (t.pages + chunk - 1) / chunk);
+    most_parts = std::max(most_parts, parts);
     if (parts > 1) { merge_rows += t.nq; part_rows += parts * t.nq; }
   }
   const int64_t need = kPlanHeader + kItemInts * n_items + 4 * merge_rows;
@@ -483,7 +509,7 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
   plan_host[4] = batch; plan_host[5] = kPlanHeader; plan_host[6] = (int32_t)(kPlanHeader + kItemInts * n_items);
   plan_host[7] = n_q_heads; plan_host[8] = n_kv_heads; plan_host[9] = head_dim; plan_host[10] = (int32_t)part_rows;
   plan_host[11] = page_size; plan_host[12] = dtype; plan_host[13] = batch > 0 ? qo_indptr_host[batch] : 0;
-  plan_host[14] = row_blocks;
+  plan_host[14] = kind; plan_host[15] = (int32_t)most_parts;
   for (int64_t k = 0; k < n_items; ++k) {
     int32_t* it = plan_host + kPlanHeader + kItemInts * k;
     for (int j = 0; j < 6; ++j) it[j] = items[k].v[j];
@@ -540,21 +566,26 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
   p.num_pages = (int)num_pages; p.nnz = nnz; p.scale_log2 = sm_scale * kLog2e; p.status = device_status_ptr();
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
-  const int row_blocks = plan_host[14];
-  DSV_REQUIRE(row_blocks >= 0 && row_blocks <= 8, "chunk: corrupt plan");
-  chunk_tma::Split sp = {};
-  CUtensorMap map;
-  bool tensor = row_blocks > 0 && page_stride == (int64_t)2 * page_size * n_kv_heads * head_dim;
-  if (tensor) {
-    const int hb = heads_per_cta(n_kv_heads, row_blocks);
-    sp.hb_log2 = ilog2_exact(hb); sp.ps_log2 = ilog2_exact(page_size);
-    tensor = chunk_tma::make_tensor_map(&map, pages_layer, num_pages, page_size, n_kv_heads, head_dim, hb, dtype == DSV_BF16);
-  }
-  if (tensor) {
+  const int ps_log2 = ilog2_exact(page_size);
+  // a pool with gaps between its pages has no tensor map: the general kernel takes any plan
+  const int kind = page_stride == (int64_t)2 * page_size * n_kv_heads * head_dim ? plan_host[14] : kSimple;
+  DSV_REQUIRE(kind >= kSimple && kind <= kTc && (kind == kSimple || (ps_log2 >= 3 && dtype != DSV_F32 && (head_dim == 64 || head_dim == 128))),
+              "chunk: corrupt plan");
+  if (kind == kMma) {
+    const int hb = heads_per_cta(n_kv_heads);
+    const chunk_tma::Split sp = {ilog2_exact(hb), ps_log2};
+    CUtensorMap map;
+    if (!chunk_tma::make_tensor_map(&map, pages_layer, num_pages, page_size, n_kv_heads, head_dim, hb, dtype == DSV_BF16))
+      return fail(DSV_E_CUDA, "chunk: tensor map of the pages rejected");
     if (dtype == DSV_F16)
       e = head_dim == 128 ? launch_tma<__half, 128>(map, p, sp, n_items, st) : launch_tma<__half, 64>(map, p, sp, n_items, st);
     else
       e = head_dim == 128 ? launch_tma<__nv_bfloat16, 128>(map, p, sp, n_items, st) : launch_tma<__nv_bfloat16, 64>(map, p, sp, n_items, st);
+  } else if (kind == kTc) {
+    chunk_tc::Maps maps;
+    if (!chunk_tma::encode_tiled_fn() || !chunk_tc::make_maps(chunk_tma::encode_tiled_fn(), maps, p, head_dim == 128 && page_size >= 16, dtype == DSV_BF16))
+      return fail(DSV_E_CUDA, "chunk: tensor maps rejected");
+    e = dtype == DSV_F16 ? launch_tc_d<__half>(maps, p, ps_log2, n_items, st) : launch_tc_d<__nv_bfloat16>(maps, p, ps_log2, n_items, st);
   } else switch (dtype) {
     case DSV_F32: e = launch_simple_d<float>(p, n_items, plan_host[3], st); break;
     case DSV_F16: e = launch_simple_d<__half>(p, n_items, plan_host[3], st); break;
@@ -563,16 +594,12 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
   if (e != cudaSuccess) return fail(DSV_E_CUDA, "chunk launch failed: %s", cudaGetErrorString(e));
   if (merge_rows > 0) {
     const int4* rows = reinterpret_cast<const int4*>(plan_dev + plan_host[6]);
-    const unsigned grid = (unsigned)merge_rows * (unsigned)n_q_heads;
+    const int units = merge_rows * n_q_heads;
+    const bool many = plan_host[15] > 8;
     switch (dtype) {
-      case DSV_F32:
-        chunk_merge_kernel<float><<<grid, kMergeWarps * 32, 0, st>>>(rows, p.part_o, p.part_ml, (float*)out, lse, out_stride_tok, n_q_heads, head_dim);
-        break;
-      case DSV_F16:
-        chunk_merge_kernel<__half><<<grid, kMergeWarps * 32, 0, st>>>(rows, p.part_o, p.part_ml, (__half*)out, lse, out_stride_tok, n_q_heads, head_dim);
-        break;
-      default:
-        chunk_merge_kernel<__nv_bfloat16><<<grid, kMergeWarps * 32, 0, st>>>(rows, p.part_o, p.part_ml, (__nv_bfloat16*)out, lse, out_stride_tok, n_q_heads, head_dim);
+      case DSV_F32: launch_merge<float>(rows, units, many, p, st); break;
+      case DSV_F16: launch_merge<__half>(rows, units, many, p, st); break;
+      default: launch_merge<__nv_bfloat16>(rows, units, many, p, st);
     }
     DSV_CUDA(cudaGetLastError());
   }

@@ -62,7 +62,7 @@ def test_chunk_plan_covers_every_row_and_page_once(dtype, hq, hkv, d, ps, new, p
 
 def test_chunk_plan_spreads_one_request_over_the_gpu():
     plan, _, _ = _plan([5], [4096])
-    assert plan[1] * 8 >= 148
+    assert 140 <= plan[1] * 8 <= 592  # one CTA per item and kv head: about one round of the 148 SMs, at most four
     plan, ws, _ = _plan([4] * 600, [40] * 600)
     assert ws == 0  # enough requests: nothing is split
 

@@ -429,8 +429,8 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
     }
   }
   // Part length: compared on a model of the launch. A CTA costs the bytes it streams plus a fixed
-  // overhead (fill and drain of its ring, q, the partial state), a launch that splits anything a merge.
-  // CTAs fill `slots` at a time; the last round is half empty on average.
+  // overhead (fill and drain of its ring, q), a launch that splits anything a merge and the partial
+  // states' way to memory and back. CTAs fill `slots` at a time; the last round is half empty on average.
   auto count_items = [&](int c) {
     int64_t k = 0;
     for (const Tile& t : tiles) k += std::max(1, (t.pages + c - 1) / c);
@@ -453,7 +453,14 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
     const double longest = std::min(c, max_pages) * page_cost + overhead;
     double cost = ctas <= slots ? longest
                                 : std::max(longest, ((double)total_pages * ctas_per_item * page_cost + (double)ctas * overhead) / (double)slots) + 0.5 * longest;
-    if (k > (int64_t)tiles.size()) cost += merge_cost;
+    if (k > (int64_t)tiles.size()) {
+      int64_t rows = 0;
+      for (const Tile& t : tiles) {
+        const int64_t parts = std::max(1, (t.pages + c - 1) / c);
+        if (parts > 1) rows += parts * t.nq;
+      }
+      cost += merge_cost + 2.0 * (double)rows * n_q_heads * (head_dim + 2) * sizeof(float) / sm_count;
+    }
     if (best < 0.0 || cost < best) { best = cost; chunk = c; }
   };
   if (!tiles.empty()) {

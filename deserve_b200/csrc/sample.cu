@@ -26,15 +26,17 @@
 namespace dsv {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kMaxCtas = 8;  // of a cluster (the portable limit)
+constexpr int kMaxCtas = 8;   // of a cluster (the portable limit)
+constexpr int kMaxWarps = 16;
+constexpr int kList = 256;    // members of the border's bin that are ranked directly
 constexpr int kMaxVocab = 1 << 18, kIndexBits = 18;
 constexpr double kOne = 17592186044416.0;          // 2^44: the fixed-point weight of the largest logit
 constexpr double kProbOne = 1152921504606846976.0;  // 2^60: fixed-point probabilities of the residual
-constexpr double kLowest = -46.0 * 64.0;            // in 1/64 of a factor of two: weights below round to 0
+constexpr float kWindow = 8.f;                      // nats below the top that the first histogram covers
 constexpr int kTable = 64;
 typedef unsigned long long u64;
+constexpr u64 kRaw = 0x4330000000000000ull;  // 2^52 as a double: integers sit behind it
 
 struct SampleParams {
   const void* logits;
@@ -66,11 +68,13 @@ struct Slot {
 struct Shared {
   uint32_t hist_lo[kBins], hist_hi[kBins];
   double table[kTable];  // 2^(j / 64 + 44)
-  Slot slot[24];
-  u64 warp_a[kWarps], warp_b[kWarps];
-  u64 seg[kWarps];  // mass of the warps' segments
-  u64 found;
-  int found_i;
+  Slot slot[32];
+  u64 warp_a[kMaxWarps], warp_b[kMaxWarps];
+  u64 seg[kMaxWarps];    // mass of the warps' segments
+  u64 list[kList];       // this CTA's members of the border's bin
+  u64 all_key[kList], all_w[kList];
+  int n_list;
+  u64 border, kept;
 };
 
 // ---- cluster plumbing ------------------------------------------------------------------------------
@@ -137,174 +141,223 @@ __device__ __forceinline__ u64 rank_key(float l, int index) {
   return ((u64)order_key<T>(l) << kIndexBits) | (u64)(kMaxVocab - 1 - index);
 }
 
-// What is known of a row: its largest logit and the scale of its exponent.
+template <typename T>
+__device__ __forceinline__ float key_value(uint32_t k) {  // the number of an order key
+  if constexpr (std::is_same<T, __half>::value) {
+    return __half2float(__ushort_as_half((unsigned short)((k & 0x8000u) ? k & 0x7fffu : k ^ 0xffffu)));
+  } else {
+    if (sizeof(T) == 2) k = (k & 0x8000u) ? k << 16 : (k << 16) | 0xffffu;
+    return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
+  }
+}
+
+// What is known of a row: its largest logit and the scale of its exponent. Fixed-point weights are
+// 2^44 2^((l c - K) / 64).
 struct RowScale {
-  float top;        // largest logit that is a number
-  double c;         // 64 log2(e) / T
-  float c32;        // log2(e) / T
-  float bin_scale;  // bins per unit of (top - l)
+  float top;     // largest logit that is a number
+  float cutoff;  // entries below have weight 0 (2^-60 and less)
+  float t;       // temperature
+  float c32;     // log2(e) / T
+  double c;      // 64 log2(e) / T
+  double magic;  // 1.5 * 2^52 - K, K = round(top c): added to l c it leaves the rounded l c - K in the low word
+  double one;    // the fixed-point weight of the top: 2^44 2^((top c - K) / 64)
 };
 __device__ __forceinline__ RowScale row_scale(float top, float temperature) {
   RowScale s;
   s.top = top;
-  const double inv = 1.0 / (double)temperature;
-  s.c = 92.332482616893657 * inv;  // 64 / ln 2
+  s.t = fminf(temperature, 1e36f);  // (so that the cutoff below stays finite)
+  const double inv = 1.0 / (double)s.t;
+  // A temperature so small that one unit in the last place of the top already gives weight 0 gives the same weights
+  // as 2^37 / |top|, which keeps the exponents in range.
+  s.c = fmin(92.332482616893657 * inv, 137438953472.0 / fabs((double)top));
   s.c32 = (float)fmin(1.4426950408889634 * inv, 3e38);
-  s.bin_scale = (float)fmin(64.0 * inv, 3e38);  // bins of 1/64: the 32 nats that a 2^-44 weight can lie below the top
+  const float ulp = __uint_as_float(__float_as_uint(fabsf(top)) + 1u) - fabsf(top);
+  s.cutoff = top - fmaxf(64.f * s.t, 2.f * ulp);
+  const double k = rint((double)top * s.c);
+  s.magic = 6755399441055744.0 - k;
+  s.one = kOne * exp2(fma((double)top, s.c, -k) * 0.015625);
   return s;
 }
-// Fixed-point weight: 2^(d / 64), d = 64 log2(e) (l - top) / T = n + r with |r| <= 1/2, from a table of 2^(j / 64)
-// and e^(r ln 2 / 64) to the fourth power (|r ln 2 / 64| < 0.0055: the next term is below 2^-44). Ten FP64
-// instructions; 128,256 entries keep one SM's FP64 units busy for about 11 us, twice what its share of HBM needs.
-__device__ __forceinline__ u64 fixed_weight(float l, const RowScale& s, const Shared& sh) {
-  const double d = ((double)l - (double)s.top) * s.c;
-  const bool any = d >= kLowest;  // NaN and -inf: no weight
-  const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it leaves the rounded integer in the low bits
-  const double m = (any ? d : 0.0) + magic;
-  const int n = __double2loint(m);
-  const double r = (any ? d : 0.0) - (m - magic);
+// Fixed-point weight behind kRaw (subtract it; sums may subtract it once per entry). With l c = N + r, |r| <= 1/2:
+// 2^((N - K) / 64) from a table of 2^(j / 64) and an exponent, e^(r ln 2 / 64) to the fourth power (its argument is
+// below 0.0055: the next term is under 2^-44). Eight FP64 instructions: 128,256 entries keep one SM's FP64 units
+// busy for 8 us, 1.5 times what its share of HBM takes to bring them in 16 bits.
+__device__ __forceinline__ u64 raw_weight(float l, const RowScale& s, const double* __restrict__ table) {
+  const double x = (double)fmaxf(l, s.cutoff);  // NaN and -inf too: weight 0
+  const double m = fma(x, s.c, s.magic);
+  const double r = fma(x, s.c, s.magic - m);
   constexpr double a = 0.010830424696249145;  // ln 2 / 64
   double e = fma(r, a * a * a * a / 24.0, a * a * a / 6.0);
   e = fma(r, e, a * a / 2.0);
   e = fma(r, e, a);
   e = fma(r, e, 1.0);
-  const double t = sh.table[n & (kTable - 1)];
+  const int n = __double2loint(m);
+  const double t = table[n & (kTable - 1)];
   const double scaled = __hiloint2double(__double2hiint(t) + ((n >> 6) << 20), __double2loint(t));
-  const u64 bits = (u64)__double_as_longlong(fma(scaled, e, 4503599627370496.0));  // + 2^52: rounded to an integer
-  return any ? bits - 0x4330000000000000ull : 0;
+  return (u64)__double_as_longlong(fma(scaled, e, 4503599627370496.0));  // + 2^52: rounded to an integer
 }
-__device__ __forceinline__ double weight(float l, const RowScale& s) {  // in units of the largest, where one entry counts
-  const double x = ((double)l - (double)s.top) * s.c;
-  return x > -64000.0 ? exp2(x * 0.015625) : 0.0;
+__device__ __forceinline__ double weight(float l, const RowScale& s) {  // in units of the largest, for single entries
+  const double x = ((double)fmaxf(l, s.cutoff) - (double)s.top) * s.c;
+  return exp2(fmax(x, -64000.0) * 0.015625);
 }
-__device__ __forceinline__ int bin_of(float l, const RowScale& s) {
-  return (int)fminf((s.top - l) * s.bin_scale, (float)(kBins - 1));
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // A CTA's slice of a row in shared memory: 16-byte vectors as in global memory, what lies before and behind
 // the slice filled with -inf (no token). Vector v holds the entries first + v * N and on.
-template <typename T>
+template <typename T, int NT>
 struct Slice {
   static constexpr int N = Vec16<T>::N;
-  const uint4* v;
+  uint4* v;
   int n_vec, first;
   int seg;  // vectors of a warp's contiguous segment
   __device__ __forceinline__ void get(int i, float (&f)[N]) const { Vec16<T>::unpack(v[i], f); }
+  __device__ __forceinline__ int begin(int warp) const { return min(warp * seg, n_vec); }
+  __device__ __forceinline__ int end(int warp) const { return min(warp * seg + seg, n_vec); }
 };
 
-template <typename T>
-__device__ __forceinline__ T minus_inf() { return from_f32<T>(-INFINITY); }
-
-// Load the slice; largest entry that is a number (NaN ignored) and its lowest index.
-template <typename T>
-__device__ Slice<T> load_slice(const T* row, int vocab, int slice, uint4* buf, float& best, int& at) {
-  constexpr int N = Slice<T>::N;
+// Load the slice; its largest entry that is a number (NaN ignored).
+template <typename T, int NT>
+__device__ __forceinline__ Slice<T, NT> load_slice(const T* row, int vocab, int slice, uint4* buf, float& best) {
+  constexpr int N = Vec16<T>::N, W = NT / 32;
   const int begin = min((int)cluster_rank() * slice, vocab), end = min(begin + slice, vocab);
   const T* src = row + begin;
   const int lead = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T)), n = end - begin;
-  Slice<T> sl;
+  Slice<T, NT> sl;
   sl.v = buf;
   sl.first = begin - lead;
   sl.n_vec = n > 0 ? (lead + n + N - 1) / N : 0;
-  sl.seg = ((sl.n_vec + kWarps * 32 - 1) / (kWarps * 32)) * 32;
+  sl.seg = ((sl.n_vec + W * 32 - 1) / (W * 32)) * 32;
   best = -INFINITY;
-  at = 0x7fffffff;
   const uint4* g = reinterpret_cast<const uint4*>(src - lead);
   auto take = [&](int v, const uint4& u) {
     buf[v] = u;
     float f[N];
     Vec16<T>::unpack(u, f);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (f[i] > best) { best = f[i]; at = sl.first + v * N + i; }
+    for (int i = 0; i < N; ++i) best = fmaxf(best, f[i]);
   };
-  const int v0 = lead > 0 ? 1 : 0, v1 = n > 0 ? (lead + n) / N : 0;  // whole vectors
   auto ragged = [&](int e) {  // a vector that reaches over an end of the slice
     __align__(16) T tmp[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int k = e * N + i - lead;
-      tmp[i] = k >= 0 && k < n ? src[k] : minus_inf<T>();
+      tmp[i] = k >= 0 && k < n ? src[k] : from_f32<T>(-INFINITY);
     }
     take(e, *reinterpret_cast<const uint4*>(tmp));
   };
-  // (every thread meets its vectors in ascending order: the first of equal maxima stays)
-  if (threadIdx.x == 0 && lead > 0 && n > 0) ragged(0);
+  const int v0 = lead > 0 ? 1 : 0, v1 = n > 0 ? (lead + n) / N : 0;  // whole vectors
   int v = v0 + threadIdx.x;
-  for (; v + 3 * kThreads < v1; v += 4 * kThreads) {
+  for (; v + 7 * NT < v1; v += 8 * NT) {
+    uint4 u[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = ld_stream16(g + v + k * NT);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) take(v + k * NT, u[k]);
+  }
+  for (; v + 3 * NT < v1; v += 4 * NT) {
     uint4 u[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) u[k] = ld_stream16(g + v + k * kThreads);
+    for (int k = 0; k < 4; ++k) u[k] = ld_stream16(g + v + k * NT);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) take(v + k * kThreads, u[k]);
+    for (int k = 0; k < 4; ++k) take(v + k * NT, u[k]);
   }
-  for (; v < v1; v += kThreads) take(v, ld_stream16(g + v));
+  for (; v < v1; v += NT) take(v, ld_stream16(g + v));
+  if (threadIdx.x == 0 && lead > 0 && n > 0) ragged(0);
   if (threadIdx.x == 1 && v1 < sl.n_vec && (sl.n_vec > 1 || lead == 0)) ragged(sl.n_vec - 1);
   return sl;
 }
 
-// The cluster's largest logit and its lowest index (index -1: nothing but NaN and -inf). A row with +inf becomes one
-// of 0 (those) and -inf. Also readies the table of the exponential.
-template <typename T>
-__device__ float row_top(const Slice<T>& sl, float best, int at, int& index, Shared& sh, uint4* buf) {
+// The cluster's largest logit, -inf when it holds nothing but NaN and -inf. Rows at the ends of the number range are
+// rewritten in place, without changing an order or a weight: +inf entries become 0 and all others -inf; a row below
+// -1e38 is scaled by 1/4 (with its temperature). Also readies the table of the exponential.
+enum : int { kAsIs = 0, kInfinite = 1, kQuartered = 2 };
+__device__ __forceinline__ float rewritten(float l, int how) {
+  return how == kInfinite ? (l == INFINITY ? 0.f : -INFINITY) : how == kQuartered ? l * 0.25f : l;
+}
+template <typename T, int NT>
+__device__ float row_top(const Slice<T, NT>& sl, float best, int& how, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // (value, lowest index) as one integer
-  u64 k = at == 0x7fffffff ? 0 : ((u64)order_key<float>(best) << 32) | (u64)(0xffffffffu - (uint32_t)at);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) k = max(k, shfl_xor64(k, o));
-  if (lane == 0) sh.warp_a[warp] = k;
+  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (lane == 0) sh.warp_a[warp] = __float_as_uint(best);
   if (threadIdx.x < kTable) sh.table[threadIdx.x] = exp2((double)threadIdx.x / kTable) * kOne;
+  if (threadIdx.x == 0) sh.n_list = 0;
   __syncthreads();
   if (warp == 0) {
-    k = lane < kWarps ? sh.warp_a[lane] : 0;
+    best = __uint_as_float((uint32_t)sh.warp_a[min(lane, NT / 32 - 1)]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) k = max(k, shfl_xor64(k, o));
-    if (lane == 0) sh.slot[0].a = k;
+    for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) sh.slot[0].a = __float_as_uint(best);
   }
   cluster_sync();
-  const int c = cluster_size();
-  k = 0;
-  for (int r = 0; r < c; ++r) k = max(k, ld_remote64(remote(&sh.slot[0].a, r)));
-  if (k == 0) {
-    index = -1;
-    return -INFINITY;
-  }
-  index = (int)(0xffffffffu - (uint32_t)k);
-  const uint32_t key = (uint32_t)(k >> 32);
-  float top = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
-  if (top == INFINITY) {
-    constexpr int N = Slice<T>::N;
-    for (int v = threadIdx.x; v < sl.n_vec; v += kThreads) {
+  float top = -INFINITY;
+  for (int r = 0; r < (int)cluster_size(); ++r) top = fmaxf(top, __uint_as_float((uint32_t)ld_remote64(remote(&sh.slot[0].a, r))));
+  how = top == INFINITY ? kInfinite : top < -1e38f && top > -INFINITY ? kQuartered : kAsIs;
+  if (how != kAsIs) {
+    for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
       float f[N];
       sl.get(v, f);
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = f[i] == INFINITY ? 0.f : -INFINITY;
-      buf[v] = Vec16<T>::pack(f);
+      for (int i = 0; i < N; ++i) f[i] = rewritten(f[i], how);
+      sl.v[v] = Vec16<T>::pack(f);
     }
     __syncthreads();
-    top = 0.f;
+    top = rewritten(top, how);
   }
   return top;
 }
+// Lowest index of the largest logit (of a row that has one), through slot 1.
+template <typename T, int NT>
+__device__ int row_first(const Slice<T, NT>& sl, float top, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
+  int at = 0x7fffffff;
+  for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
+    float f[N];
+    sl.get(v, f);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (f[i] == top) at = min(at, sl.first + v * N + i);
+  }
+  at = __reduce_min_sync(0xffffffffu, at);
+  if ((threadIdx.x & 31) == 0) sh.warp_a[threadIdx.x >> 5] = (u64)at;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    u64 m = sh.warp_a[0];
+    for (int w = 1; w < NT / 32; ++w) m = min(m, sh.warp_a[w]);
+    sh.slot[1].a = m;
+  }
+  cluster_sync();
+  u64 m = ~0ull;
+  for (int r = 0; r < (int)cluster_size(); ++r) m = min(m, ld_remote64(remote(&sh.slot[1].a, r)));
+  return (int)m;
+}
 
-// Sum over the cluster of one integer per warp, through slot `s`: the whole, and what the CTAs before this one have.
-__device__ u64 cluster_total(u64 mine, Shared& sh, int s, u64& before) {
+// Sums over the cluster of two integers per warp (in its lane 0), through slot `s`: the wholes, and what the CTAs before this
+// one have of the first.
+template <int NT>
+__device__ Slot cluster_total(u64 a, u64 b, Shared& sh, int s, u64& before) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __syncthreads();
-  if (lane == 0) sh.warp_a[warp] = mine;
+  if (lane == 0) { sh.warp_a[warp] = a; sh.warp_b[warp] = b; }
   __syncthreads();
   if (warp == 0) {
-    const u64 v = warp_sum(lane < kWarps ? sh.warp_a[lane] : 0);
-    if (lane == 0) sh.slot[s].a = v;
+    const u64 va = warp_sum(lane < NT / 32 ? sh.warp_a[lane] : 0), vb = warp_sum(lane < NT / 32 ? sh.warp_b[lane] : 0);
+    if (lane == 0) { sh.slot[s].a = va; sh.slot[s].b = vb; }
   }
   cluster_sync();
   const int c = cluster_size(), rank = cluster_rank();
-  u64 all = 0;
+  Slot all = {0, 0};
   before = 0;
   for (int r = 0; r < c; ++r) {
     const u64 v = ld_remote64(remote(&sh.slot[s].a, r));
     if (r < rank) before += v;
-    all += v;
+    all.a += v;
+    all.b += ld_remote64(remote(&sh.slot[s].b, r));
   }
   return all;
 }
@@ -316,21 +369,28 @@ __device__ __forceinline__ void hist_add(Shared& sh, int bin, u64 w) {
   const uint32_t up = hi + (old + lo < old ? 1u : 0u);
   if (up) atomicAdd(&sh.hist_hi[bin], up);
 }
+template <int NT>
 __device__ __forceinline__ void hist_clear(Shared& sh) {
-  for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist_lo[i] = sh.hist_hi[i] = 0;
+  for (int i = threadIdx.x; i < kBins / 4; i += NT) {
+    reinterpret_cast<uint4*>(sh.hist_lo)[i] = make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4*>(sh.hist_hi)[i] = make_uint4(0, 0, 0, 0);
+  }
 }
 
 // First bin of the cluster's summed histogram whose inclusive running sum exceeds a limit, the sum before it and its own
-// mass; -1: none. limit_of(whole) gives the limit. Each CTA sums its share of the bins over the cluster; three slots.
-template <typename F>
-__device__ int hist_find(Shared& sh, int s, F limit_of, u64& limit, u64& before, u64& mass) {
+// mass; -1: none, `before` is the whole. `extra` (per warp, lane 0) is summed over the cluster along with it;
+// limit_of(histogram's whole, extra's whole) gives the limit. Each CTA sums its share of the bins over the cluster. Slots
+// s to s + 2.
+template <int NT, typename F>
+__device__ int hist_find(Shared& sh, int s, u64 extra, F limit_of, u64& limit, u64& before, u64& mass) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = cluster_size(), rank = cluster_rank();
-  const int bins = kBins / c, per = max(1, bins / kThreads);  // bins of this CTA, of a thread
+  constexpr int MAX = kBins / NT;
+  const int bins = kBins / c, per = max(1, bins / NT);  // bins of this CTA, of a thread
   cluster_sync();  // all histograms are complete
-  u64 v[kBins / kThreads], mine = 0;
+  u64 v[MAX], mine = 0;
   const int b0 = threadIdx.x * per;
 #pragma unroll
-  for (int i = 0; i < kBins / kThreads; ++i) {
+  for (int i = 0; i < MAX; ++i) {
     v[i] = 0;
     if (i < per && b0 + i < bins) {
       const int b = rank * bins + b0 + i;
@@ -344,15 +404,15 @@ __device__ int hist_find(Shared& sh, int s, F limit_of, u64& limit, u64& before,
     mine += v[i];
   }
   const u64 inc = warp_scan(mine, lane), warp_mass = __shfl_sync(0xffffffffu, inc, 31);
-  if (lane == 0) sh.warp_b[warp] = warp_mass;
   if (threadIdx.x == 0) sh.slot[s + 1].a = ~0ull;
   u64 cta_before, base = 0;
-  limit = limit_of(cluster_total(warp_mass, sh, s, cta_before));
-  for (int w = 0; w < warp; ++w) base += sh.warp_b[w];
+  const Slot all = cluster_total<NT>(warp_mass, extra, sh, s, cta_before);
+  limit = limit_of(all.a, all.b);
+  for (int w = 0; w < warp; ++w) base += sh.warp_a[w];
   u64 at = cta_before + base + inc - mine;
   if (at <= limit && at + mine > limit) {
 #pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) {
+    for (int i = 0; i < MAX; ++i) {
       if (at <= limit && at + v[i] > limit) {
         sh.slot[s + 1].a = (u64)(rank * bins + b0 + i);
         sh.slot[s + 1].b = at;
@@ -361,6 +421,8 @@ __device__ int hist_find(Shared& sh, int s, F limit_of, u64& limit, u64& before,
       at += v[i];
     }
   }
+  before = all.a;
+  if (all.a <= limit) return -1;
   cluster_sync();
   int bin = -1;
   for (int r = 0; r < c; ++r) {
@@ -374,58 +436,102 @@ __device__ int hist_find(Shared& sh, int s, F limit_of, u64& limit, u64& before,
   return bin;
 }
 
+// The kept tokens: those above `value`, and of those equal to it the ones up to index `index`.
 struct Kept {
-  u64 border;  // rank key of the last kept token; 0: all
-  u64 total;   // sum of the kept weights
+  float value;
+  int index;
+  u64 total;  // sum of the kept weights
+  __device__ __forceinline__ bool holds(float l, int i) const { return l > value || (l == value && i <= index); }
 };
-
-// Top-p border of the row. Without a cut the masses of the warps' segments are left in sh.seg.
 template <typename T>
-__device__ Kept find_kept(const Slice<T>& sl, const RowScale& s, float top_p, Shared& sh) {
-  constexpr int N = Slice<T>::N;
+__device__ __forceinline__ void set_border(Kept& k, u64 key) {
+  k.value = key_value<T>((uint32_t)(key >> kIndexBits));
+  k.index = kMaxVocab - 1 - (int)(key & (kMaxVocab - 1));
+}
+
+// Top-p border of the row. Without a cut the masses of the warps' segments are left in sh.seg. Slots 2 to 26.
+template <typename T, int NT>
+__device__ Kept find_kept(const Slice<T, NT>& sl, const RowScale& s, float top_p, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Kept k;
-  k.border = 0;
-  const int w0 = min(warp * sl.seg, sl.n_vec), w1 = min(w0 + sl.seg, sl.n_vec);
+  k.value = -INFINITY;
+  k.index = -1;
+  const int w0 = sl.begin(warp), w1 = sl.end(warp);
   if (!(top_p < 1.f)) {  // NaN: no cut
     u64 sum = 0, before;
     for (int v = w0 + lane; v < w1; v += 32) {
       float f[N];
       sl.get(v, f);
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum += fixed_weight(f[i], s, sh);
+      for (int i = 0; i < N; ++i) sum += raw_weight(f[i], s, sh.table);
+      sum -= N * kRaw;
     }
     sum = warp_sum(sum);
     if (lane == 0) sh.seg[warp] = sum;
-    k.total = cluster_total(sum, sh, 1, before);
+    k.total = cluster_total<NT>(sum, 0, sh, 2, before).a;
     return k;
   }
-  hist_clear(sh);
+  // Histogram of the tokens within kWindow nats of the top; the others' weight is one sum. (The tail of a vocabulary is
+  // most of its entries and seldom holds the border: their atomics would cost more than all the rest.)
+  hist_clear<NT>(sh);
   __syncthreads();
+  const float light = s.top - kWindow * s.t, near_scale = (float)kBins / (kWindow * s.t);
+  auto near_bin = [&](float l) { return min((int)((s.top - l) * near_scale), kBins - 1); };
+  u64 tail = 0;
   for (int v = w0 + lane; v < w1; v += 32) {
     float f[N];
     sl.get(v, f);
+    u64 w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = raw_weight(f[i], s, sh.table) - kRaw;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const u64 w = fixed_weight(f[i], s, sh);
-      if (w) hist_add(sh, bin_of(f[i], s), w);
+      if (f[i] >= light) hist_add(sh, near_bin(f[i]), w[i]);
+      else tail += w[i];
     }
   }
-  u64 limit, before, mass;
+  u64 limit, before, mass, lo = ~0ull, hi = 0;
   const double share = (double)fmaxf(top_p, 0.f);
-  int bin = hist_find(sh, 2, [&](u64 all) { k.total = all; return (u64)(share * (double)all); }, limit, before, mass);
-  if (bin < 0) return k;  // cannot happen with top_p < 1
+  int bin = hist_find<NT>(sh, 3, warp_sum(tail), [&](u64 a, u64 b) { k.total = a + b; return (u64)(share * (double)(a + b)); }, limit,
+                          before, mass);
   limit -= before;
-  u64 kept = before, lo = ~0ull, hi = 0;
+  u64 kept = before;
+  // The border lies in the tail: a histogram of it, over the 64 nats that hold any weight.
+  const bool far = bin < 0;
+  const float far_scale = (float)kBins / (56.f * s.t);
+  auto far_bin = [&](float l) { return min((int)(fmaxf(light - l, 0.f) * far_scale), kBins - 1); };
+  if (far) {
+    hist_clear<NT>(sh);  // (every CTA has read it: the cluster barrier in cluster_total)
+    __syncthreads();
+    for (int v = w0 + lane; v < w1; v += 32) {
+      float f[N];
+      sl.get(v, f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const u64 w = raw_weight(f[i], s, sh.table) - kRaw;
+        if (w && !(f[i] >= light)) hist_add(sh, far_bin(f[i]), w);
+      }
+    }
+    u64 same;
+    bin = hist_find<NT>(sh, 6, 0, [&](u64, u64) { return limit; }, same, before, mass);
+    if (bin < 0) return k;  // cannot happen with top_p < 1: the whole exceeds the limit
+    limit -= before;
+    kept += before;
+  }
+  // Members of the border's bin: listed, and the range of their rank keys.
   for (int v = w0 + lane; v < w1; v += 32) {
     float f[N];
     sl.get(v, f);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (!(f[i] > -INFINITY) || bin_of(f[i], s) != bin) continue;
-      const u64 key = rank_key<T>(f[i], sl.first + v * N + i);
+      const float l = f[i];
+      if (!(l > s.cutoff) || (l >= light) == far || (far ? far_bin(l) : near_bin(l)) != bin) continue;
+      const u64 key = rank_key<T>(l, sl.first + v * N + i);
       lo = min(lo, key);
       hi = max(hi, key);
+      const int at = atomicAdd(&sh.n_list, 1);
+      if (at < kList) sh.list[at] = key;
     }
   }
 #pragma unroll
@@ -433,33 +539,60 @@ __device__ Kept find_kept(const Slice<T>& sl, const RowScale& s, float top_p, Sh
   if (lane == 0) { sh.warp_a[warp] = lo; sh.warp_b[warp] = hi; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kWarps; ++w) { lo = min(lo, sh.warp_a[w]); hi = max(hi, sh.warp_b[w]); }
-    sh.slot[5].a = lo;
-    sh.slot[5].b = hi;
+    for (int w = 1; w < NT / 32; ++w) { lo = min(lo, sh.warp_a[w]); hi = max(hi, sh.warp_b[w]); }
+    sh.slot[9].a = lo;
+    sh.slot[9].b = hi;
+    sh.slot[10].a = (u64)sh.n_list;
   }
   cluster_sync();  // also: every CTA has read the histogram that is cleared next
+  int members = 0;
   for (int r = 0; r < (int)cluster_size(); ++r) {
-    lo = min(lo, ld_remote64(remote(&sh.slot[5].a, r)));
-    hi = max(hi, ld_remote64(remote(&sh.slot[5].b, r)));
+    lo = min(lo, ld_remote64(remote(&sh.slot[9].a, r)));
+    hi = max(hi, ld_remote64(remote(&sh.slot[9].b, r)));
+    members += (int)min(ld_remote64(remote(&sh.slot[10].a, r)), (u64)1 << 20);
   }
-  for (int s0 = 6;; s0 += 3) {  // 50 bits of rank key, 11 a round: five rounds at most
+  if (members <= kList) {  // few: every CTA ranks all of them
+    int base = 0;
+    for (int r = 0; r < (int)cluster_size(); ++r) {
+      const int n = (int)ld_remote64(remote(&sh.slot[10].a, r));
+      for (int i = threadIdx.x; i < n; i += NT) {
+        const u64 key = ld_remote64(remote(&sh.list[i], r));
+        sh.all_key[base + i] = key;
+        sh.all_w[base + i] = raw_weight(key_value<T>((uint32_t)(key >> kIndexBits)), s, sh.table) - kRaw;
+      }
+      base += n;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < members; i += NT) {
+      const u64 key = sh.all_key[i];
+      u64 above = 0;
+      for (int j = 0; j < members; ++j) above += sh.all_key[j] > key ? sh.all_w[j] : 0;
+      if (above <= limit && above + sh.all_w[i] > limit) {  // the last kept one
+        sh.border = key;
+        sh.kept = above + sh.all_w[i];
+      }
+    }
+    __syncthreads();
+    set_border<T>(k, sh.border);
+    k.total = kept + sh.kept;
+    return k;
+  }
+  for (int s0 = 11;; s0 += 3) {  // 50 bits of rank key, 11 a round: five rounds at most
     const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 11);
-    hist_clear(sh);
+    hist_clear<NT>(sh);
     __syncthreads();
     for (int v = w0 + lane; v < w1; v += 32) {
       float f[N];
       sl.get(v, f);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (!(f[i] > -INFINITY)) continue;
+        if (!(f[i] > s.cutoff)) continue;
         const u64 key = rank_key<T>(f[i], sl.first + v * N + i);
-        if (key < lo || key > hi) continue;
-        const u64 w = fixed_weight(f[i], s, sh);
-        if (w) hist_add(sh, (int)((hi - key) >> shift), w);
+        if (key >= lo && key <= hi) hist_add(sh, (int)((hi - key) >> shift), raw_weight(f[i], s, sh.table) - kRaw);
       }
     }
     u64 same;
-    bin = hist_find(sh, s0, [&](u64) { return limit; }, same, before, mass);
+    bin = hist_find<NT>(sh, s0, 0, [&](u64, u64) { return limit; }, same, before, mass);
     if (bin < 0) return k;  // cannot happen: the members' mass exceeds the limit
     limit -= before;
     kept += before;
@@ -467,7 +600,7 @@ __device__ Kept find_kept(const Slice<T>& sl, const RowScale& s, float top_p, Sh
     const u64 width = (1ull << shift) - 1;
     lo = hi - lo > width ? hi - width : lo;
     if (shift == 0) {
-      k.border = hi;
+      set_border<T>(k, hi);
       k.total = kept + mass;
       return k;
     }
@@ -475,17 +608,16 @@ __device__ Kept find_kept(const Slice<T>& sl, const RowScale& s, float top_p, Sh
 }
 
 // One entry's mass in a draw.
-template <typename T>
 struct Mass {
   RowScale s;
-  u64 border;
+  Kept kept;
   double inv_z;         // 1 / Z in units of 2^-44, residual only
   const float* minus;   // row of the draft distribution to subtract, or null
   int one_hot;          // or the token whose draft probability is 1, or -1
   bool residual;
   __device__ __forceinline__ u64 operator()(float l, int i, const Shared& sh) const {
-    if (!(l > -INFINITY) || rank_key<T>(l, i) < border) return 0;
-    u64 w = fixed_weight(l, s, sh);
+    if (!kept.holds(l, i)) return 0;  // NaN and -inf are never kept
+    u64 w = raw_weight(l, s, sh.table) - kRaw;
     if (residual && w) {
       const double q = minus != nullptr ? (double)__ldg(minus + i) : i == one_hot ? 1.0 : 0.0;
       const double r = (double)w * inv_z - q;
@@ -497,9 +629,9 @@ struct Mass {
 
 // First index whose running sum of mass exceeds u * (whole sum). The CTA that holds it writes it to *out; false when
 // there is no mass. `ready`: sh.seg holds the masses of the warps' segments already.
-template <typename T>
-__device__ bool draw(const Slice<T>& sl, const Mass<T>& mass, float u, bool ready, int slot, int32_t* out, Shared& sh) {
-  constexpr int N = Slice<T>::N;
+template <typename T, int NT>
+__device__ bool draw(const Slice<T, NT>& sl, const Mass& mass, float u, bool ready, int slot, int32_t* out, Shared& sh) {
+  constexpr int N = Vec16<T>::N, W = NT / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto sum_of = [&](int a, int b) {
     u64 sum = 0;
@@ -512,41 +644,40 @@ __device__ bool draw(const Slice<T>& sl, const Mass<T>& mass, float u, bool read
     return warp_sum(sum);
   };
   if (!ready) {
-    const int w0 = min(warp * sl.seg, sl.n_vec);
-    const u64 sum = sum_of(w0, min(w0 + sl.seg, sl.n_vec));
+    const u64 sum = sum_of(sl.begin(warp), sl.end(warp));
     if (lane == 0) sh.seg[warp] = sum;
   }
   __syncthreads();
   u64 before;
-  const u64 all = cluster_total(sh.seg[warp], sh, slot, before);
+  const u64 all = cluster_total<NT>(sh.seg[warp], 0, sh, slot, before).a;
   if (all == 0) return false;
   const double x = u > 0.f ? (double)u * (double)all : 0.0;  // NaN: 0
   u64 target = x < (double)all ? min((u64)x, all - 1) : all - 1;
   u64 mine = 0;
-  for (int w = 0; w < kWarps; ++w) mine += sh.seg[w];
+  for (int w = 0; w < W; ++w) mine += sh.seg[w];
   if (target < before || target - before >= mine) return true;  // another CTA's
   target -= before;
   int w = 0;
-  while (w < kWarps - 1 && target >= sh.seg[w]) target -= sh.seg[w++];
+  while (w < W - 1 && target >= sh.seg[w]) target -= sh.seg[w++];
   // the warps share that segment
-  const int begin = min(w * sl.seg, sl.n_vec), end = min(begin + sl.seg, sl.n_vec);
-  const int sub = (end - begin + kWarps - 1) / kWarps;
-  const int a = min(begin + warp * sub, end);
-  const u64 sum = sum_of(a, min(a + sub, end));
+  const int begin = sl.begin(w), end = sl.end(w);
+  const int sub = (end - begin + W - 1) / W;
+  const int a = min(begin + warp * sub, end), b = min(a + sub, end);
+  const u64 sum = sum_of(a, b);
+  __syncthreads();
   if (lane == 0) sh.warp_b[warp] = sum;
   __syncthreads();
   w = 0;
-  while (w < kWarps - 1 && target >= sh.warp_b[w]) target -= sh.warp_b[w++];
+  while (w < W - 1 && target >= sh.warp_b[w]) target -= sh.warp_b[w++];
   if (warp != w) return true;
-  for (int v0 = a; v0 < min(a + sub, end); v0 += 32) {
+  for (int v0 = a; v0 < b; v0 += 32) {
     const int v = v0 + lane;
     u64 m[N], total = 0;
-    const bool in = v < min(a + sub, end);
     float f[N];
-    if (in) sl.get(v, f);
+    if (v < b) sl.get(v, f);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      m[i] = in ? mass(f[i], sl.first + v * N + i, sh) : 0;
+      m[i] = v < b ? mass(f[i], sl.first + v * N + i, sh) : 0;
       total += m[i];
     }
     const u64 inc = warp_scan(total, lane);
@@ -569,42 +700,41 @@ __device__ bool draw(const Slice<T>& sl, const Mass<T>& mass, float u, bool read
   return true;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ Shared sh;
-  uint4* buf = reinterpret_cast<uint4*>(dyn);
+  __shared__ __align__(16) Shared sh;
+  constexpr int N = Vec16<T>::N;
   const int r = blockIdx.x / cluster_size();
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
-  const float t = __ldg(p.temperature + r);
+  const float t = __ldg(p.temperature + r), top_p = __ldg(p.top_p + r), u = __ldg(p.uniform + r);
   float best;
-  int at, first;
-  const Slice<T> sl = load_slice(row, p.vocab, p.slice, buf, best, at);
-  const float top = row_top(sl, best, at, first, sh, buf);
-  constexpr int N = Slice<T>::N;
+  int how;
+  const Slice<T, NT> sl = load_slice<T, NT>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best);
+  const float top = row_top(sl, best, how, sh);
   const int begin = min((int)cluster_rank() * p.slice, p.vocab), end = min(begin + p.slice, p.vocab);
   float* probs = p.probs == nullptr ? nullptr : p.probs + (int64_t)r * p.probs_stride;
-  if (!(t > 0.f) || first < 0) {  // greedy, or a row without a token
+  if (!(t > 0.f) || top == -INFINITY) {  // greedy, or a row without a token
+    const int first = top == -INFINITY ? -1 : row_first(sl, top, sh);
     if (cluster_rank() == 0 && threadIdx.x == 0) p.tokens[r] = max(first, 0);
     if (probs != nullptr)
-      for (int i = begin + threadIdx.x; i < end; i += kThreads) probs[i] = i == first ? 1.f : 0.f;
+      for (int i = begin + threadIdx.x; i < end; i += NT) probs[i] = i == first ? 1.f : 0.f;
   } else {
-    Mass<T> mass;
-    mass.s = row_scale(top, t);
-    const float top_p = __ldg(p.top_p + r);
-    const Kept k = find_kept(sl, mass.s, top_p, sh);
-    mass.border = k.border; mass.inv_z = 0.0; mass.minus = nullptr; mass.one_hot = -1; mass.residual = false;
-    draw(sl, mass, __ldg(p.uniform + r), !(top_p < 1.f), 22, p.tokens + r, sh);
+    Mass mass;
+    mass.s = row_scale(top, how == kQuartered ? t * 0.25f : t);
+    mass.kept = find_kept(sl, mass.s, top_p, sh);
+    mass.residual = false;
+    mass.inv_z = 0.0; mass.minus = nullptr; mass.one_hot = -1;
+    draw(sl, mass, u, !(top_p < 1.f), 27, p.tokens + r, sh);
     if (probs != nullptr) {
-      const float inv = (float)(kOne / (double)k.total);
-      for (int v = threadIdx.x; v < sl.n_vec; v += kThreads) {
+      const float inv = (float)(mass.s.one / (double)mass.kept.total);
+      for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
         float f[N];
         sl.get(v, f);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int x = sl.first + v * N + i;
-          if (x >= begin && x < end)
-            probs[x] = f[i] > -INFINITY && rank_key<T>(f[i], x) >= k.border ? exp2f((f[i] - top) * mass.s.c32) * inv : 0.f;
+          if (x >= begin && x < end) probs[x] = mass.kept.holds(f[i], x) ? exp2f((f[i] - top) * mass.s.c32) * inv : 0.f;
         }
       }
     }
@@ -621,51 +751,94 @@ __device__ __forceinline__ int owner_of(const int32_t* __restrict__ indptr, int 
   return lo;
 }
 
+// Does the draft x of a row pass, u q(x) < p(x)? The answer needs p(x) only to one side of u q(x): sums in fp32 decide
+// unless they come too close (1e-5 bounds their error: 2^-22 of ex2.approx, 2^-23 of the exponent's size, which the
+// weights average to at most log2 of the vocabulary, 128 additions), or the nucleus' exact mass is needed: Z lies
+// between top_p and 1 times the whole sum. 1: yes, 0: no, -1: not known.
+template <typename T, int NT>
+__device__ int quick_test(const Slice<T, NT>& sl, const RowScale& s, float top_p, int x, float lx, double wx, double uq, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
+  constexpr double kFix = 1099511627776.0, kGuard = 4e-5;  // 2^40
+  float all = 0.f, above = 0.f;
+  const bool cut = top_p < 1.f;
+  u64 fall = 0, fabove = 0;
+  int n = 0;
+  for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
+    float f[N];
+    sl.get(v, f);
+    const int i0 = sl.first + v * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float w = ex2((fmaxf(f[i], s.cutoff) - s.top) * s.c32);
+      all += w;
+      if (cut) above += f[i] > lx || (f[i] == lx && i0 + i < x) ? w : 0.f;
+    }
+    if (++n * N >= 128) {
+      fall += (u64)(all * (float)kFix);
+      fabove += (u64)(above * (float)kFix);
+      all = above = 0.f;
+      n = 0;
+    }
+  }
+  fall = warp_sum(fall + (u64)(all * (float)kFix));
+  fabove = warp_sum(fabove + (u64)(above * (float)kFix));
+  u64 before;
+  const Slot sum = cluster_total<NT>(fall, fabove, sh, 28, before);
+  const double total = (double)sum.a / kFix, ahead = (double)sum.b / kFix;
+  double least = total;  // of Z
+  if (cut) {
+    least = total * fmax((double)top_p, 0.0);
+    if (ahead * (1 - kGuard) > least * (1 + kGuard)) return 0;      // not in the nucleus
+    if (!(ahead * (1 + kGuard) <= least * (1 - kGuard))) return -1;  // (and its first token when top_p is 0)
+  }
+  if (uq * total * (1 + kGuard) < wx) return 1;
+  if (uq * least * (1 - kGuard) >= wx) return 0;
+  return -1;
+}
+
 // One cluster per row that has a draft behind it: is the draft accepted?
-template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const SampleParams p) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ Shared sh;
-  uint4* buf = reinterpret_cast<uint4*>(dyn);
+  __shared__ __align__(16) Shared sh;
   const int r = blockIdx.x / cluster_size();
   const int req = owner_of(p.indptr, p.batch, r);
   const int begin = __ldg(p.indptr + req), end = __ldg(p.indptr + req + 1);
   if (r < begin || r + 1 >= end || end > p.nnz) return;  // a last row, or behind the last request (the whole cluster)
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const int x = __ldg(p.draft + r + 1);
-  const float t = __ldg(p.temperature + req);
+  const float t = __ldg(p.temperature + req), top_p = __ldg(p.top_p + req);
+  const bool token = x >= 0 && x < p.vocab;
+  const float lx = token ? to_f32(row[x]) : -INFINITY;
+  const double q = p.draft_probs == nullptr || !token ? 1.0 : (double)__ldg(p.draft_probs + (int64_t)r * p.draft_stride + x);
+  const double uq = (double)__ldg(p.uniform + r) * q;
   float best;
-  int at, first;
-  const Slice<T> sl = load_slice(row, p.vocab, p.slice, buf, best, at);
-  const float top = row_top(sl, best, at, first, sh, buf);
-  double px = 0.0;
-  if (first >= 0 && x >= 0 && x < p.vocab) {
+  int how, ok = 0;
+  const Slice<T, NT> sl = load_slice<T, NT>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best);
+  const float top = row_top(sl, best, how, sh), l = rewritten(lx, how);
+  if (l > -INFINITY) {  // a token (and so the row has a top)
     if (!(t > 0.f)) {
-      px = x == first ? 1.0 : 0.0;
+      ok = l == top && row_first(sl, top, sh) == x && uq < 1.0;
     } else {
-      const RowScale s = row_scale(top, t);
-      const Kept k = find_kept(sl, s, __ldg(p.top_p + req), sh);
-      float l = to_f32(row[x]);
-      if (l == INFINITY) l = 0.f;  // as row_top rewrote the row
-      else if (top == 0.f && to_f32(row[first]) == INFINITY) l = -INFINITY;
-      if (l > -INFINITY && rank_key<T>(l, x) >= k.border) px = weight(l, s) * (kOne / (double)k.total);
+      const RowScale s = row_scale(top, how == kQuartered ? t * 0.25f : t);
+      const double wx = weight(l, s);
+      ok = quick_test(sl, s, top_p, x, l, wx, uq, sh);
+      if (ok < 0) {
+        const Kept k = find_kept(sl, s, top_p, sh);
+        ok = k.holds(l, x) && uq < wx * (s.one / (double)k.total);
+      }
     }
   }
-  if (cluster_rank() == 0 && threadIdx.x == 0) {
-    const double q = p.draft_probs == nullptr || x < 0 || x >= p.vocab
-                         ? 1.0 : (double)__ldg(p.draft_probs + (int64_t)r * p.draft_stride + x);
-    p.ok[r] = (double)__ldg(p.uniform + r) * q < px ? 1 : 0;
-  }
+  if (cluster_rank() == 0 && threadIdx.x == 0) p.ok[r] = (uint8_t)ok;
   cluster_sync();
 }
 
 // One cluster per request: the accepted prefix, then a draw from the residual of the first rejected row or
 // from the last row.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_draw_kernel(const SampleParams p) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ Shared sh;
-  uint4* buf = reinterpret_cast<uint4*>(dyn);
+  __shared__ __align__(16) Shared sh;
   const int req = blockIdx.x / cluster_size();
   const bool lead = cluster_rank() == 0 && threadIdx.x == 0;
   const int begin = __ldg(p.indptr + req), end = __ldg(p.indptr + req + 1);
@@ -681,27 +854,26 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const SampleParam
   while (r + 1 < end && p.ok[r]) ++r;
   const bool rejected = r + 1 < end;
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
-  const float t = __ldg(p.temperature + req);
+  const float t = __ldg(p.temperature + req), top_p = __ldg(p.top_p + req), u = __ldg(p.uniform + end - 1);
   float best;
-  int at, first;
-  const Slice<T> sl = load_slice(row, p.vocab, p.slice, buf, best, at);
-  const float top = row_top(sl, best, at, first, sh, buf);
+  int how;
+  const Slice<T, NT> sl = load_slice<T, NT>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best);
+  const float top = row_top(sl, best, how, sh);
   if (lead) p.accepted[req] = r - begin;
-  if (!(t > 0.f) || first < 0) {
-    if (lead) p.tokens[req] = max(first, 0);
+  if (!(t > 0.f) || top == -INFINITY) {
+    const int first = top == -INFINITY ? 0 : row_first(sl, top, sh);
+    if (lead) p.tokens[req] = first;
   } else {
-    Mass<T> mass;
-    mass.s = row_scale(top, t);
-    const float top_p = __ldg(p.top_p + req), u = __ldg(p.uniform + end - 1);
-    const Kept k = find_kept(sl, mass.s, top_p, sh);
-    mass.border = k.border;
-    mass.inv_z = 1.0 / (double)k.total;
+    Mass mass;
+    mass.s = row_scale(top, how == kQuartered ? t * 0.25f : t);
+    mass.kept = find_kept(sl, mass.s, top_p, sh);
+    mass.inv_z = 1.0 / (double)mass.kept.total;
     mass.residual = rejected;
     mass.minus = rejected && p.draft_probs != nullptr ? p.draft_probs + (int64_t)r * p.draft_stride : nullptr;
     mass.one_hot = rejected ? __ldg(p.draft + r + 1) : -1;
-    if (!draw(sl, mass, u, !rejected && !(top_p < 1.f), 22, p.tokens + req, sh)) {
+    if (!draw(sl, mass, u, !rejected && !(top_p < 1.f), 29, p.tokens + req, sh)) {
       mass.residual = false;  // nothing left above the draft's distribution: the target's own
-      draw(sl, mass, u, false, 23, p.tokens + req, sh);
+      draw(sl, mass, u, false, 30, p.tokens + req, sh);
     }
   }
   cluster_sync();
@@ -710,27 +882,29 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const SampleParam
 // ---- host --------------------------------------------------------------------------------------------
 struct Shape {
   int ctas, slice;
+  bool wide;  // 512 threads, else 256
   size_t smem;
 };
-// CTAs of a row: as few as keep a slice within 64 KB (two CTAs per SM, so that one loads while the other
-// computes); more, up to 8, while all of them still fit the machine at once and a slice keeps 2048 entries.
+// CTAs of a row: as few as keep a slice within 32 KB, four CTAs of 256 threads per SM, so that some load while others
+// compute; where all rows fit the SMs at once anyway, more CTAs (up to 8, slices of 2048 entries at least) of 512 threads.
 Shape pick_shape(int rows, int vocab, int es) {
   Shape s;
   s.ctas = 1;
-  while (s.ctas < kMaxCtas && (int64_t)vocab * es > (int64_t)s.ctas * 65536) s.ctas *= 2;
-  while (s.ctas < kMaxCtas && (int64_t)rows * s.ctas * 2 <= 296 && vocab / (s.ctas * 2) >= 2048) s.ctas *= 2;
+  while (s.ctas < kMaxCtas && (int64_t)vocab * es > (int64_t)s.ctas * 32768) s.ctas *= 2;
+  while (s.ctas < kMaxCtas && (int64_t)rows * s.ctas * 2 <= 148 && vocab / (s.ctas * 2) >= 2048) s.ctas *= 2;
+  s.wide = (int64_t)rows * s.ctas <= 148;
   s.slice = ((vocab + s.ctas - 1) / s.ctas + 63) & ~63;
   s.smem = (size_t)s.slice * es + 32;
   return s;
 }
 
-template <typename K>
+template <int NT, typename K>
 cudaError_t launch(K kernel, int rows, const Shape& s, const SampleParams& p, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * s.ctas);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = s.smem;
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -764,12 +938,11 @@ int dsv_sample_top_p(const void* logits, int64_t row_stride, int rows, int vocab
   const Shape shape = pick_shape(rows, vocab, elem_size(dtype));
   p.slice = shape.slice;
   cudaStream_t st = (cudaStream_t)stream;
-  cudaError_t e;
-  switch (dtype) {
-    case DSV_F32: e = launch(sample_kernel<float>, rows, shape, p, st); break;
-    case DSV_F16: e = launch(sample_kernel<__half>, rows, shape, p, st); break;
-    default: e = launch(sample_kernel<__nv_bfloat16>, rows, shape, p, st);
-  }
+  auto go = [&](auto tag) -> cudaError_t {
+    using T = decltype(tag);
+    return shape.wide ? launch<512>(sample_kernel<T, 512>, rows, shape, p, st) : launch<256>(sample_kernel<T, 256>, rows, shape, p, st);
+  };
+  const cudaError_t e = dtype == DSV_F32 ? go(float{}) : dtype == DSV_F16 ? go(__half{}) : go(__nv_bfloat16{});
   if (e != cudaSuccess) return fail(DSV_E_CUDA, "sample_top_p launch failed: %s", cudaGetErrorString(e));
   return DSV_OK;
 }
@@ -795,23 +968,21 @@ int dsv_verify_draft(const void* logits, int64_t row_stride, int nnz, int vocab,
   p.draft_stride = draft_stride; p.ok = workspace; p.accepted = accepted; p.batch = batch; p.nnz = nnz;
   p.status = device_status_ptr();
   cudaStream_t st = (cudaStream_t)stream;
-  auto go = [&](auto rows_kernel, auto draw_kernel) -> cudaError_t {
+  auto go = [&](auto tag) -> cudaError_t {
+    using T = decltype(tag);
     if (nnz > 0) {
       const Shape shape = pick_shape(nnz, vocab, elem_size(dtype));
       p.slice = shape.slice;
-      const cudaError_t er = launch(rows_kernel, nnz, shape, p, st);
+      const cudaError_t er = shape.wide ? launch<512>(verify_rows_kernel<T, 512>, nnz, shape, p, st)
+                                        : launch<256>(verify_rows_kernel<T, 256>, nnz, shape, p, st);
       if (er != cudaSuccess) return er;
     }
     const Shape shape = pick_shape(batch, vocab, elem_size(dtype));
     p.slice = shape.slice;
-    return launch(draw_kernel, batch, shape, p, st);
+    return shape.wide ? launch<512>(verify_draw_kernel<T, 512>, batch, shape, p, st)
+                      : launch<256>(verify_draw_kernel<T, 256>, batch, shape, p, st);
   };
-  cudaError_t e;
-  switch (dtype) {
-    case DSV_F32: e = go(verify_rows_kernel<float>, verify_draw_kernel<float>); break;
-    case DSV_F16: e = go(verify_rows_kernel<__half>, verify_draw_kernel<__half>); break;
-    default: e = go(verify_rows_kernel<__nv_bfloat16>, verify_draw_kernel<__nv_bfloat16>);
-  }
+  const cudaError_t e = dtype == DSV_F32 ? go(float{}) : dtype == DSV_F16 ? go(__half{}) : go(__nv_bfloat16{});
   if (e != cudaSuccess) return fail(DSV_E_CUDA, "verify_draft launch failed: %s", cudaGetErrorString(e));
   return DSV_OK;
 }

@@ -11,9 +11,9 @@
 // so every cut of the row, and every order of the atomics, gives the same token. 2^18 entries of
 // weight one still fit 63 bits, hence the bound on the vocabulary.
 //
-// A cluster of 1 to 8 CTAs owns a row and keeps it in shared memory (one pass over HBM): the largest
-// logit, the weight sums, the top-p border and the draw each walk it again there. Sums and histograms
-// of the CTAs meet through distributed shared memory.
+// A row is read from HBM once: a cluster of up to 8 CTAs keeps it in shared memory, or, with many rows, one
+// CTA finds it in L2 again. The largest logit, the weight sums, the top-p border and the draw each walk it
+// there. Sums and histograms of a cluster's CTAs meet through distributed shared memory.
 //
 // The top-p border is found without sorting: a histogram of weight over 2048 bins of (max - l) / T gives
 // the bin of the border; the members of that bin are then split 2048 ways again by (value, index) until
@@ -30,6 +30,7 @@ constexpr int kBins = 2048;
 constexpr int kMaxCtas = 8;   // of a cluster (the portable limit)
 constexpr int kMaxWarps = 16;
 constexpr int kList = 256;    // members of the border's bin that are ranked directly
+constexpr int kSub = 16;      // subsegments of a warp's part of a row
 constexpr int kMaxVocab = 1 << 18, kIndexBits = 18;
 constexpr double kOne = 17592186044416.0;          // 2^44: the fixed-point weight of the largest logit
 constexpr double kProbOne = 1152921504606846976.0;  // 2^60: fixed-point probabilities of the residual
@@ -37,6 +38,26 @@ constexpr float kWindow = 8.f;                      // nats below the top that t
 constexpr int kTable = 64;
 typedef unsigned long long u64;
 constexpr u64 kRaw = 0x4330000000000000ull;  // 2^52 as a double: integers sit behind it
+
+// 2^(j / 64)
+__constant__ double kPowers[kTable] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
+};
 
 struct SampleParams {
   const void* logits;
@@ -68,12 +89,13 @@ struct Slot {
 struct Shared {
   uint32_t hist_lo[kBins], hist_hi[kBins];
   double table[kTable];  // 2^(j / 64 + 44)
-  Slot slot[32];
+  Slot slot[36];
   u64 warp_a[kMaxWarps], warp_b[kMaxWarps];
-  u64 seg[kMaxWarps];    // mass of the warps' segments
+  u64 seg[kMaxWarps * kSub];  // mass of the subsegments
   u64 list[kList];       // this CTA's members of the border's bin
   u64 all_key[kList], all_w[kList];
   int n_list;
+  int32_t tie;
   u64 border, kept;
 };
 
@@ -89,6 +111,10 @@ __device__ __forceinline__ uint32_t cluster_size() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+  if (cluster_size() == 1) {
+    __syncthreads();
+    return;
+  }
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {  // the same shared-memory object of CTA `rank`
@@ -112,6 +138,28 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += shfl_xor64(v, o);
   return v;
+}
+// The cluster's sum / maximum / minimum of one integer per CTA (lane r asks CTA r: one round trip).
+__device__ __forceinline__ u64 cluster_sum(const u64* p, int upto) {
+  const uint32_t lane = threadIdx.x & 31;
+  u64 v = (int)lane < upto ? ld_remote64(remote(p, lane)) : 0;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v += shfl_xor64(v, o);
+  return __shfl_sync(0xffffffffu, v, 0);
+}
+__device__ __forceinline__ u64 cluster_max(const u64* p) {
+  const uint32_t lane = threadIdx.x & 31;
+  u64 v = lane < cluster_size() ? ld_remote64(remote(p, lane)) : 0;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v = max(v, shfl_xor64(v, o));
+  return __shfl_sync(0xffffffffu, v, 0);
+}
+__device__ __forceinline__ u64 cluster_min(const u64* p) {
+  const uint32_t lane = threadIdx.x & 31;
+  u64 v = lane < cluster_size() ? ld_remote64(remote(p, lane)) : ~0ull;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v = min(v, shfl_xor64(v, o));
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
 #pragma unroll
@@ -160,23 +208,24 @@ struct RowScale {
   float c32;     // log2(e) / T
   double c;      // 64 log2(e) / T
   double magic;  // 1.5 * 2^52 - K, K = round(top c): added to l c it leaves the rounded l c - K in the low word
-  double one;    // the fixed-point weight of the top: 2^44 2^((top c - K) / 64)
 };
 __device__ __forceinline__ RowScale row_scale(float top, float temperature) {
   RowScale s;
   s.top = top;
-  s.t = fminf(temperature, 1e36f);  // (so that the cutoff below stays finite)
-  const double inv = 1.0 / (double)s.t;
+  s.t = fminf(fmaxf(temperature, 1e-30f), 1e36f);  // (so that the cutoff below stays finite)
+  s.c = 92.332482616893657 / (double)s.t;
+  s.c32 = 1.442695041f / s.t;
   // A temperature so small that one unit in the last place of the top already gives weight 0 gives the same weights
   // as 2^37 / |top|, which keeps the exponents in range.
-  s.c = fmin(92.332482616893657 * inv, 137438953472.0 / fabs((double)top));
-  s.c32 = (float)fmin(1.4426950408889634 * inv, 3e38);
+  if (fabs((double)top * s.c) > 137438953472.0) s.c = 137438953472.0 / fabs((double)top);
   const float ulp = __uint_as_float(__float_as_uint(fabsf(top)) + 1u) - fabsf(top);
   s.cutoff = top - fmaxf(64.f * s.t, 2.f * ulp);
-  const double k = rint((double)top * s.c);
-  s.magic = 6755399441055744.0 - k;
-  s.one = kOne * exp2(fma((double)top, s.c, -k) * 0.015625);
+  s.magic = 6755399441055744.0 - rint((double)top * s.c);
   return s;
+}
+// The fixed-point weight of the top, 2^44 2^((top c - K) / 64), as a number.
+__device__ __forceinline__ double top_weight(const RowScale& s) {
+  return kOne * exp2(fma((double)s.top, s.c, s.magic - 6755399441055744.0) * 0.015625);
 }
 // Fixed-point weight behind kRaw (subtract it; sums may subtract it once per entry). With l c = N + r, |r| <= 1/2:
 // 2^((N - K) / 64) from a table of 2^(j / 64) and an exponent, e^(r ln 2 / 64) to the fourth power (its argument is
@@ -206,123 +255,176 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A CTA's slice of a row in shared memory: 16-byte vectors as in global memory, what lies before and behind
-// the slice filled with -inf (no token). Vector v holds the entries first + v * N and on.
-template <typename T, int NT>
+// A CTA's slice of a row as 16-byte vectors, aligned as in global memory: vector v holds the entries first + v * N and
+// on; what lies before and behind the slice reads as -inf (no token). kShared: in shared memory, else in global memory
+// (where the first pass has left it in L2). Rows at the ends of the number range are rewritten as they are read, without
+// changing an order or a weight: +inf entries become 0 and all others -inf; a row below -1e38 is scaled by 1/4 (with its
+// temperature).
+enum : int { kAsIs = 0, kInfinite = 1, kQuartered = 2 };
+__device__ __forceinline__ float rewritten(float l, int how) {
+  return how == kInfinite ? (l == INFINITY ? 0.f : -INFINITY) : how == kQuartered ? l * 0.25f : l;
+}
+template <typename T, int NT, bool kShared>
 struct Slice {
   static constexpr int N = Vec16<T>::N;
   uint4* v;
   int n_vec, first;
-  int seg;  // vectors of a warp's contiguous segment
-  __device__ __forceinline__ void get(int i, float (&f)[N]) const { Vec16<T>::unpack(v[i], f); }
+  int seg, sub;    // vectors of a warp's contiguous segment, of a subsegment
+  int lead, tail;  // entries of the first and of the last vector that lie outside
+  int how;
+  __device__ __forceinline__ void mask(int i, float (&f)[N]) const {
+    if (i == 0 || i == n_vec - 1) {
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if ((i == 0 && k < lead) || (i == n_vec - 1 && k >= N - tail)) f[k] = -INFINITY;
+    }
+  }
+  __device__ __forceinline__ void finish(int i, float (&f)[N]) const {
+    mask(i, f);
+    if (how != kAsIs) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) f[k] = rewritten(f[k], how);
+    }
+  }
+  __device__ __forceinline__ void get(int i, float (&f)[N]) const {
+    Vec16<T>::unpack(kShared ? v[i] : ld_stream16(v + i), f);
+    finish(i, f);
+  }
+  // of(values, first index) for the vectors [a, b), lane by lane; from L2 two vectors are on their way while one is used.
+  template <typename F>
+  __device__ __forceinline__ void each(int a, int b, int step, F of) const {
+    float f[N];
+    if (kShared) {
+      for (int i = a; i < b; i += step) {
+        get(i, f);
+        of(f, first + i * N);
+      }
+      return;
+    }
+    uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0, u2 = u0;
+    if (a < b) u0 = ld_stream16(v + a);
+    if (a + step < b) u1 = ld_stream16(v + a + step);
+    for (int i = a; i < b; i += step) {
+      if (i + 2 * step < b) u2 = ld_stream16(v + i + 2 * step);
+      Vec16<T>::unpack(u0, f);
+      finish(i, f);
+      of(f, first + i * N);
+      u0 = u1;
+      u1 = u2;
+    }
+  }
   __device__ __forceinline__ int begin(int warp) const { return min(warp * seg, n_vec); }
   __device__ __forceinline__ int end(int warp) const { return min(warp * seg + seg, n_vec); }
+  // Sum of `of(values, first index)` over every subsegment of the warp, into sh.seg; the warp's total.
+  template <typename F>
+  __device__ __forceinline__ u64 sum(Shared& sh, F of) const {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = end(warp);
+    u64 total = 0;
+    int at = begin(warp);
+    for (int k = 0; k < kSub; ++k) {
+      const int stop = min(at + sub, e);
+      u64 x = 0;
+      each(at + lane, stop, 32, [&](const float (&f)[N], int i) { x += of(f, i); });
+      if (at < stop) x = warp_sum(x);
+      if (lane == 0) sh.seg[warp * kSub + k] = x;
+      total += x;
+      at = stop;
+    }
+    return total;
+  }
 };
 
-// Load the slice; its largest entry that is a number (NaN ignored).
-template <typename T, int NT>
-__device__ __forceinline__ Slice<T, NT> load_slice(const T* row, int vocab, int slice, uint4* buf, float& best) {
+// of(value, place) for the entries of a vector that `in` marks: one by one where they are few, side by side where many.
+template <int N, typename F>
+__device__ __forceinline__ void marked(const float (&f)[N], unsigned in, F of) {
+  if (__popc(in) > 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (in >> i & 1) of(f[i], i);
+    return;
+  }
+  while (in) {
+    const int i = __ffs(in) - 1;
+    in &= in - 1;
+    float l = f[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) l = i == j ? f[j] : l;
+    of(l, i);
+  }
+}
+
+// First pass: the slice's largest entry that is a number (NaN ignored), and its copy in shared memory.
+template <typename T, int NT, bool kShared>
+__device__ __forceinline__ Slice<T, NT, kShared> load_slice(const T* row, int vocab, int slice, uint4* buf, float& best, Shared& sh) {
   constexpr int N = Vec16<T>::N, W = NT / 32;
-  const int begin = min((int)cluster_rank() * slice, vocab), end = min(begin + slice, vocab);
+  if (threadIdx.x < kTable) sh.table[threadIdx.x] = kPowers[threadIdx.x] * kOne;
+  if (threadIdx.x == 0) sh.n_list = 0;
+  const int begin = min((int)cluster_rank() * slice, vocab), n = min(begin + slice, vocab) - begin;
   const T* src = row + begin;
-  const int lead = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T)), n = end - begin;
-  Slice<T, NT> sl;
-  sl.v = buf;
-  sl.first = begin - lead;
-  sl.n_vec = n > 0 ? (lead + n + N - 1) / N : 0;
+  Slice<T, NT, kShared> sl;
+  sl.lead = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
+  uint4* g = reinterpret_cast<uint4*>(const_cast<T*>(src - sl.lead));
+  sl.v = kShared ? buf : g;
+  sl.first = begin - sl.lead;
+  sl.n_vec = n > 0 ? (sl.lead + n + N - 1) / N : 0;
+  sl.tail = sl.n_vec * N - sl.lead - n;
   sl.seg = ((sl.n_vec + W * 32 - 1) / (W * 32)) * 32;
+  sl.sub = ((sl.seg + kSub * 32 - 1) / (kSub * 32)) * 32;
+  sl.how = kAsIs;
   best = -INFINITY;
-  const uint4* g = reinterpret_cast<const uint4*>(src - lead);
   auto take = [&](int v, const uint4& u) {
-    buf[v] = u;
+    if (kShared) buf[v] = u;
     float f[N];
     Vec16<T>::unpack(u, f);
+    sl.mask(v, f);
 #pragma unroll
     for (int i = 0; i < N; ++i) best = fmaxf(best, f[i]);
   };
-  auto ragged = [&](int e) {  // a vector that reaches over an end of the slice
-    __align__(16) T tmp[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int k = e * N + i - lead;
-      tmp[i] = k >= 0 && k < n ? src[k] : from_f32<T>(-INFINITY);
-    }
-    take(e, *reinterpret_cast<const uint4*>(tmp));
-  };
-  const int v0 = lead > 0 ? 1 : 0, v1 = n > 0 ? (lead + n) / N : 0;  // whole vectors
-  int v = v0 + threadIdx.x;
-  for (; v + 7 * NT < v1; v += 8 * NT) {
+  int v = threadIdx.x;
+  for (; v + 7 * NT < sl.n_vec; v += 8 * NT) {
     uint4 u[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) u[k] = ld_stream16(g + v + k * NT);
 #pragma unroll
     for (int k = 0; k < 8; ++k) take(v + k * NT, u[k]);
   }
-  for (; v + 3 * NT < v1; v += 4 * NT) {
-    uint4 u[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) u[k] = ld_stream16(g + v + k * NT);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) take(v + k * NT, u[k]);
-  }
-  for (; v < v1; v += NT) take(v, ld_stream16(g + v));
-  if (threadIdx.x == 0 && lead > 0 && n > 0) ragged(0);
-  if (threadIdx.x == 1 && v1 < sl.n_vec && (sl.n_vec > 1 || lead == 0)) ragged(sl.n_vec - 1);
+  for (; v < sl.n_vec; v += NT) take(v, ld_stream16(g + v));
   return sl;
 }
 
-// The cluster's largest logit, -inf when it holds nothing but NaN and -inf. Rows at the ends of the number range are
-// rewritten in place, without changing an order or a weight: +inf entries become 0 and all others -inf; a row below
-// -1e38 is scaled by 1/4 (with its temperature). Also readies the table of the exponential.
-enum : int { kAsIs = 0, kInfinite = 1, kQuartered = 2 };
-__device__ __forceinline__ float rewritten(float l, int how) {
-  return how == kInfinite ? (l == INFINITY ? 0.f : -INFINITY) : how == kQuartered ? l * 0.25f : l;
-}
-template <typename T, int NT>
-__device__ float row_top(const Slice<T, NT>& sl, float best, int& how, Shared& sh) {
-  constexpr int N = Vec16<T>::N;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The cluster's largest logit, -inf when it holds nothing but NaN and -inf.
+template <typename T, int NT, bool kShared>
+__device__ float row_top(Slice<T, NT, kShared>& sl, float best, Shared& sh) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (lane == 0) sh.warp_a[warp] = __float_as_uint(best);
-  if (threadIdx.x < kTable) sh.table[threadIdx.x] = exp2((double)threadIdx.x / kTable) * kOne;
-  if (threadIdx.x == 0) sh.n_list = 0;
   __syncthreads();
   if (warp == 0) {
-    best = __uint_as_float((uint32_t)sh.warp_a[min(lane, NT / 32 - 1)]);
+    best = __uint_as_float((uint32_t)sh.warp_a[min(lane, NT / 32u - 1)]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (lane == 0) sh.slot[0].a = __float_as_uint(best);
   }
   cluster_sync();
-  float top = -INFINITY;
-  for (int r = 0; r < (int)cluster_size(); ++r) top = fmaxf(top, __uint_as_float((uint32_t)ld_remote64(remote(&sh.slot[0].a, r))));
-  how = top == INFINITY ? kInfinite : top < -1e38f && top > -INFINITY ? kQuartered : kAsIs;
-  if (how != kAsIs) {
-    for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
-      float f[N];
-      sl.get(v, f);
+  const uint32_t c = cluster_size();
+  float top = lane < c ? __uint_as_float((uint32_t)ld_remote64(remote(&sh.slot[0].a, lane))) : -INFINITY;
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = rewritten(f[i], how);
-      sl.v[v] = Vec16<T>::pack(f);
-    }
-    __syncthreads();
-    top = rewritten(top, how);
-  }
-  return top;
+  for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  top = __shfl_sync(0xffffffffu, top, 0);
+  sl.how = top == INFINITY ? kInfinite : top < -1e38f && top > -INFINITY ? kQuartered : kAsIs;
+  return rewritten(top, sl.how);
 }
 // Lowest index of the largest logit (of a row that has one), through slot 1.
-template <typename T, int NT>
-__device__ int row_first(const Slice<T, NT>& sl, float top, Shared& sh) {
+template <typename T, int NT, bool kShared>
+__device__ int row_first(const Slice<T, NT, kShared>& sl, float top, Shared& sh) {
   constexpr int N = Vec16<T>::N;
   int at = 0x7fffffff;
-  for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
-    float f[N];
-    sl.get(v, f);
+  sl.each(threadIdx.x, sl.n_vec, NT, [&](const float (&f)[N], int i0) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (f[i] == top) at = min(at, sl.first + v * N + i);
-  }
+      if (f[i] == top) at = min(at, i0 + i);
+  });
   at = __reduce_min_sync(0xffffffffu, at);
   if ((threadIdx.x & 31) == 0) sh.warp_a[threadIdx.x >> 5] = (u64)at;
   __syncthreads();
@@ -332,9 +434,7 @@ __device__ int row_first(const Slice<T, NT>& sl, float top, Shared& sh) {
     sh.slot[1].a = m;
   }
   cluster_sync();
-  u64 m = ~0ull;
-  for (int r = 0; r < (int)cluster_size(); ++r) m = min(m, ld_remote64(remote(&sh.slot[1].a, r)));
-  return (int)m;
+  return (int)cluster_min(&sh.slot[1].a);
 }
 
 // Sums over the cluster of two integers per warp (in its lane 0), through slot `s`: the wholes, and what the CTAs before this
@@ -350,14 +450,20 @@ __device__ Slot cluster_total(u64 a, u64 b, Shared& sh, int s, u64& before) {
     if (lane == 0) { sh.slot[s].a = va; sh.slot[s].b = vb; }
   }
   cluster_sync();
-  const int c = cluster_size(), rank = cluster_rank();
-  Slot all = {0, 0};
-  before = 0;
-  for (int r = 0; r < c; ++r) {
-    const u64 v = ld_remote64(remote(&sh.slot[s].a, r));
-    if (r < rank) before += v;
-    all.a += v;
-    all.b += ld_remote64(remote(&sh.slot[s].b, r));
+  const int c = cluster_size();
+  Slot all;
+  if (c == 1) {
+    all = sh.slot[s];
+    before = 0;
+  } else {
+    const uint32_t l = lane;
+    u64 v = l < c ? ld_remote64(remote(&sh.slot[s].a, l)) : 0, w = l < c ? ld_remote64(remote(&sh.slot[s].b, l)) : 0;
+    u64 x = l < cluster_rank() ? v : 0;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) { v += shfl_xor64(v, o); w += shfl_xor64(w, o); x += shfl_xor64(x, o); }
+    all.a = __shfl_sync(0xffffffffu, v, 0);
+    all.b = __shfl_sync(0xffffffffu, w, 0);
+    before = __shfl_sync(0xffffffffu, x, 0);
   }
   return all;
 }
@@ -394,12 +500,18 @@ __device__ int hist_find(Shared& sh, int s, u64 extra, F limit_of, u64& limit, u
     v[i] = 0;
     if (i < per && b0 + i < bins) {
       const int b = rank * bins + b0 + i;
-      u64 lo = 0, hi = 0;
-      for (int r = 0; r < c; ++r) {
-        lo += ld_remote32(remote(&sh.hist_lo[b], r));
-        hi += ld_remote32(remote(&sh.hist_hi[b], r));
+      if (c == 1) {
+        v[i] = ((u64)sh.hist_hi[b] << 32) + sh.hist_lo[b];
+      } else {
+        uint32_t lo[kMaxCtas], hi[kMaxCtas];  // all in flight at once
+#pragma unroll
+        for (int r = 0; r < kMaxCtas; ++r) {
+          lo[r] = r < c ? ld_remote32(remote(&sh.hist_lo[b], r)) : 0;
+          hi[r] = r < c ? ld_remote32(remote(&sh.hist_hi[b], r)) : 0;
+        }
+#pragma unroll
+        for (int r = 0; r < kMaxCtas; ++r) v[i] += ((u64)hi[r] << 32) + lo[r];
       }
-      v[i] = (hi << 32) + lo;
     }
     mine += v[i];
   }
@@ -424,16 +536,13 @@ __device__ int hist_find(Shared& sh, int s, u64 extra, F limit_of, u64& limit, u
   before = all.a;
   if (all.a <= limit) return -1;
   cluster_sync();
-  int bin = -1;
-  for (int r = 0; r < c; ++r) {
-    const u64 x = ld_remote64(remote(&sh.slot[s + 1].a, r));
-    if (x != ~0ull) {
-      bin = (int)x;
-      before = ld_remote64(remote(&sh.slot[s + 1].b, r));
-      mass = ld_remote64(remote(&sh.slot[s + 2].a, r));
-    }
-  }
-  return bin;
+  const uint32_t l = lane < c ? lane : 0;
+  const u64 x = ld_remote64(remote(&sh.slot[s + 1].a, l)), y = ld_remote64(remote(&sh.slot[s + 1].b, l)),
+            z = ld_remote64(remote(&sh.slot[s + 2].a, l));
+  const int from = __ffs(__ballot_sync(0xffffffffu, x != ~0ull)) - 1;
+  before = __shfl_sync(0xffffffffu, y, from);
+  mass = __shfl_sync(0xffffffffu, z, from);
+  return (int)__shfl_sync(0xffffffffu, x, from);
 }
 
 // The kept tokens: those above `value`, and of those equal to it the ones up to index `index`.
@@ -449,118 +558,195 @@ __device__ __forceinline__ void set_border(Kept& k, u64 key) {
   k.index = kMaxVocab - 1 - (int)(key & (kMaxVocab - 1));
 }
 
-// Top-p border of the row. Without a cut the masses of the warps' segments are left in sh.seg. Slots 2 to 26.
-template <typename T, int NT>
-__device__ Kept find_kept(const Slice<T, NT>& sl, const RowScale& s, float top_p, Shared& sh) {
+// First index whose running sum of mass exceeds a target; sh.seg holds the masses of the subsegments, `mine` (per warp)
+// their sum. target_of(whole) gives the target, below the whole. The CTA that holds the index writes it to *out. Returns the
+// whole; 0: there is no mass. One slot.
+template <typename T, int NT, bool kShared, typename M, typename F>
+__device__ u64 locate(const Slice<T, NT, kShared>& sl, Shared& sh, int slot, u64 mine, M mass, F target_of, int32_t* out) {
+  constexpr int N = Vec16<T>::N, PER = NT / 32 * kSub / 32;  // subsegments of a lane
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 before;
+  const u64 all = cluster_total<NT>(mine, 0, sh, slot, before).a;
+  if (all == 0 || warp != 0) return all;
+  u64 target = target_of(all);
+  u64 own[PER], sum = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) { own[k] = sh.seg[lane * PER + k]; sum += own[k]; }
+  u64 inc = warp_scan(sum, lane);
+  const u64 cta = __shfl_sync(0xffffffffu, inc, 31);
+  if (target < before || target - before >= cta) return all;  // another CTA's
+  target -= before;
+  const int who = __ffs(__ballot_sync(0xffffffffu, inc > target)) - 1;
+  int which = 0;
+  u64 run = inc - sum;  // of the lane that holds it: its subsegment and what lies before
+  if (lane == who) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if (which == k && run + own[k] <= target) { run += own[k]; which = k + 1; }
+    }
+  }
+  which = who * PER + __shfl_sync(0xffffffffu, which, who);
+  target -= __shfl_sync(0xffffffffu, run, who);
+  const int w = which / kSub, a = min(sl.begin(w) + which % kSub * sl.sub, sl.end(w)), b = min(a + sl.sub, sl.end(w));
+  for (int v0 = a; v0 < b; v0 += 32) {
+    const int v = v0 + lane;
+    u64 m[N], total = 0;
+    float f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = -INFINITY;
+    if (v < b) sl.get(v, f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      m[i] = f[i] > -INFINITY ? mass(f[i], sl.first + v * N + i) : 0;
+      total += m[i];
+    }
+    inc = warp_scan(total, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, inc > target);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) {
+        run = inc - total;
+        int i = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          run += m[k];
+          if (run <= target) i = k + 1;
+        }
+        *out = sl.first + v * N + i;
+      }
+      break;
+    }
+    target -= __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return all;
+}
+
+// Top-p border of the row. Without a cut the masses of the subsegments are left in sh.seg (`mine`: the warp's). Slots 2 to 30.
+template <typename T, int NT, bool kShared>
+__device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, float top_p, Shared& sh, u64& mine) {
   constexpr int N = Vec16<T>::N;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Kept k;
   k.value = -INFINITY;
   k.index = -1;
   const int w0 = sl.begin(warp), w1 = sl.end(warp);
+  mine = 0;
   if (!(top_p < 1.f)) {  // NaN: no cut
-    u64 sum = 0, before;
-    for (int v = w0 + lane; v < w1; v += 32) {
-      float f[N];
-      sl.get(v, f);
+    mine = sl.sum(sh, [&](const float (&f)[N], int) {
+      u64 x = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum += raw_weight(f[i], s, sh.table);
-      sum -= N * kRaw;
-    }
-    sum = warp_sum(sum);
-    if (lane == 0) sh.seg[warp] = sum;
-    k.total = cluster_total<NT>(sum, 0, sh, 2, before).a;
+      for (int i = 0; i < N; ++i) x += raw_weight(f[i], s, sh.table);
+      return x - N * kRaw;
+    });
+    u64 before;
+    k.total = cluster_total<NT>(mine, 0, sh, 2, before).a;
     return k;
   }
-  // Histogram of the tokens within kWindow nats of the top; the others' weight is one sum. (The tail of a vocabulary is
-  // most of its entries and seldom holds the border: their atomics would cost more than all the rest.)
-  hist_clear<NT>(sh);
-  __syncthreads();
-  const float light = s.top - kWindow * s.t, near_scale = (float)kBins / (kWindow * s.t);
-  auto near_bin = [&](float l) { return min((int)((s.top - l) * near_scale), kBins - 1); };
-  u64 tail = 0;
-  for (int v = w0 + lane; v < w1; v += 32) {
-    float f[N];
-    sl.get(v, f);
-    u64 w[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = raw_weight(f[i], s, sh.table) - kRaw;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (f[i] >= light) hist_add(sh, near_bin(f[i]), w[i]);
-      else tail += w[i];
-    }
-  }
-  u64 limit, before, mass, lo = ~0ull, hi = 0;
-  const double share = (double)fmaxf(top_p, 0.f);
-  int bin = hist_find<NT>(sh, 3, warp_sum(tail), [&](u64 a, u64 b) { k.total = a + b; return (u64)(share * (double)(a + b)); }, limit,
-                          before, mass);
-  limit -= before;
-  u64 kept = before;
-  // The border lies in the tail: a histogram of it, over the 64 nats that hold any weight.
-  const bool far = bin < 0;
-  const float far_scale = (float)kBins / (56.f * s.t);
-  auto far_bin = [&](float l) { return min((int)(fmaxf(light - l, 0.f) * far_scale), kBins - 1); };
-  if (far) {
+  // Histograms over windows of kWindow nats: the first with the tokens near the top, everything behind it one sum. (The tail
+  // of a vocabulary is most of its entries and seldom holds the border: their atomics would cost more than all the rest.) Only
+  // when the border lies behind a window is the next one counted; the last reaches to where weights end.
+  u64 limit = 0, before, mass;
+  float from = INFINITY, base = s.top, to = s.top - kWindow * s.t, scale = (float)kBins / (kWindow * s.t);
+  int bin = -1;
+  u64 kept = 0;
+  for (int window = 0; bin < 0; ++window) {
     hist_clear<NT>(sh);  // (every CTA has read it: the cluster barrier in cluster_total)
     __syncthreads();
-    for (int v = w0 + lane; v < w1; v += 32) {
-      float f[N];
-      sl.get(v, f);
+    u64 tail = 0;
+    auto count = [&](float l, u64 w) { hist_add(sh, min((int)((base - l) * scale), kBins - 1), w); };
+    if (window == 0) {
+      sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int) {
+        unsigned in = 0;
+        u64 w[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const u64 w = raw_weight(f[i], s, sh.table) - kRaw;
-        if (w && !(f[i] >= light)) hist_add(sh, far_bin(f[i]), w);
-      }
+        for (int i = 0; i < N; ++i) {
+          w[i] = raw_weight(f[i], s, sh.table) - kRaw;
+          const bool near = f[i] >= to;
+          in |= near ? 1u << i : 0u;
+          tail += near ? 0 : w[i];
+        }
+        if (__popc(in) > 2) {
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (in >> i & 1) count(f[i], w[i]);
+        } else {
+          marked(f, in, [&](float l, int) { count(l, raw_weight(l, s, sh.table) - kRaw); });
+        }
+      });
+    } else {
+      sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int) {
+        unsigned in = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) in |= f[i] >= to && f[i] < from && f[i] > s.cutoff ? 1u << i : 0u;
+        marked(f, in, [&](float l, int) { count(l, raw_weight(l, s, sh.table) - kRaw); });
+      });
     }
-    u64 same;
-    bin = hist_find<NT>(sh, 6, 0, [&](u64, u64) { return limit; }, same, before, mass);
-    if (bin < 0) return k;  // cannot happen with top_p < 1: the whole exceeds the limit
-    limit -= before;
+    const double share = (double)fmaxf(top_p, 0.f);
+    u64 now;
+    bin = hist_find<NT>(sh, 3 + 3 * window, warp_sum(tail),
+                        [&](u64 a, u64 b) { return window == 0 ? (u64)(share * (double)(a + b)) : limit; }, now, before, mass);
+    limit = now - before;
     kept += before;
+    if (bin < 0) {
+      if (window == 2) {  // cannot happen with top_p < 1: the whole exceeds the limit
+        k.total = kept;
+        return k;
+      }
+      from = base = to;
+      to = window == 0 ? s.top - 2.f * kWindow * s.t : s.cutoff;
+      scale = (float)kBins / (window == 0 ? kWindow * s.t : (64.f - 2.f * kWindow) * s.t);
+    }
   }
-  // Members of the border's bin: listed, and the range of their rank keys.
-  for (int v = w0 + lane; v < w1; v += 32) {
-    float f[N];
-    sl.get(v, f);
+  // Members of the border's bin: listed, and the range of their rank keys. The values around the bin are found by two
+  // comparisons (with room for the rounding of the bin's arithmetic), the members among them by their bin.
+  const float width = 1.f / scale, slack = 1e-6f * (fabsf(base) + (float)(bin + 1) * width);
+  const float v_hi = base - (float)bin * width + slack, v_lo = bin == kBins - 1 ? to : base - (float)(bin + 1) * width - slack;
+  u64 lo = ~0ull, hi = 0;
+  sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int i0) {
+    unsigned in = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float l = f[i];
-      if (!(l > s.cutoff) || (l >= light) == far || (far ? far_bin(l) : near_bin(l)) != bin) continue;
-      const u64 key = rank_key<T>(l, sl.first + v * N + i);
+    for (int i = 0; i < N; ++i) in |= f[i] <= v_hi && f[i] >= v_lo ? 1u << i : 0u;
+    while (in) {
+      const int i = __ffs(in) - 1;
+      in &= in - 1;
+      float l = f[0];
+#pragma unroll
+      for (int j = 1; j < N; ++j) l = i == j ? f[j] : l;
+      if (!(l >= to && l < from && l > s.cutoff) || min((int)((base - l) * scale), kBins - 1) != bin) continue;
+      const u64 key = rank_key<T>(l, i0 + i);
       lo = min(lo, key);
       hi = max(hi, key);
       const int at = atomicAdd(&sh.n_list, 1);
       if (at < kList) sh.list[at] = key;
     }
-  }
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) { lo = min(lo, shfl_xor64(lo, o)); hi = max(hi, shfl_xor64(hi, o)); }
   if (lane == 0) { sh.warp_a[warp] = lo; sh.warp_b[warp] = hi; }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < NT / 32; ++w) { lo = min(lo, sh.warp_a[w]); hi = max(hi, sh.warp_b[w]); }
-    sh.slot[9].a = lo;
-    sh.slot[9].b = hi;
-    sh.slot[10].a = (u64)sh.n_list;
+  if (warp == 0) {
+    lo = lane < NT / 32 ? sh.warp_a[lane] : ~0ull;
+    hi = lane < NT / 32 ? sh.warp_b[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { lo = min(lo, shfl_xor64(lo, o)); hi = max(hi, shfl_xor64(hi, o)); }
+    if (lane == 0) {
+      sh.slot[12].a = lo;
+      sh.slot[12].b = hi;
+      sh.slot[13].a = (u64)sh.n_list;
+    }
   }
   cluster_sync();  // also: every CTA has read the histogram that is cleared next
-  int members = 0;
-  for (int r = 0; r < (int)cluster_size(); ++r) {
-    lo = min(lo, ld_remote64(remote(&sh.slot[9].a, r)));
-    hi = max(hi, ld_remote64(remote(&sh.slot[9].b, r)));
-    members += (int)min(ld_remote64(remote(&sh.slot[10].a, r)), (u64)1 << 20);
-  }
+  lo = cluster_min(&sh.slot[12].a);
+  hi = cluster_max(&sh.slot[12].b);
+  const int c = cluster_size();
+  const int members = (int)cluster_sum(&sh.slot[13].a, c);
   if (members <= kList) {  // few: every CTA ranks all of them
-    int base = 0;
-    for (int r = 0; r < (int)cluster_size(); ++r) {
-      const int n = (int)ld_remote64(remote(&sh.slot[10].a, r));
-      for (int i = threadIdx.x; i < n; i += NT) {
-        const u64 key = ld_remote64(remote(&sh.list[i], r));
-        sh.all_key[base + i] = key;
-        sh.all_w[base + i] = raw_weight(key_value<T>((uint32_t)(key >> kIndexBits)), s, sh.table) - kRaw;
+    if (warp < c) {  // warp r fetches CTA r's
+      const int n = (int)ld_remote64(remote(&sh.slot[13].a, warp)), first = (int)cluster_sum(&sh.slot[13].a, warp);
+      for (int i = lane; i < n; i += 32) {
+        const u64 key = ld_remote64(remote(&sh.list[i], warp));
+        sh.all_key[first + i] = key;
+        sh.all_w[first + i] = raw_weight(key_value<T>((uint32_t)(key >> kIndexBits)), s, sh.table) - kRaw;
       }
-      base += n;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < members; i += NT) {
@@ -577,28 +763,54 @@ __device__ Kept find_kept(const Slice<T, NT>& sl, const RowScale& s, float top_p
     k.total = kept + sh.kept;
     return k;
   }
-  for (int s0 = 11;; s0 += 3) {  // 50 bits of rank key, 11 a round: five rounds at most
+  if ((lo >> kIndexBits) == (hi >> kIndexBits)) {  // many, but of one value (16-bit logits): the ones with the lowest indices
+    set_border<T>(k, lo);
+    const u64 w = raw_weight(k.value, s, sh.table) - kRaw, n = limit / w + 1;
+    k.total = kept + n * w;
+    if (threadIdx.x == 0) sh.tie = -1;
+    const float value = k.value;
+    const u64 count = sl.sum(sh, [&](const float (&f)[N], int) {
+      int x = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x += f[i] == value ? 1 : 0;
+      return (u64)x;
+    });
+    locate(sl, sh, 14, count, [&](float l, int) { return l == value ? (u64)1 : 0; }, [&](u64) { return n - 1; }, &sh.tie);
+    __syncthreads();
+    if (threadIdx.x == 0) sh.slot[15].a = (u64)(sh.tie + 1);
+    cluster_sync();
+    k.index = (int)cluster_max(&sh.slot[15].a) - 1;
+    return k;
+  }
+  for (int s0 = 16;; s0 += 3) {  // 50 bits of rank key, 11 a round: five rounds at most
     const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 11);
     hist_clear<NT>(sh);
     __syncthreads();
-    for (int v = w0 + lane; v < w1; v += 32) {
-      float f[N];
-      sl.get(v, f);
+    sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int i0) {
+      unsigned in = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (!(f[i] > s.cutoff)) continue;
-        const u64 key = rank_key<T>(f[i], sl.first + v * N + i);
-        if (key >= lo && key <= hi) hist_add(sh, (int)((hi - key) >> shift), raw_weight(f[i], s, sh.table) - kRaw);
+      for (int i = 0; i < N; ++i) in |= f[i] <= v_hi && f[i] >= v_lo && f[i] > s.cutoff ? 1u << i : 0u;
+      while (in) {
+        const int i = __ffs(in) - 1;
+        in &= in - 1;
+        float l = f[0];
+#pragma unroll
+        for (int j = 1; j < N; ++j) l = i == j ? f[j] : l;
+        const u64 key = rank_key<T>(l, i0 + i);
+        if (key >= lo && key <= hi) hist_add(sh, (int)((hi - key) >> shift), raw_weight(l, s, sh.table) - kRaw);
       }
-    }
+    });
     u64 same;
     bin = hist_find<NT>(sh, s0, 0, [&](u64, u64) { return limit; }, same, before, mass);
-    if (bin < 0) return k;  // cannot happen: the members' mass exceeds the limit
+    if (bin < 0) {  // cannot happen: the members' mass exceeds the limit
+      k.total = kept + before;
+      return k;
+    }
     limit -= before;
     kept += before;
     hi -= (u64)bin << shift;
-    const u64 width = (1ull << shift) - 1;
-    lo = hi - lo > width ? hi - width : lo;
+    const u64 wide = (1ull << shift) - 1;
+    lo = hi - lo > wide ? hi - wide : lo;
     if (shift == 0) {
       set_border<T>(k, hi);
       k.total = kept + mass;
@@ -615,9 +827,8 @@ struct Mass {
   const float* minus;   // row of the draft distribution to subtract, or null
   int one_hot;          // or the token whose draft probability is 1, or -1
   bool residual;
-  __device__ __forceinline__ u64 operator()(float l, int i, const Shared& sh) const {
-    if (!kept.holds(l, i)) return 0;  // NaN and -inf are never kept
-    u64 w = raw_weight(l, s, sh.table) - kRaw;
+  __device__ __forceinline__ u64 of_kept(float l, int i, const double* table) const {
+    u64 w = raw_weight(l, s, table) - kRaw;
     if (residual && w) {
       const double q = minus != nullptr ? (double)__ldg(minus + i) : i == one_hot ? 1.0 : 0.0;
       const double r = (double)w * inv_z - q;
@@ -627,80 +838,30 @@ struct Mass {
   }
 };
 
-// First index whose running sum of mass exceeds u * (whole sum). The CTA that holds it writes it to *out; false when
-// there is no mass. `ready`: sh.seg holds the masses of the warps' segments already.
-template <typename T, int NT>
-__device__ bool draw(const Slice<T, NT>& sl, const Mass& mass, float u, bool ready, int slot, int32_t* out, Shared& sh) {
-  constexpr int N = Vec16<T>::N, W = NT / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto sum_of = [&](int a, int b) {
-    u64 sum = 0;
-    for (int v = a + lane; v < b; v += 32) {
-      float f[N];
-      sl.get(v, f);
-#pragma unroll
-      for (int i = 0; i < N; ++i) sum += mass(f[i], sl.first + v * N + i, sh);
-    }
-    return warp_sum(sum);
-  };
+// First index whose running sum of mass exceeds u * (whole sum); false when there is no mass. `ready`: sh.seg holds the masses
+// of the subsegments already, `mine` the warp's.
+template <typename T, int NT, bool kShared>
+__device__ bool draw(const Slice<T, NT, kShared>& sl, const Mass& mass, float u, bool ready, u64 mine, int slot, int32_t* out, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
   if (!ready) {
-    const u64 sum = sum_of(sl.begin(warp), sl.end(warp));
-    if (lane == 0) sh.seg[warp] = sum;
-  }
-  __syncthreads();
-  u64 before;
-  const u64 all = cluster_total<NT>(sh.seg[warp], 0, sh, slot, before).a;
-  if (all == 0) return false;
-  const double x = u > 0.f ? (double)u * (double)all : 0.0;  // NaN: 0
-  u64 target = x < (double)all ? min((u64)x, all - 1) : all - 1;
-  u64 mine = 0;
-  for (int w = 0; w < W; ++w) mine += sh.seg[w];
-  if (target < before || target - before >= mine) return true;  // another CTA's
-  target -= before;
-  int w = 0;
-  while (w < W - 1 && target >= sh.seg[w]) target -= sh.seg[w++];
-  // the warps share that segment
-  const int begin = sl.begin(w), end = sl.end(w);
-  const int sub = (end - begin + W - 1) / W;
-  const int a = min(begin + warp * sub, end), b = min(a + sub, end);
-  const u64 sum = sum_of(a, b);
-  __syncthreads();
-  if (lane == 0) sh.warp_b[warp] = sum;
-  __syncthreads();
-  w = 0;
-  while (w < W - 1 && target >= sh.warp_b[w]) target -= sh.warp_b[w++];
-  if (warp != w) return true;
-  for (int v0 = a; v0 < b; v0 += 32) {
-    const int v = v0 + lane;
-    u64 m[N], total = 0;
-    float f[N];
-    if (v < b) sl.get(v, f);
+    mine = sl.sum(sh, [&](const float (&f)[N], int at) {
+      unsigned in = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      m[i] = v < b ? mass(f[i], sl.first + v * N + i, sh) : 0;
-      total += m[i];
-    }
-    const u64 inc = warp_scan(total, lane);
-    const unsigned hit = __ballot_sync(0xffffffffu, inc > target);
-    if (hit) {
-      if (lane == __ffs(hit) - 1) {
-        u64 run = inc - total;
-        int i = 0;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          run += m[k];
-          if (run <= target) i = k + 1;
-        }
-        *out = sl.first + v * N + i;
-      }
-      break;
-    }
-    target -= __shfl_sync(0xffffffffu, inc, 31);
+      for (int i = 0; i < N; ++i) in |= f[i] >= mass.kept.value && mass.kept.holds(f[i], at + i) ? 1u << i : 0u;
+      u64 x = 0;
+      marked(f, in, [&](float l, int i) { x += mass.of_kept(l, at + i, sh.table); });
+      return x;
+    });
   }
-  return true;
+  return locate(sl, sh, slot, mine, [&](float l, int i) { return mass.kept.holds(l, i) ? mass.of_kept(l, i, sh.table) : 0; },
+                [&](u64 all) {
+                  const double x = u > 0.f ? (double)u * (double)all : 0.0;  // NaN: 0
+                  return x < (double)all ? min((u64)x, all - 1) : all - 1;
+                },
+                out) != 0;
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool kShared>
 __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ __align__(16) Shared sh;
@@ -709,9 +870,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const float t = __ldg(p.temperature + r), top_p = __ldg(p.top_p + r), u = __ldg(p.uniform + r);
   float best;
-  int how;
-  const Slice<T, NT> sl = load_slice<T, NT>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best);
-  const float top = row_top(sl, best, how, sh);
+  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best, sh);
+  const float top = row_top(sl, best, sh);
   const int begin = min((int)cluster_rank() * p.slice, p.vocab), end = min(begin + p.slice, p.vocab);
   float* probs = p.probs == nullptr ? nullptr : p.probs + (int64_t)r * p.probs_stride;
   if (!(t > 0.f) || top == -INFINITY) {  // greedy, or a row without a token
@@ -721,13 +881,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
       for (int i = begin + threadIdx.x; i < end; i += NT) probs[i] = i == first ? 1.f : 0.f;
   } else {
     Mass mass;
-    mass.s = row_scale(top, how == kQuartered ? t * 0.25f : t);
-    mass.kept = find_kept(sl, mass.s, top_p, sh);
+    mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
+    u64 mine;
+    mass.kept = find_kept(sl, mass.s, top_p, sh, mine);
     mass.residual = false;
     mass.inv_z = 0.0; mass.minus = nullptr; mass.one_hot = -1;
-    draw(sl, mass, u, !(top_p < 1.f), 27, p.tokens + r, sh);
+    draw(sl, mass, u, !(top_p < 1.f), mine, 32, p.tokens + r, sh);
     if (probs != nullptr) {
-      const float inv = (float)(mass.s.one / (double)mass.kept.total);
+      const float inv = (float)(top_weight(mass.s) / (double)mass.kept.total);
       for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
         float f[N];
         sl.get(v, f);
@@ -755,18 +916,15 @@ __device__ __forceinline__ int owner_of(const int32_t* __restrict__ indptr, int 
 // unless they come too close (1e-5 bounds their error: 2^-22 of ex2.approx, 2^-23 of the exponent's size, which the
 // weights average to at most log2 of the vocabulary, 128 additions), or the nucleus' exact mass is needed: Z lies
 // between top_p and 1 times the whole sum. 1: yes, 0: no, -1: not known.
-template <typename T, int NT>
-__device__ int quick_test(const Slice<T, NT>& sl, const RowScale& s, float top_p, int x, float lx, double wx, double uq, Shared& sh) {
+template <typename T, int NT, bool kShared>
+__device__ int quick_test(const Slice<T, NT, kShared>& sl, const RowScale& s, float top_p, int x, float lx, double wx, double uq, Shared& sh) {
   constexpr int N = Vec16<T>::N;
   constexpr double kFix = 1099511627776.0, kGuard = 4e-5;  // 2^40
   float all = 0.f, above = 0.f;
   const bool cut = top_p < 1.f;
   u64 fall = 0, fabove = 0;
   int n = 0;
-  for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
-    float f[N];
-    sl.get(v, f);
-    const int i0 = sl.first + v * N;
+  sl.each(threadIdx.x, sl.n_vec, NT, [&](const float (&f)[N], int i0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float w = ex2((fmaxf(f[i], s.cutoff) - s.top) * s.c32);
@@ -779,11 +937,11 @@ __device__ int quick_test(const Slice<T, NT>& sl, const RowScale& s, float top_p
       all = above = 0.f;
       n = 0;
     }
-  }
+  });
   fall = warp_sum(fall + (u64)(all * (float)kFix));
   fabove = warp_sum(fabove + (u64)(above * (float)kFix));
   u64 before;
-  const Slot sum = cluster_total<NT>(fall, fabove, sh, 28, before);
+  const Slot sum = cluster_total<NT>(fall, fabove, sh, 31, before);
   const double total = (double)sum.a / kFix, ahead = (double)sum.b / kFix;
   double least = total;  // of Z
   if (cut) {
@@ -797,7 +955,7 @@ __device__ int quick_test(const Slice<T, NT>& sl, const RowScale& s, float top_p
 }
 
 // One cluster per row that has a draft behind it: is the draft accepted?
-template <typename T, int NT>
+template <typename T, int NT, bool kShared>
 __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ __align__(16) Shared sh;
@@ -813,19 +971,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Sample
   const double q = p.draft_probs == nullptr || !token ? 1.0 : (double)__ldg(p.draft_probs + (int64_t)r * p.draft_stride + x);
   const double uq = (double)__ldg(p.uniform + r) * q;
   float best;
-  int how, ok = 0;
-  const Slice<T, NT> sl = load_slice<T, NT>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best);
-  const float top = row_top(sl, best, how, sh), l = rewritten(lx, how);
+  int ok = 0;
+  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best, sh);
+  const float top = row_top(sl, best, sh), l = rewritten(lx, sl.how);
   if (l > -INFINITY) {  // a token (and so the row has a top)
     if (!(t > 0.f)) {
       ok = l == top && row_first(sl, top, sh) == x && uq < 1.0;
     } else {
-      const RowScale s = row_scale(top, how == kQuartered ? t * 0.25f : t);
+      const RowScale s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
       const double wx = weight(l, s);
       ok = quick_test(sl, s, top_p, x, l, wx, uq, sh);
       if (ok < 0) {
-        const Kept k = find_kept(sl, s, top_p, sh);
-        ok = k.holds(l, x) && uq < wx * (s.one / (double)k.total);
+        u64 mine;
+        const Kept k = find_kept(sl, s, top_p, sh, mine);
+        ok = k.holds(l, x) && uq < wx * (top_weight(s) / (double)k.total);
       }
     }
   }
@@ -835,7 +994,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Sample
 
 // One cluster per request: the accepted prefix, then a draw from the residual of the first rejected row or
 // from the last row.
-template <typename T, int NT>
+template <typename T, int NT, bool kShared>
 __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ __align__(16) Shared sh;
@@ -856,24 +1015,24 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const float t = __ldg(p.temperature + req), top_p = __ldg(p.top_p + req), u = __ldg(p.uniform + end - 1);
   float best;
-  int how;
-  const Slice<T, NT> sl = load_slice<T, NT>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best);
-  const float top = row_top(sl, best, how, sh);
+  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best, sh);
+  const float top = row_top(sl, best, sh);
   if (lead) p.accepted[req] = r - begin;
   if (!(t > 0.f) || top == -INFINITY) {
     const int first = top == -INFINITY ? 0 : row_first(sl, top, sh);
     if (lead) p.tokens[req] = first;
   } else {
     Mass mass;
-    mass.s = row_scale(top, how == kQuartered ? t * 0.25f : t);
-    mass.kept = find_kept(sl, mass.s, top_p, sh);
+    mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
+    u64 mine;
+    mass.kept = find_kept(sl, mass.s, top_p, sh, mine);
     mass.inv_z = 1.0 / (double)mass.kept.total;
     mass.residual = rejected;
     mass.minus = rejected && p.draft_probs != nullptr ? p.draft_probs + (int64_t)r * p.draft_stride : nullptr;
     mass.one_hot = rejected ? __ldg(p.draft + r + 1) : -1;
-    if (!draw(sl, mass, u, !rejected && !(top_p < 1.f), 29, p.tokens + req, sh)) {
+    if (!draw(sl, mass, u, !rejected && !(top_p < 1.f), mine, 33, p.tokens + req, sh)) {
       mass.residual = false;  // nothing left above the draft's distribution: the target's own
-      draw(sl, mass, u, false, 30, p.tokens + req, sh);
+      draw(sl, mass, u, false, 0, 34, p.tokens + req, sh);
     }
   }
   cluster_sync();
@@ -882,19 +1041,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
 // ---- host --------------------------------------------------------------------------------------------
 struct Shape {
   int ctas, slice;
-  bool wide;  // 512 threads, else 256
+  bool shared;  // rows in shared memory, 512 threads; else in L2, 256 threads
   size_t smem;
 };
-// CTAs of a row: as few as keep a slice within 32 KB, four CTAs of 256 threads per SM, so that some load while others
-// compute; where all rows fit the SMs at once anyway, more CTAs (up to 8, slices of 2048 entries at least) of 512 threads.
+// Few rows: as many CTAs (up to 8) per row as the SMs have room for, the row in shared memory. Many rows: one CTA per
+// row and four per SM, later passes from L2 (592 rows at once, so 128,256 entries of 16 bits for each just about fill
+// its 126 MB); the CTAs of a cluster wait for one another at every exchange, which costs more than reading L2.
 Shape pick_shape(int rows, int vocab, int es) {
   Shape s;
   s.ctas = 1;
-  while (s.ctas < kMaxCtas && (int64_t)vocab * es > (int64_t)s.ctas * 32768) s.ctas *= 2;
-  while (s.ctas < kMaxCtas && (int64_t)rows * s.ctas * 2 <= 148 && vocab / (s.ctas * 2) >= 2048) s.ctas *= 2;
-  s.wide = (int64_t)rows * s.ctas <= 148;
+  while (s.ctas < kMaxCtas && (int64_t)rows * s.ctas * 2 <= 296 && vocab / (s.ctas * 2) >= 2048) s.ctas *= 2;
   s.slice = ((vocab + s.ctas - 1) / s.ctas + 63) & ~63;
   s.smem = (size_t)s.slice * es + 32;
+  s.shared = (int64_t)rows * s.ctas <= 296 && s.smem <= 80 * 1024;
+  if (!s.shared) s.smem = 0;
   return s;
 }
 
@@ -940,7 +1100,8 @@ int dsv_sample_top_p(const void* logits, int64_t row_stride, int rows, int vocab
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
-    return shape.wide ? launch<512>(sample_kernel<T, 512>, rows, shape, p, st) : launch<256>(sample_kernel<T, 256>, rows, shape, p, st);
+    return shape.shared ? launch<512>(sample_kernel<T, 512, true>, rows, shape, p, st)
+                        : launch<256>(sample_kernel<T, 256, false>, rows, shape, p, st);
   };
   const cudaError_t e = dtype == DSV_F32 ? go(float{}) : dtype == DSV_F16 ? go(__half{}) : go(__nv_bfloat16{});
   if (e != cudaSuccess) return fail(DSV_E_CUDA, "sample_top_p launch failed: %s", cudaGetErrorString(e));
@@ -973,14 +1134,14 @@ int dsv_verify_draft(const void* logits, int64_t row_stride, int nnz, int vocab,
     if (nnz > 0) {
       const Shape shape = pick_shape(nnz, vocab, elem_size(dtype));
       p.slice = shape.slice;
-      const cudaError_t er = shape.wide ? launch<512>(verify_rows_kernel<T, 512>, nnz, shape, p, st)
-                                        : launch<256>(verify_rows_kernel<T, 256>, nnz, shape, p, st);
+      const cudaError_t er = shape.shared ? launch<512>(verify_rows_kernel<T, 512, true>, nnz, shape, p, st)
+                                        : launch<256>(verify_rows_kernel<T, 256, false>, nnz, shape, p, st);
       if (er != cudaSuccess) return er;
     }
     const Shape shape = pick_shape(batch, vocab, elem_size(dtype));
     p.slice = shape.slice;
-    return shape.wide ? launch<512>(verify_draw_kernel<T, 512>, batch, shape, p, st)
-                      : launch<256>(verify_draw_kernel<T, 256>, batch, shape, p, st);
+    return shape.shared ? launch<512>(verify_draw_kernel<T, 512, true>, batch, shape, p, st)
+                      : launch<256>(verify_draw_kernel<T, 256, false>, batch, shape, p, st);
   };
   const cudaError_t e = dtype == DSV_F32 ? go(float{}) : dtype == DSV_F16 ? go(__half{}) : go(__nv_bfloat16{});
   if (e != cudaSuccess) return fail(DSV_E_CUDA, "verify_draft launch failed: %s", cudaGetErrorString(e));

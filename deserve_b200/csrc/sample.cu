@@ -78,24 +78,26 @@ struct SampleParams {
   int32_t* accepted;
   int batch, nnz;
   int slice;             // entries of a CTA
+  int cap;               // entries of a warp's list
   int* status;
 };
 
 // What the CTAs of a cluster show one another. Every exchange uses a slot of its own, so one cluster
 // barrier per exchange is enough.
 struct Slot {
-  u64 a, b;
+  u64 a, b, c;
 };
 struct Shared {
   uint32_t hist_lo[kBins], hist_hi[kBins];
   double table[kTable];  // 2^(j / 64 + 44)
   Slot slot[36];
-  u64 warp_a[kMaxWarps], warp_b[kMaxWarps];
+  u64 warp_a[kMaxWarps], warp_b[kMaxWarps], warp_c[kMaxWarps];
   u64 seg[kMaxWarps * kSub];  // mass of the subsegments
   u64 list[kList];       // this CTA's members of the border's bin
   u64 all_key[kList], all_w[kList];
   int n_list;
   int32_t tie;
+  int near_n[kMaxWarps];
   u64 border, kept;
 };
 
@@ -313,6 +315,29 @@ struct Slice {
       u1 = u2;
     }
   }
+  // The same for the warp's 32 lanes together: of(values, first index) runs in all of them, with -inf behind the end.
+  template <typename F>
+  __device__ __forceinline__ void each_warp(int a, int b, F of) const {
+    const int lane = threadIdx.x & 31;
+    float f[N];
+    uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0, u2 = u0;
+    if (!kShared && a + lane < b) u0 = ld_stream16(v + a + lane);
+    if (!kShared && a + 32 + lane < b) u1 = ld_stream16(v + a + 32 + lane);
+    for (int i0 = a; i0 < b; i0 += 32) {
+      const int i = i0 + lane;
+      if (kShared) u0 = v[min(i, b - 1)];
+      else if (i + 64 < b) u2 = ld_stream16(v + i + 64);
+      Vec16<T>::unpack(u0, f);
+      finish(i, f);
+      if (i >= b) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[k] = -INFINITY;
+      }
+      of(f, first + i * N);
+      u0 = u1;
+      u1 = u2;
+    }
+  }
   __device__ __forceinline__ int begin(int warp) const { return min(warp * seg, n_vec); }
   __device__ __forceinline__ int end(int warp) const { return min(warp * seg + seg, n_vec); }
   // Sum of `of(values, first index)` over every subsegment of the warp, into sh.seg; the warp's total.
@@ -437,34 +462,33 @@ __device__ int row_first(const Slice<T, NT, kShared>& sl, float top, Shared& sh)
   return (int)cluster_min(&sh.slot[1].a);
 }
 
-// Sums over the cluster of two integers per warp (in its lane 0), through slot `s`: the wholes, and what the CTAs before this
-// one have of the first.
+// Sums over the cluster of up to three integers per warp (in its lane 0), through slot `s`: the wholes, and what the CTAs
+// before this one have of the first. The warps' first integers stay in sh.warp_a.
 template <int NT>
-__device__ Slot cluster_total(u64 a, u64 b, Shared& sh, int s, u64& before) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ Slot cluster_total(u64 a, u64 b, u64 c, Shared& sh, int s, u64& before) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __syncthreads();
-  if (lane == 0) { sh.warp_a[warp] = a; sh.warp_b[warp] = b; }
+  if (lane == 0) { sh.warp_a[warp] = a; sh.warp_b[warp] = b; sh.warp_c[warp] = c; }
   __syncthreads();
-  if (warp == 0) {
-    const u64 va = warp_sum(lane < NT / 32 ? sh.warp_a[lane] : 0), vb = warp_sum(lane < NT / 32 ? sh.warp_b[lane] : 0);
-    if (lane == 0) { sh.slot[s].a = va; sh.slot[s].b = vb; }
+  if (warp < 3) {
+    const u64 v = warp_sum(lane < NT / 32 ? (warp == 0 ? sh.warp_a : warp == 1 ? sh.warp_b : sh.warp_c)[lane] : 0);
+    if (lane == 0) (warp == 0 ? sh.slot[s].a : warp == 1 ? sh.slot[s].b : sh.slot[s].c) = v;
   }
   cluster_sync();
-  const int c = cluster_size();
-  Slot all;
-  if (c == 1) {
-    all = sh.slot[s];
+  const uint32_t n = cluster_size();
+  if (n == 1) {
     before = 0;
-  } else {
-    const uint32_t l = lane;
-    u64 v = l < c ? ld_remote64(remote(&sh.slot[s].a, l)) : 0, w = l < c ? ld_remote64(remote(&sh.slot[s].b, l)) : 0;
-    u64 x = l < cluster_rank() ? v : 0;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) { v += shfl_xor64(v, o); w += shfl_xor64(w, o); x += shfl_xor64(x, o); }
-    all.a = __shfl_sync(0xffffffffu, v, 0);
-    all.b = __shfl_sync(0xffffffffu, w, 0);
-    before = __shfl_sync(0xffffffffu, x, 0);
+    return sh.slot[s];
   }
+  u64 v = lane < n ? ld_remote64(remote(&sh.slot[s].a, lane)) : 0, w = lane < n ? ld_remote64(remote(&sh.slot[s].b, lane)) : 0,
+      y = lane < n ? ld_remote64(remote(&sh.slot[s].c, lane)) : 0, x = lane < cluster_rank() ? v : 0;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) { v += shfl_xor64(v, o); w += shfl_xor64(w, o); x += shfl_xor64(x, o); y += shfl_xor64(y, o); }
+  Slot all;
+  all.a = __shfl_sync(0xffffffffu, v, 0);
+  all.b = __shfl_sync(0xffffffffu, w, 0);
+  all.c = __shfl_sync(0xffffffffu, y, 0);
+  before = __shfl_sync(0xffffffffu, x, 0);
   return all;
 }
 
@@ -484,11 +508,9 @@ __device__ __forceinline__ void hist_clear(Shared& sh) {
 }
 
 // First bin of the cluster's summed histogram whose inclusive running sum exceeds a limit, the sum before it and its own
-// mass; -1: none, `before` is the whole. `extra` (per warp, lane 0) is summed over the cluster along with it;
-// limit_of(histogram's whole, extra's whole) gives the limit. Each CTA sums its share of the bins over the cluster. Slots
-// s to s + 2.
-template <int NT, typename F>
-__device__ int hist_find(Shared& sh, int s, u64 extra, F limit_of, u64& limit, u64& before, u64& mass) {
+// mass; -1: none, `before` is the whole. Each CTA sums its share of the bins over the cluster. Slots s to s + 2.
+template <int NT>
+__device__ int hist_find(Shared& sh, int s, u64 limit, u64& before, u64& mass) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = cluster_size(), rank = cluster_rank();
   constexpr int MAX = kBins / NT;
   const int bins = kBins / c, per = max(1, bins / NT);  // bins of this CTA, of a thread
@@ -518,8 +540,7 @@ __device__ int hist_find(Shared& sh, int s, u64 extra, F limit_of, u64& limit, u
   const u64 inc = warp_scan(mine, lane), warp_mass = __shfl_sync(0xffffffffu, inc, 31);
   if (threadIdx.x == 0) sh.slot[s + 1].a = ~0ull;
   u64 cta_before, base = 0;
-  const Slot all = cluster_total<NT>(warp_mass, extra, sh, s, cta_before);
-  limit = limit_of(all.a, all.b);
+  const Slot all = cluster_total<NT>(warp_mass, 0, 0, sh, s, cta_before);
   for (int w = 0; w < warp; ++w) base += sh.warp_a[w];
   u64 at = cta_before + base + inc - mine;
   if (at <= limit && at + mine > limit) {
@@ -546,6 +567,20 @@ __device__ int hist_find(Shared& sh, int s, u64 extra, F limit_of, u64& limit, u
 }
 
 // The kept tokens: those above `value`, and of those equal to it the ones up to index `index`.
+// A warp's entries within kWindow nats of the top, in index order. They are a small part of most rows, and where all of them
+// are held and the border lies among them, nothing behind them is looked at again.
+struct Entry {
+  u64 w;
+  float l;
+  int i;
+};
+struct Near {
+  Entry* all;  // of the CTA: `cap` for each warp
+  int cap, n;  // entries of this warp (n > cap: not all are held)
+  bool usable;
+  __device__ __forceinline__ Entry* mine() const { return all + (threadIdx.x >> 5) * cap; }
+};
+
 struct Kept {
   float value;
   int index;
@@ -566,7 +601,7 @@ __device__ u64 locate(const Slice<T, NT, kShared>& sl, Shared& sh, int slot, u64
   constexpr int N = Vec16<T>::N, PER = NT / 32 * kSub / 32;  // subsegments of a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 before;
-  const u64 all = cluster_total<NT>(mine, 0, sh, slot, before).a;
+  const u64 all = cluster_total<NT>(mine, 0, 0, sh, slot, before).a;
   if (all == 0 || warp != 0) return all;
   u64 target = target_of(all);
   u64 own[PER], sum = 0;
@@ -622,14 +657,17 @@ __device__ u64 locate(const Slice<T, NT, kShared>& sl, Shared& sh, int slot, u64
 
 // Top-p border of the row. Without a cut the masses of the subsegments are left in sh.seg (`mine`: the warp's). Slots 2 to 30.
 template <typename T, int NT, bool kShared>
-__device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, float top_p, Shared& sh, u64& mine) {
+__device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, float top_p, Near& near, Shared& sh, u64& mine) {
   constexpr int N = Vec16<T>::N;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Kept k;
   k.value = -INFINITY;
   k.index = -1;
   const int w0 = sl.begin(warp), w1 = sl.end(warp);
+  u64 before;
   mine = 0;
+  near.n = 0;
+  near.usable = false;
   if (!(top_p < 1.f)) {  // NaN: no cut
     mine = sl.sum(sh, [&](const float (&f)[N], int) {
       u64 x = 0;
@@ -637,88 +675,118 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
       for (int i = 0; i < N; ++i) x += raw_weight(f[i], s, sh.table);
       return x - N * kRaw;
     });
-    u64 before;
-    k.total = cluster_total<NT>(mine, 0, sh, 2, before).a;
+    k.total = cluster_total<NT>(mine, 0, 0, sh, 2, before).a;
     return k;
   }
-  // Histograms over windows of kWindow nats: the first with the tokens near the top, everything behind it one sum. (The tail
-  // of a vocabulary is most of its entries and seldom holds the border: their atomics would cost more than all the rest.) Only
-  // when the border lies behind a window is the next one counted; the last reaches to where weights end.
-  u64 limit = 0, before, mass;
+  // One walk gives the sums of the tokens near the top and of the others, and the list of the former.
   float from = INFINITY, base = s.top, to = s.top - kWindow * s.t, scale = (float)kBins / (kWindow * s.t);
-  int bin = -1;
-  u64 kept = 0;
-  for (int window = 0; bin < 0; ++window) {
-    hist_clear<NT>(sh);  // (every CTA has read it: the cluster barrier in cluster_total)
-    __syncthreads();
-    u64 tail = 0;
-    auto count = [&](float l, u64 w) { hist_add(sh, min((int)((base - l) * scale), kBins - 1), w); };
-    if (window == 0) {
-      sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int) {
-        unsigned in = 0;
-        u64 w[N];
+  u64 tail = 0, sum = 0;
+  Entry* list = near.mine();
+  sl.each_warp(w0, w1, [&](const float (&f)[N], int i0) {
+    unsigned in = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          w[i] = raw_weight(f[i], s, sh.table) - kRaw;
-          const bool near = f[i] >= to;
-          in |= near ? 1u << i : 0u;
-          tail += near ? 0 : w[i];
-        }
-        if (__popc(in) > 2) {
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (in >> i & 1) count(f[i], w[i]);
-        } else {
-          marked(f, in, [&](float l, int) { count(l, raw_weight(l, s, sh.table) - kRaw); });
-        }
-      });
-    } else {
-      sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int) {
-        unsigned in = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) in |= f[i] >= to && f[i] < from && f[i] > s.cutoff ? 1u << i : 0u;
-        marked(f, in, [&](float l, int) { count(l, raw_weight(l, s, sh.table) - kRaw); });
-      });
+    for (int i = 0; i < N; ++i) {
+      tail += raw_weight(f[i], s, sh.table);
+      in |= f[i] >= to ? 1u << i : 0u;
     }
-    const double share = (double)fmaxf(top_p, 0.f);
-    u64 now;
-    bin = hist_find<NT>(sh, 3 + 3 * window, warp_sum(tail),
-                        [&](u64 a, u64 b) { return window == 0 ? (u64)(share * (double)(a + b)) : limit; }, now, before, mass);
-    limit = now - before;
-    kept += before;
-    if (bin < 0) {
-      if (window == 2) {  // cannot happen with top_p < 1: the whole exceeds the limit
-        k.total = kept;
-        return k;
+    tail -= N * kRaw;
+    const int n = __popc(in);
+    if (__any_sync(0xffffffffu, n)) {
+      int at = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += t;
       }
-      from = base = to;
-      to = window == 0 ? s.top - 2.f * kWindow * s.t : s.cutoff;
-      scale = (float)kBins / (window == 0 ? kWindow * s.t : (64.f - 2.f * kWindow) * s.t);
+      const int total = __shfl_sync(0xffffffffu, at, 31);
+      at += near.n - n;
+      while (in) {
+        const int i = __ffs(in) - 1;
+        in &= in - 1;
+        float l = f[0];
+#pragma unroll
+        for (int j = 1; j < N; ++j) l = i == j ? f[j] : l;
+        const u64 w = raw_weight(l, s, sh.table) - kRaw;  // evaluated again
+        sum += w;
+        if (at < near.cap) list[at] = {w, l, i0 + i};
+        ++at;
+      }
+      near.n += total;
+    }
+  });
+  if (lane == 0) sh.near_n[warp] = near.n;
+  const Slot whole = cluster_total<NT>(warp_sum(sum), warp_sum(tail), (u64)near.n + (near.n > near.cap ? 1ull << 40 : 0), sh, 2, before);
+  k.total = whole.b;
+  u64 limit = (u64)((double)fmaxf(top_p, 0.f) * (double)whole.b), mass, kept = 0;
+  near.usable = limit < whole.a && whole.c < 1ull << 40;
+  int bin = -1, window = 0;
+  if (!(near.usable && whole.c <= kList)) {
+    // Histograms over windows of kWindow nats, the last one to where weights end. (The tail of a vocabulary is most of its
+    // entries and seldom holds the border.)
+    for (; bin < 0; ++window) {
+      if (window > 0 || limit >= whole.a) {
+        if (window == 0) {
+          limit -= whole.a;
+          kept = whole.a;
+          window = 1;
+        }
+        if (window == 3) {  // cannot happen with top_p < 1: the whole exceeds the limit
+          k.total = kept;
+          return k;
+        }
+        from = base = to;
+        to = window == 1 ? s.top - 2.f * kWindow * s.t : s.cutoff;
+        scale = (float)kBins / (window == 1 ? kWindow * s.t : (64.f - 2.f * kWindow) * s.t);
+      }
+      hist_clear<NT>(sh);  // (every CTA has read it: the cluster barrier in cluster_total)
+      __syncthreads();
+      auto count = [&](float l, u64 w) { hist_add(sh, min((int)((base - l) * scale), kBins - 1), w); };
+      if (near.usable) {
+        for (int i = lane; i < near.n; i += 32) count(list[i].l, list[i].w);
+      } else {
+        sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int) {
+          unsigned in = 0;
+#pragma unroll
+          for (int i = 0; i < N; ++i) in |= f[i] >= to && f[i] < from && f[i] > s.cutoff ? 1u << i : 0u;
+          marked(f, in, [&](float l, int) { count(l, raw_weight(l, s, sh.table) - kRaw); });
+        });
+      }
+      bin = hist_find<NT>(sh, 3 + 3 * window, limit, before, mass);
+      limit -= before;
+      kept += before;
     }
   }
-  // Members of the border's bin: listed, and the range of their rank keys. The values around the bin are found by two
-  // comparisons (with room for the rounding of the bin's arithmetic), the members among them by their bin.
+  // Members of the border's bin (all that are near, where those are few): listed, and the range of their rank keys. In the row
+  // the values around the bin are found by two comparisons, with room for the rounding of the bin's arithmetic, the members
+  // among them by their bin.
   const float width = 1.f / scale, slack = 1e-6f * (fabsf(base) + (float)(bin + 1) * width);
   const float v_hi = base - (float)bin * width + slack, v_lo = bin == kBins - 1 ? to : base - (float)(bin + 1) * width - slack;
   u64 lo = ~0ull, hi = 0;
-  sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int i0) {
-    unsigned in = 0;
+  auto member = [&](float l, int i) {
+    if (bin >= 0 && min((int)((base - l) * scale), kBins - 1) != bin) return;
+    const u64 key = rank_key<T>(l, i);
+    lo = min(lo, key);
+    hi = max(hi, key);
+    const int at = atomicAdd(&sh.n_list, 1);
+    if (at < kList) sh.list[at] = key;
+  };
+  if (near.usable) {
+    for (int i = lane; i < near.n; i += 32) member(list[i].l, list[i].i);
+  } else {
+    sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int i0) {
+      unsigned in = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) in |= f[i] <= v_hi && f[i] >= v_lo ? 1u << i : 0u;
-    while (in) {
-      const int i = __ffs(in) - 1;
-      in &= in - 1;
-      float l = f[0];
+      for (int i = 0; i < N; ++i) in |= f[i] <= v_hi && f[i] >= v_lo ? 1u << i : 0u;
+      while (in) {
+        const int i = __ffs(in) - 1;
+        in &= in - 1;
+        float l = f[0];
 #pragma unroll
-      for (int j = 1; j < N; ++j) l = i == j ? f[j] : l;
-      if (!(l >= to && l < from && l > s.cutoff) || min((int)((base - l) * scale), kBins - 1) != bin) continue;
-      const u64 key = rank_key<T>(l, i0 + i);
-      lo = min(lo, key);
-      hi = max(hi, key);
-      const int at = atomicAdd(&sh.n_list, 1);
-      if (at < kList) sh.list[at] = key;
-    }
-  });
+        for (int j = 1; j < N; ++j) l = i == j ? f[j] : l;
+        if (l >= to && l < from && l > s.cutoff) member(l, i0 + i);
+      }
+    });
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) { lo = min(lo, shfl_xor64(lo, o)); hi = max(hi, shfl_xor64(hi, o)); }
   if (lane == 0) { sh.warp_a[warp] = lo; sh.warp_b[warp] = hi; }
@@ -800,8 +868,7 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
         if (key >= lo && key <= hi) hist_add(sh, (int)((hi - key) >> shift), raw_weight(l, s, sh.table) - kRaw);
       }
     });
-    u64 same;
-    bin = hist_find<NT>(sh, s0, 0, [&](u64, u64) { return limit; }, same, before, mass);
+    bin = hist_find<NT>(sh, s0, limit, before, mass);
     if (bin < 0) {  // cannot happen: the members' mass exceeds the limit
       k.total = kept + before;
       return k;
@@ -827,8 +894,8 @@ struct Mass {
   const float* minus;   // row of the draft distribution to subtract, or null
   int one_hot;          // or the token whose draft probability is 1, or -1
   bool residual;
-  __device__ __forceinline__ u64 of_kept(float l, int i, const double* table) const {
-    u64 w = raw_weight(l, s, table) - kRaw;
+  __device__ __forceinline__ u64 of_kept(float l, int i, const double* table) const { return of_weight(raw_weight(l, s, table) - kRaw, i); }
+  __device__ __forceinline__ u64 of_weight(u64 w, int i) const {
     if (residual && w) {
       const double q = minus != nullptr ? (double)__ldg(minus + i) : i == one_hot ? 1.0 : 0.0;
       const double r = (double)w * inv_z - q;
@@ -841,8 +908,44 @@ struct Mass {
 // First index whose running sum of mass exceeds u * (whole sum); false when there is no mass. `ready`: sh.seg holds the masses
 // of the subsegments already, `mine` the warp's.
 template <typename T, int NT, bool kShared>
-__device__ bool draw(const Slice<T, NT, kShared>& sl, const Mass& mass, float u, bool ready, u64 mine, int slot, int32_t* out, Shared& sh) {
+__device__ bool draw(const Slice<T, NT, kShared>& sl, const Mass& mass, const Near& near, float u, bool ready, u64 mine, int slot, int32_t* out,
+                     Shared& sh) {
   constexpr int N = Vec16<T>::N;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto target_of = [&](u64 all) {
+    const double x = u > 0.f ? (double)u * (double)all : 0.0;  // NaN: 0
+    return x < (double)all ? min((u64)x, all - 1) : all - 1;
+  };
+  if (near.usable) {  // every kept token is in the lists
+    auto of = [&](const Entry& e) { return mass.kept.holds(e.l, e.i) ? mass.of_weight(e.w, e.i) : 0; };
+    const Entry* list = near.mine();
+    mine = 0;
+    for (int i = lane; i < near.n; i += 32) mine += of(list[i]);
+    u64 before;
+    const u64 all = cluster_total<NT>(warp_sum(mine), 0, 0, sh, slot, before).a;
+    if (all == 0 || warp != 0) return all != 0;
+    u64 target = target_of(all);
+    const u64 own = lane < NT / 32 ? sh.warp_a[lane] : 0;
+    u64 inc = warp_scan(own, lane);
+    const u64 cta = __shfl_sync(0xffffffffu, inc, 31);
+    if (target < before || target - before >= cta) return true;  // another CTA's
+    target -= before;
+    const int w = __ffs(__ballot_sync(0xffffffffu, inc > target)) - 1;
+    target -= __shfl_sync(0xffffffffu, inc - own, w);
+    list = near.all + w * near.cap;
+    const int n = sh.near_n[w];
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const u64 m = i0 + lane < n ? of(list[i0 + lane]) : 0;
+      inc = warp_scan(m, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, inc > target);
+      if (hit) {
+        if (lane == 0) *out = list[i0 + __ffs(hit) - 1].i;
+        break;
+      }
+      target -= __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return true;
+  }
   if (!ready) {
     mine = sl.sum(sh, [&](const float (&f)[N], int at) {
       unsigned in = 0;
@@ -853,12 +956,13 @@ __device__ bool draw(const Slice<T, NT, kShared>& sl, const Mass& mass, float u,
       return x;
     });
   }
-  return locate(sl, sh, slot, mine, [&](float l, int i) { return mass.kept.holds(l, i) ? mass.of_kept(l, i, sh.table) : 0; },
-                [&](u64 all) {
-                  const double x = u > 0.f ? (double)u * (double)all : 0.0;  // NaN: 0
-                  return x < (double)all ? min((u64)x, all - 1) : all - 1;
-                },
-                out) != 0;
+  return locate(sl, sh, slot, mine, [&](float l, int i) { return mass.kept.holds(l, i) ? mass.of_kept(l, i, sh.table) : 0; }, target_of, out) != 0;
+}
+
+// The lists lie at the start of the dynamic shared memory, the slice behind them.
+template <int NT>
+__device__ __forceinline__ uint4* slice_of(unsigned char* dyn, const SampleParams& p) {
+  return reinterpret_cast<uint4*>(dyn + (size_t)p.cap * (NT / 32) * sizeof(Entry));
 }
 
 template <typename T, int NT, bool kShared>
@@ -870,7 +974,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const float t = __ldg(p.temperature + r), top_p = __ldg(p.top_p + r), u = __ldg(p.uniform + r);
   float best;
-  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best, sh);
+  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, slice_of<NT>(dyn, p), best, sh);
   const float top = row_top(sl, best, sh);
   const int begin = min((int)cluster_rank() * p.slice, p.vocab), end = min(begin + p.slice, p.vocab);
   float* probs = p.probs == nullptr ? nullptr : p.probs + (int64_t)r * p.probs_stride;
@@ -883,10 +987,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     Mass mass;
     mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
     u64 mine;
-    mass.kept = find_kept(sl, mass.s, top_p, sh, mine);
+    Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
+    mass.kept = find_kept(sl, mass.s, top_p, near, sh, mine);
     mass.residual = false;
     mass.inv_z = 0.0; mass.minus = nullptr; mass.one_hot = -1;
-    draw(sl, mass, u, !(top_p < 1.f), mine, 32, p.tokens + r, sh);
+    draw(sl, mass, near, u, !(top_p < 1.f), mine, 32, p.tokens + r, sh);
     if (probs != nullptr) {
       const float inv = (float)(top_weight(mass.s) / (double)mass.kept.total);
       for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
@@ -941,7 +1046,7 @@ __device__ int quick_test(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
   fall = warp_sum(fall + (u64)(all * (float)kFix));
   fabove = warp_sum(fabove + (u64)(above * (float)kFix));
   u64 before;
-  const Slot sum = cluster_total<NT>(fall, fabove, sh, 31, before);
+  const Slot sum = cluster_total<NT>(fall, fabove, 0, sh, 31, before);
   const double total = (double)sum.a / kFix, ahead = (double)sum.b / kFix;
   double least = total;  // of Z
   if (cut) {
@@ -972,7 +1077,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Sample
   const double uq = (double)__ldg(p.uniform + r) * q;
   float best;
   int ok = 0;
-  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best, sh);
+  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, slice_of<NT>(dyn, p), best, sh);
   const float top = row_top(sl, best, sh), l = rewritten(lx, sl.how);
   if (l > -INFINITY) {  // a token (and so the row has a top)
     if (!(t > 0.f)) {
@@ -983,7 +1088,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Sample
       ok = quick_test(sl, s, top_p, x, l, wx, uq, sh);
       if (ok < 0) {
         u64 mine;
-        const Kept k = find_kept(sl, s, top_p, sh, mine);
+        Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
+        const Kept k = find_kept(sl, s, top_p, near, sh, mine);
         ok = k.holds(l, x) && uq < wx * (top_weight(s) / (double)k.total);
       }
     }
@@ -1015,7 +1121,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const float t = __ldg(p.temperature + req), top_p = __ldg(p.top_p + req), u = __ldg(p.uniform + end - 1);
   float best;
-  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, reinterpret_cast<uint4*>(dyn), best, sh);
+  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, slice_of<NT>(dyn, p), best, sh);
   const float top = row_top(sl, best, sh);
   if (lead) p.accepted[req] = r - begin;
   if (!(t > 0.f) || top == -INFINITY) {
@@ -1025,14 +1131,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
     Mass mass;
     mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
     u64 mine;
-    mass.kept = find_kept(sl, mass.s, top_p, sh, mine);
+    Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
+    mass.kept = find_kept(sl, mass.s, top_p, near, sh, mine);
     mass.inv_z = 1.0 / (double)mass.kept.total;
     mass.residual = rejected;
     mass.minus = rejected && p.draft_probs != nullptr ? p.draft_probs + (int64_t)r * p.draft_stride : nullptr;
     mass.one_hot = rejected ? __ldg(p.draft + r + 1) : -1;
-    if (!draw(sl, mass, u, !rejected && !(top_p < 1.f), mine, 33, p.tokens + req, sh)) {
+    if (!draw(sl, mass, near, u, !rejected && !(top_p < 1.f), mine, 33, p.tokens + req, sh)) {
       mass.residual = false;  // nothing left above the draft's distribution: the target's own
-      draw(sl, mass, u, false, 0, 34, p.tokens + req, sh);
+      draw(sl, mass, near, u, false, 0, 34, p.tokens + req, sh);
     }
   }
   cluster_sync();
@@ -1040,7 +1147,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
 
 // ---- host --------------------------------------------------------------------------------------------
 struct Shape {
-  int ctas, slice;
+  int ctas, slice, cap;
   bool shared;  // rows in shared memory, 512 threads; else in L2, 256 threads
   size_t smem;
 };
@@ -1052,9 +1159,9 @@ Shape pick_shape(int rows, int vocab, int es) {
   s.ctas = 1;
   while (s.ctas < kMaxCtas && (int64_t)rows * s.ctas * 2 <= 296 && vocab / (s.ctas * 2) >= 2048) s.ctas *= 2;
   s.slice = ((vocab + s.ctas - 1) / s.ctas + 63) & ~63;
-  s.smem = (size_t)s.slice * es + 32;
-  s.shared = (int64_t)rows * s.ctas <= 296 && s.smem <= 80 * 1024;
-  if (!s.shared) s.smem = 0;
+  s.shared = (int64_t)rows * s.ctas <= 296 && (int64_t)s.slice * es <= 72 * 1024;
+  s.cap = s.shared ? 64 : 176;
+  s.smem = (s.shared ? (size_t)s.slice * es + 32 : 0) + (size_t)s.cap * (s.shared ? 16 : 8) * sizeof(Entry);
   return s;
 }
 
@@ -1096,7 +1203,7 @@ int dsv_sample_top_p(const void* logits, int64_t row_stride, int rows, int vocab
   p.logits = logits; p.row_stride = row_stride; p.vocab = vocab; p.temperature = temperature; p.top_p = top_p;
   p.uniform = uniform; p.tokens = tokens; p.probs = probs; p.probs_stride = probs_stride;
   const Shape shape = pick_shape(rows, vocab, elem_size(dtype));
-  p.slice = shape.slice;
+  p.slice = shape.slice; p.cap = shape.cap;
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
@@ -1133,13 +1240,13 @@ int dsv_verify_draft(const void* logits, int64_t row_stride, int nnz, int vocab,
     using T = decltype(tag);
     if (nnz > 0) {
       const Shape shape = pick_shape(nnz, vocab, elem_size(dtype));
-      p.slice = shape.slice;
+      p.slice = shape.slice; p.cap = shape.cap;
       const cudaError_t er = shape.shared ? launch<512>(verify_rows_kernel<T, 512, true>, nnz, shape, p, st)
                                         : launch<256>(verify_rows_kernel<T, 256, false>, nnz, shape, p, st);
       if (er != cudaSuccess) return er;
     }
     const Shape shape = pick_shape(batch, vocab, elem_size(dtype));
-    p.slice = shape.slice;
+    p.slice = shape.slice; p.cap = shape.cap;
     return shape.shared ? launch<512>(verify_draw_kernel<T, 512, true>, batch, shape, p, st)
                       : launch<256>(verify_draw_kernel<T, 256, false>, batch, shape, p, st);
   };

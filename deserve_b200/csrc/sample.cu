@@ -89,7 +89,7 @@ struct Slot {
 };
 struct Shared {
   uint32_t hist_lo[kBins], hist_hi[kBins];
-  double table[kTable];  // 2^(j / 64 + 44)
+  double table[kTable];  // 2^(j / 64)
   Slot slot[36];
   u64 warp_a[kMaxWarps], warp_b[kMaxWarps], warp_c[kMaxWarps];
   u64 seg[kMaxWarps * kSub];  // mass of the subsegments
@@ -244,7 +244,7 @@ __device__ __forceinline__ u64 raw_weight(float l, const RowScale& s, const doub
   e = fma(r, e, 1.0);
   const int n = __double2loint(m);
   const double t = table[n & (kTable - 1)];
-  const double scaled = __hiloint2double(__double2hiint(t) + ((n >> 6) << 20), __double2loint(t));
+  const double scaled = __hiloint2double(__double2hiint(t) + ((n >> 6) << 20) + (44 << 20), __double2loint(t));
   return (u64)__double_as_longlong(fma(scaled, e, 4503599627370496.0));  // + 2^52: rounded to an integer
 }
 __device__ __forceinline__ double weight(float l, const RowScale& s) {  // in units of the largest, for single entries
@@ -269,7 +269,8 @@ __device__ __forceinline__ float rewritten(float l, int how) {
 template <typename T, int NT, bool kShared>
 struct Slice {
   static constexpr int N = Vec16<T>::N;
-  uint4* v;
+  const uint4* g;  // in global memory
+  const uint4* v;  // where walks after the first read it
   int n_vec, first;
   int seg, sub;    // vectors of a warp's contiguous segment, of a subsegment
   int lead, tail;  // entries of the first and of the last vector that lie outside
@@ -359,6 +360,14 @@ struct Slice {
   }
 };
 
+template <int N>
+__device__ __forceinline__ float largest(const float (&f)[N]) {  // NaN ignored
+  float m = fmaxf(f[0], f[1]);
+#pragma unroll
+  for (int i = 2; i < N; ++i) m = fmaxf(m, f[i]);
+  return m;
+}
+
 // of(value, place) for the entries of a vector that `in` marks: one by one where they are few, side by side where many.
 template <int N, typename F>
 __device__ __forceinline__ void marked(const float (&f)[N], unsigned in, F of) {
@@ -378,88 +387,316 @@ __device__ __forceinline__ void marked(const float (&f)[N], unsigned in, F of) {
   }
 }
 
-// First pass: the slice's largest entry that is a number (NaN ignored), and its copy in shared memory.
+// Geometry of the slice; `first_walk` brings it in.
 template <typename T, int NT, bool kShared>
-__device__ __forceinline__ Slice<T, NT, kShared> load_slice(const T* row, int vocab, int slice, uint4* buf, float& best, Shared& sh) {
+__device__ __forceinline__ Slice<T, NT, kShared> make_slice(const T* row, int vocab, int slice, uint4* buf, Shared& sh) {
   constexpr int N = Vec16<T>::N, W = NT / 32;
-  if (threadIdx.x < kTable) sh.table[threadIdx.x] = kPowers[threadIdx.x] * kOne;
+  if (threadIdx.x < kTable) sh.table[threadIdx.x] = kPowers[threadIdx.x];
   if (threadIdx.x == 0) sh.n_list = 0;
   const int begin = min((int)cluster_rank() * slice, vocab), n = min(begin + slice, vocab) - begin;
   const T* src = row + begin;
   Slice<T, NT, kShared> sl;
   sl.lead = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
-  uint4* g = reinterpret_cast<uint4*>(const_cast<T*>(src - sl.lead));
-  sl.v = kShared ? buf : g;
+  sl.g = reinterpret_cast<const uint4*>(src - sl.lead);
+  sl.v = kShared ? buf : sl.g;
   sl.first = begin - sl.lead;
   sl.n_vec = n > 0 ? (sl.lead + n + N - 1) / N : 0;
   sl.tail = sl.n_vec * N - sl.lead - n;
   sl.seg = ((sl.n_vec + W * 32 - 1) / (W * 32)) * 32;
   sl.sub = ((sl.seg + kSub * 32 - 1) / (kSub * 32)) * 32;
   sl.how = kAsIs;
-  best = -INFINITY;
-  auto take = [&](int v, const uint4& u) {
-    if (kShared) buf[v] = u;
-    float f[N];
-    Vec16<T>::unpack(u, f);
-    sl.mask(v, f);
-#pragma unroll
-    for (int i = 0; i < N; ++i) best = fmaxf(best, f[i]);
-  };
-  int v = threadIdx.x;
-  for (; v + 7 * NT < sl.n_vec; v += 8 * NT) {
-    uint4 u[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) u[k] = ld_stream16(g + v + k * NT);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) take(v + k * NT, u[k]);
-  }
-  for (; v < sl.n_vec; v += NT) take(v, ld_stream16(g + v));
   return sl;
 }
 
-// The cluster's largest logit, -inf when it holds nothing but NaN and -inf.
-template <typename T, int NT, bool kShared>
-__device__ float row_top(Slice<T, NT, kShared>& sl, float best, Shared& sh) {
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The one walk over HBM: of(values, first index, first vector of the warp's turn) for the warp's segment, its 32 lanes together,
+// -inf behind the end; four vectors a lane on their way. A shared slice gets its copy.
+template <typename T, int NT, bool kShared, typename F>
+__device__ __forceinline__ void first_walk(const Slice<T, NT, kShared>& sl, uint4* buf, F of) {
+  constexpr int N = Vec16<T>::N, DEPTH = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, a = sl.begin(warp), b = sl.end(warp);
+  uint4 u[DEPTH];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (lane == 0) sh.warp_a[warp] = __float_as_uint(best);
-  __syncthreads();
-  if (warp == 0) {
-    best = __uint_as_float((uint32_t)sh.warp_a[min(lane, NT / 32u - 1)]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) sh.slot[0].a = __float_as_uint(best);
+  for (int k = 0; k < DEPTH; ++k) {
+    u[k] = make_uint4(0, 0, 0, 0);
+    if (a + 32 * k + lane < b) u[k] = ld_stream16(sl.g + a + 32 * k + lane);
   }
-  cluster_sync();
-  const uint32_t c = cluster_size();
-  float top = lane < c ? __uint_as_float((uint32_t)ld_remote64(remote(&sh.slot[0].a, lane))) : -INFINITY;
+  for (int i0 = a; i0 < b; i0 += 32 * DEPTH) {
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  top = __shfl_sync(0xffffffffu, top, 0);
+    for (int k = 0; k < DEPTH; ++k) {
+      const int at = i0 + 32 * k, i = at + lane;
+      if (at >= b) break;
+      const uint4 now = u[k];
+      if (i + 32 * DEPTH < b) u[k] = ld_stream16(sl.g + i + 32 * DEPTH);
+      if (kShared && i < b) buf[i] = now;
+      float f[N];
+      Vec16<T>::unpack(now, f);
+      sl.mask(i, f);
+      if (i >= b) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = -INFINITY;
+      }
+      of(f, sl.first + i * N, at);
+    }
+  }
+}
+
+// How a row at the end of the number range is rewritten from here on, and its rewritten top.
+template <typename T, int NT, bool kShared>
+__device__ __forceinline__ float settle(Slice<T, NT, kShared>& sl, float top) {
   sl.how = top == INFINITY ? kInfinite : top < -1e38f && top > -INFINITY ? kQuartered : kAsIs;
   return rewritten(top, sl.how);
 }
-// Lowest index of the largest logit (of a row that has one), through slot 1.
+
+// Greedy walk: the row's largest entry that is a number and its lowest index (-1: there is none). Slot 0.
 template <typename T, int NT, bool kShared>
-__device__ int row_first(const Slice<T, NT, kShared>& sl, float top, Shared& sh) {
+__device__ int greedy_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float& top, Shared& sh) {
   constexpr int N = Vec16<T>::N;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float best = -INFINITY;
   int at = 0x7fffffff;
-  sl.each(threadIdx.x, sl.n_vec, NT, [&](const float (&f)[N], int i0) {
+  first_walk(sl, buf, [&](const float (&f)[N], int i0, int) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (f[i] == top) at = min(at, i0 + i);
+      if (f[i] > best) { best = f[i]; at = i0 + i; }  // ascending: the first of equal ones stays
   });
-  at = __reduce_min_sync(0xffffffffu, at);
-  if ((threadIdx.x & 31) == 0) sh.warp_a[threadIdx.x >> 5] = (u64)at;
+  // (value, lowest index) as one integer; 0: nothing
+  u64 k = at == 0x7fffffff ? 0 : ((u64)order_key<float>(best) << 32) | (u64)(0xffffffffu - (uint32_t)at);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) k = max(k, shfl_xor64(k, o));
+  if (lane == 0) sh.warp_a[warp] = k;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    u64 m = sh.warp_a[0];
-    for (int w = 1; w < NT / 32; ++w) m = min(m, sh.warp_a[w]);
-    sh.slot[1].a = m;
+  if (warp == 0) {
+    k = lane < NT / 32 ? sh.warp_a[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) k = max(k, shfl_xor64(k, o));
+    if (lane == 0) sh.slot[0].a = k;
   }
   cluster_sync();
-  return (int)cluster_min(&sh.slot[1].a);
+  k = cluster_max(&sh.slot[0].a);
+  top = k ? key_value<float>((uint32_t)(k >> 32)) : -INFINITY;
+  return k ? (int)(0xffffffffu - (uint32_t)k) : -1;
+}
+
+__device__ __forceinline__ double as_double(u64 v) { return __longlong_as_double((long long)v); }
+__device__ __forceinline__ u64 as_bits(double v) { return (u64)__double_as_longlong(v); }
+__device__ __forceinline__ double power(double n) { return exp2(fmax(n, -2000.0)); }  // of an integer; 0 far below
+
+// Sum of the row's weights in double, and its top, from the first walk. Every warp measures against a power of two of its
+// own, 2^E near its first entries' maximum (a double's range leaves 600 factors of two to both sides), so nothing has to be known
+// before; the powers are joined exactly. `far`: an entry outgrew that range, or l c leaves the integers of a double: the sum
+// does not hold.
+struct Walk {
+  float top;
+  bool far;
+  double e;              // the row's power
+  double total;          // weights of the row in units of 2^e
+  double inc;            // lane r: those of the CTAs up to r
+};
+constexpr double kReach = 600.0;
+
+// Joins (mass, power) over the lanes below n: the larger power, the running sums in it.
+__device__ __forceinline__ void join(double& mass, double& e, double& inc, int lane) {
+  double g = e;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) g = fmax(g, __shfl_xor_sync(0xffffffffu, g, o));
+  mass = g > -INFINITY && e > -INFINITY ? mass * power(e - g) : 0.0;
+  e = g;
+  inc = mass;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+}
+
+// (Slot 0. sh.warp_a / b keep every warp's mass and power, sh.seg the subsegments' masses as doubles in the warp's power.)
+template <typename T, int NT, bool kShared>
+__device__ Walk weight_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float temperature, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float t = fminf(fmaxf(temperature, 1e-30f), 1e36f);
+  const double c = 92.332482616893657 / (double)t;
+  __syncthreads();  // the table
+  float top = -INFINITY, cutoff = 0.f;
+  double e = -INFINITY, magic = 0.0, mass = 0.0, part = 0.0;
+  bool far = false;
+  int sub = 0, next = sl.begin(warp) + sl.sub;
+  auto close = [&]() {  // end of a subsegment
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    if (lane == 0) sh.seg[warp * kSub + sub] = as_bits(part);
+    mass += part;
+    part = 0.0;
+    ++sub;
+  };
+  first_walk(sl, buf, [&](const float (&f)[N], int, int at) {
+    if (at >= next) {
+      close();
+      next += sl.sub;
+    }
+    float m = largest(f);
+    top = fmaxf(top, m);
+    if (e == -INFINITY) {  // warp-uniform: until there is an entry to measure against
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const double x = (double)m * c * 0.015625;
+      if (m > -INFINITY) {
+        e = fabs(x) < 1e6 ? rint(x) : 0.0;
+        far |= !(fabs(x) < 1e6);
+        cutoff = m - fminf(0.69f * (float)kReach * t, 1e37f);
+        far |= !(cutoff > -3e38f && cutoff < m);
+        magic = 6755399441055744.0 - 64.0 * e;
+      }
+    }
+    if (e > -INFINITY && !far) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {  // as in raw_weight, summed as a double
+        const double x = (double)fmaxf(f[i], cutoff);
+        const double w = fma(x, c, magic), r = fma(x, c, magic - w);
+        constexpr double a = 0.010830424696249145;
+        double y = fma(r, a * a * a * a / 24.0, a * a * a / 6.0);
+        y = fma(r, y, a * a / 2.0);
+        y = fma(r, y, a);
+        y = fma(r, y, 1.0);
+        const int n = __double2loint(w);
+        const double p = sh.table[n & (kTable - 1)];
+        part = fma(__hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p)), y, part);
+      }
+    }
+  });
+  while (sub < kSub) close();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // An entry more than kReach above the warp's first ones makes the sum meaningless (it may have wrapped an exponent).
+  far |= top > -INFINITY && !(((double)top * c * 0.015625 - e) < kReach);
+  far = __any_sync(0xffffffffu, far);
+  if (lane == 0) {
+    sh.warp_a[warp] = as_bits(far ? 0.0 : mass);
+    sh.warp_b[warp] = as_bits(e);
+    sh.warp_c[warp] = (u64)__float_as_uint(top) | (far ? 1ull << 32 : 0);
+  }
+  __syncthreads();
+  double inc;
+  if (warp == 0) {
+    const bool in = lane < NT / 32;
+    mass = in ? as_double(sh.warp_a[lane]) : 0.0;
+    e = in ? as_double(sh.warp_b[lane]) : -INFINITY;
+    top = in ? __uint_as_float((uint32_t)sh.warp_c[lane]) : -INFINITY;
+    far = __any_sync(0xffffffffu, in && (sh.warp_c[lane] >> 32) != 0);
+    join(mass, e, inc, lane);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const double all = __shfl_sync(0xffffffffu, inc, 31);
+    if (lane == 0) {
+      sh.slot[0].a = as_bits(all);
+      sh.slot[0].b = as_bits(e);
+      sh.slot[0].c = (u64)__float_as_uint(top) | (far ? 1ull << 32 : 0);
+    }
+  }
+  cluster_sync();
+  Walk w;
+  const uint32_t n = cluster_size();
+  const bool in = (uint32_t)lane < n;
+  mass = in ? as_double(ld_remote64(remote(&sh.slot[0].a, lane))) : 0.0;
+  e = in ? as_double(ld_remote64(remote(&sh.slot[0].b, lane))) : -INFINITY;
+  const u64 x = in ? ld_remote64(remote(&sh.slot[0].c, lane)) : (u64)__float_as_uint(-INFINITY);
+  join(mass, e, inc, lane);
+  w.top = __uint_as_float((uint32_t)x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) w.top = fmaxf(w.top, __shfl_xor_sync(0xffffffffu, w.top, o));
+  w.far = __any_sync(0xffffffffu, (x >> 32) != 0) || w.top == INFINITY || w.top < -1e38f;
+  w.e = e;
+  w.total = __shfl_sync(0xffffffffu, inc, 31);
+  w.inc = inc;
+  return w;
+}
+
+// First lane whose running sum exceeds the target; where rounding leaves none, the first that reaches the whole.
+__device__ __forceinline__ int pick(double inc, double target, double& rest) {
+  const double all = __shfl_sync(0xffffffffu, inc, 31);
+  const unsigned hit = __ballot_sync(0xffffffffu, inc > target);
+  const int who = __ffs(hit ? hit : __ballot_sync(0xffffffffu, inc == all)) - 1;
+  const double before = __shfl_sync(0xffffffffu, inc, max(who - 1, 0));
+  rest = fmax(who > 0 ? target - before : target, 0.0);
+  return who;
+}
+
+// The draw of a row without a cut from the sums that weight_walk left: only the subsegment that holds the target is read again.
+// (Every CTA joins the same numbers in the same order, so exactly one of them finds the target its own.)
+template <typename T, int NT, bool kShared>
+__device__ void draw_all(const Slice<T, NT, kShared>& sl, const Walk& walk, float temperature, float u, int32_t* out, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x >= 32) return;
+  const float t = fminf(fmaxf(temperature, 1e-30f), 1e36f);
+  const double c = 92.332482616893657 / (double)t;
+  double rest, inc;
+  const int owner = pick(walk.inc, fmin((double)u, 1.0) * walk.total, rest);
+  if (owner != (int)cluster_rank()) return;
+  const bool in = lane < NT / 32;
+  const double own_e = in ? as_double(sh.warp_b[lane]) : -INFINITY;
+  double mass = in ? as_double(sh.warp_a[lane]) : 0.0, e = own_e;
+  join(mass, e, inc, lane);
+  const int w = pick(inc, rest * power(walk.e - e), rest);
+  const double e_w = __shfl_sync(0xffffffffu, own_e, w);
+  rest *= power(e - e_w);
+  inc = lane < kSub ? as_double(sh.seg[w * kSub + lane]) : 0.0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
+  }
+  const int k = pick(inc, rest, rest);
+  const float lowest = walk.top - 31.2f * t;  // weights below 2^-45 of the largest cannot be drawn
+  const double magic = 6755399441055744.0 - 64.0 * e_w;
+  const int a = min(sl.begin(w) + k * sl.sub, sl.end(w)), b = min(a + sl.sub, sl.end(w));
+  int last = -1;
+  for (int v0 = a; v0 < b; v0 += 32) {
+    const int v = v0 + lane;
+    double m[N], total = 0.0;
+    float f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = -INFINITY;
+    if (v < b) sl.get(v, f);
+    int mine = -1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      m[i] = 0.0;
+      if (f[i] >= lowest) {
+        const double x = (double)f[i], y = fma(x, c, magic), r = fma(x, c, magic - y);
+        const int n = __double2loint(y);
+        m[i] = sh.table[n & (kTable - 1)] * exp2(r * 0.015625) * power((double)(n >> 6));
+        mine = sl.first + v * N + i;
+      }
+      total += m[i];
+    }
+    inc = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, inc > rest);
+    if (hit) {
+      const int who = __ffs(hit) - 1;
+      const double before = __shfl_up_sync(0xffffffffu, inc, 1);
+      if (lane == who) {
+        double run = lane > 0 ? before : 0.0;
+        int i = -1;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (m[j] > 0.0 && (i < 0 || run <= rest)) i = j;
+          run += m[j];
+        }
+        *out = sl.first + v * N + i;
+      }
+      return;
+    }
+    mine = __reduce_max_sync(0xffffffffu, mine);
+    last = max(last, mine);
+    rest = fmax(rest - __shfl_sync(0xffffffffu, inc, 31), 0.0);
+  }
+  if (lane == 0) *out = max(last, 0);  // (a last unit of rounding left nothing: its last entry)
 }
 
 // Sums over the cluster of up to three integers per warp (in its lane 0), through slot `s`: the wholes, and what the CTAs
@@ -655,9 +892,10 @@ __device__ u64 locate(const Slice<T, NT, kShared>& sl, Shared& sh, int slot, u64
   return all;
 }
 
-// Top-p border of the row. Without a cut the masses of the subsegments are left in sh.seg (`mine`: the warp's). Slots 2 to 30.
+// Top-p border of the row. `known`: the sum of its weights in units of the fixed-point weights, or -1. Without a cut and
+// with an unknown sum the masses of the subsegments are left in sh.seg (`mine`: the warp's). Slots 2 to 30.
 template <typename T, int NT, bool kShared>
-__device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, float top_p, Near& near, Shared& sh, u64& mine) {
+__device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, float top_p, double known, Near& near, Shared& sh, u64& mine) {
   constexpr int N = Vec16<T>::N;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Kept k;
@@ -668,6 +906,10 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
   mine = 0;
   near.n = 0;
   near.usable = false;
+  if (!(top_p < 1.f) && known >= 0.0) {
+    k.total = (u64)known;
+    return k;
+  }
   if (!(top_p < 1.f)) {  // NaN: no cut
     mine = sl.sum(sh, [&](const float (&f)[N], int) {
       u64 x = 0;
@@ -678,20 +920,21 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
     k.total = cluster_total<NT>(mine, 0, 0, sh, 2, before).a;
     return k;
   }
-  // One walk gives the sums of the tokens near the top and of the others, and the list of the former.
+  // One walk gives the sum and the list of the tokens near the top (and the sum of all, where that is not known).
   float from = INFINITY, base = s.top, to = s.top - kWindow * s.t, scale = (float)kBins / (kWindow * s.t);
-  u64 tail = 0, sum = 0;
+  u64 whole_mass = 0, sum = 0;
   Entry* list = near.mine();
   sl.each_warp(w0, w1, [&](const float (&f)[N], int i0) {
-    unsigned in = 0;
+    if (known < 0.0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      tail += raw_weight(f[i], s, sh.table);
-      in |= f[i] >= to ? 1u << i : 0u;
+      for (int i = 0; i < N; ++i) whole_mass += raw_weight(f[i], s, sh.table);
+      whole_mass -= N * kRaw;
     }
-    tail -= N * kRaw;
-    const int n = __popc(in);
-    if (__any_sync(0xffffffffu, n)) {
+    if (__any_sync(0xffffffffu, largest(f) >= to)) {
+      unsigned in = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) in |= f[i] >= to ? 1u << i : 0u;
+      const int n = __popc(in);
       int at = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -715,7 +958,8 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
     }
   });
   if (lane == 0) sh.near_n[warp] = near.n;
-  const Slot whole = cluster_total<NT>(warp_sum(sum), warp_sum(tail), (u64)near.n + (near.n > near.cap ? 1ull << 40 : 0), sh, 2, before);
+  Slot whole = cluster_total<NT>(warp_sum(sum), warp_sum(whole_mass), (u64)near.n + (near.n > near.cap ? 1ull << 40 : 0), sh, 2, before);
+  if (known >= 0.0) whole.b = (u64)known;
   k.total = whole.b;
   u64 limit = (u64)((double)fmaxf(top_p, 0.f) * (double)whole.b), mass, kept = 0;
   near.usable = limit < whole.a && whole.c < 1ull << 40;
@@ -746,6 +990,7 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
       } else {
         sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int) {
           unsigned in = 0;
+          if (largest(f) < to) return;
 #pragma unroll
           for (int i = 0; i < N; ++i) in |= f[i] >= to && f[i] < from && f[i] > s.cutoff ? 1u << i : 0u;
           marked(f, in, [&](float l, int) { count(l, raw_weight(l, s, sh.table) - kRaw); });
@@ -774,6 +1019,7 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
     for (int i = lane; i < near.n; i += 32) member(list[i].l, list[i].i);
   } else {
     sl.each(w0 + lane, w1, 32, [&](const float (&f)[N], int i0) {
+      if (largest(f) < v_lo) return;
       unsigned in = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) in |= f[i] <= v_hi && f[i] >= v_lo ? 1u << i : 0u;
@@ -948,6 +1194,7 @@ __device__ bool draw(const Slice<T, NT, kShared>& sl, const Mass& mass, const Ne
   }
   if (!ready) {
     mine = sl.sum(sh, [&](const float (&f)[N], int at) {
+      if (largest(f) < mass.kept.value) return (u64)0;
       unsigned in = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) in |= f[i] >= mass.kept.value && mass.kept.holds(f[i], at + i) ? 1u << i : 0u;
@@ -965,6 +1212,12 @@ __device__ __forceinline__ uint4* slice_of(unsigned char* dyn, const SampleParam
   return reinterpret_cast<uint4*>(dyn + (size_t)p.cap * (NT / 32) * sizeof(Entry));
 }
 
+// The sum of weight_walk in units of the fixed-point weights, -1 where it does not hold.
+__device__ __forceinline__ double in_fixed_units(const Walk& w, const RowScale& s) {
+  return w.far ? -1.0 : w.total * exp2(44.0 + (w.e - (6755399441055744.0 - s.magic) * 0.015625));
+}
+constexpr float kLeastU = 1e-7f;  // random numbers below go the exact way: what cannot be drawn must not be met there
+
 template <typename T, int NT, bool kShared>
 __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -973,27 +1226,40 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   const int r = blockIdx.x / cluster_size();
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const float t = __ldg(p.temperature + r), top_p = __ldg(p.top_p + r), u = __ldg(p.uniform + r);
-  float best;
-  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, slice_of<NT>(dyn, p), best, sh);
-  const float top = row_top(sl, best, sh);
+  uint4* buf = slice_of<NT>(dyn, p);
+  Slice<T, NT, kShared> sl = make_slice<T, NT, kShared>(row, p.vocab, p.slice, buf, sh);
   const int begin = min((int)cluster_rank() * p.slice, p.vocab), end = min(begin + p.slice, p.vocab);
   float* probs = p.probs == nullptr ? nullptr : p.probs + (int64_t)r * p.probs_stride;
-  if (!(t > 0.f) || top == -INFINITY) {  // greedy, or a row without a token
-    const int first = top == -INFINITY ? -1 : row_first(sl, top, sh);
+  const bool greedy = !(t > 0.f);
+  Walk walk;
+  int first = -1;
+  if (greedy) first = greedy_walk(sl, buf, walk.top, sh);
+  else walk = weight_walk(sl, buf, t, sh);
+  if (greedy || walk.top == -INFINITY) {  // or a row without a token
     if (cluster_rank() == 0 && threadIdx.x == 0) p.tokens[r] = max(first, 0);
     if (probs != nullptr)
       for (int i = begin + threadIdx.x; i < end; i += NT) probs[i] = i == first ? 1.f : 0.f;
   } else {
+    const float top = settle(sl, walk.top);
     Mass mass;
     mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
-    u64 mine;
-    Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
-    mass.kept = find_kept(sl, mass.s, top_p, near, sh, mine);
-    mass.residual = false;
-    mass.inv_z = 0.0; mass.minus = nullptr; mass.one_hot = -1;
-    draw(sl, mass, near, u, !(top_p < 1.f), mine, 32, p.tokens + r, sh);
+    mass.kept.value = -INFINITY;
+    mass.kept.index = -1;
+    double z;  // the kept weights' sum, in units of the top's
+    if (!(top_p < 1.f) && !walk.far && u >= kLeastU) {
+      draw_all(sl, walk, t, u, p.tokens + r, sh);
+      z = in_fixed_units(walk, mass.s);
+    } else {
+      u64 mine;
+      Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
+      mass.kept = find_kept(sl, mass.s, top_p, top_p < 1.f ? in_fixed_units(walk, mass.s) : -1.0, near, sh, mine);
+      mass.residual = false;
+      mass.inv_z = 0.0; mass.minus = nullptr; mass.one_hot = -1;
+      draw(sl, mass, near, u, !(top_p < 1.f), mine, 32, p.tokens + r, sh);
+      z = (double)mass.kept.total;
+    }
     if (probs != nullptr) {
-      const float inv = (float)(top_weight(mass.s) / (double)mass.kept.total);
+      const float inv = (float)(top_weight(mass.s) / z);
       for (int v = threadIdx.x; v < sl.n_vec; v += NT) {
         float f[N];
         sl.get(v, f);
@@ -1017,42 +1283,108 @@ __device__ __forceinline__ int owner_of(const int32_t* __restrict__ indptr, int 
   return lo;
 }
 
-// Does the draft x of a row pass, u q(x) < p(x)? The answer needs p(x) only to one side of u q(x): sums in fp32 decide
-// unless they come too close (1e-5 bounds their error: 2^-22 of ex2.approx, 2^-23 of the exponent's size, which the
-// weights average to at most log2 of the vocabulary, 128 additions), or the nucleus' exact mass is needed: Z lies
-// between top_p and 1 times the whole sum. 1: yes, 0: no, -1: not known.
+// Does the draft x of a row pass, u q(x) < p(x)? The answer needs p(x) only to one side of u q(x): sums in fp32 from the first
+// walk decide unless they come too close, or the nucleus' exact mass is needed (Z lies between top_p and 1 times the whole sum).
+// Relative error of the sums: 2^-22 of ex2.approx, 2^-22 for each of at most 80 factors of two of the exponent, 2^-24 for each of a
+// subsegment's additions: below 3e-5. 1: yes, 0: no, -1: not known. Also the row's top. Slots 0 and 1.
 template <typename T, int NT, bool kShared>
-__device__ int quick_test(const Slice<T, NT, kShared>& sl, const RowScale& s, float top_p, int x, float lx, double wx, double uq, Shared& sh) {
+__device__ int quick_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float temperature, float top_p, int x, float lx, double uq, float& top,
+                          Shared& sh) {
   constexpr int N = Vec16<T>::N;
-  constexpr double kFix = 1099511627776.0, kGuard = 4e-5;  // 2^40
-  float all = 0.f, above = 0.f;
+  constexpr double kGuard = 6e-5;
+  constexpr float kOctaves = 80.f;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float t = fminf(fmaxf(temperature, 1e-30f), 1e36f), c32 = 1.442695041f / t;
   const bool cut = top_p < 1.f;
-  u64 fall = 0, fabove = 0;
-  int n = 0;
-  sl.each(threadIdx.x, sl.n_vec, NT, [&](const float (&f)[N], int i0) {
+  float m0 = -INFINITY, cutoff = 0.f, best = -INFINITY, all = 0.f, above = 0.f;
+  double sum_all = 0.0, sum_above = 0.0;
+  int turn = 0;
+  first_walk(sl, buf, [&](const float (&f)[N], int i0, int) {
+    float m = largest(f);
+    best = fmaxf(best, m);
+    if (m0 == -INFINITY) {  // warp-uniform
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float w = ex2((fmaxf(f[i], s.cutoff) - s.top) * s.c32);
-      all += w;
-      if (cut) above += f[i] > lx || (f[i] == lx && i0 + i < x) ? w : 0.f;
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      m0 = m;
+      cutoff = m - fminf(0.69f * 120.f * t, 1e37f);
     }
-    if (++n * N >= 128) {
-      fall += (u64)(all * (float)kFix);
-      fabove += (u64)(above * (float)kFix);
+    if (m0 > -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float w = ex2((fmaxf(f[i], cutoff) - m0) * c32);
+        all += w;
+        if (cut) above += f[i] > lx || (f[i] == lx && i0 + i < x) ? w : 0.f;
+      }
+    }
+    if (++turn == 16) {
+      sum_all += (double)all;
+      sum_above += (double)above;
       all = above = 0.f;
-      n = 0;
+      turn = 0;
     }
   });
-  fall = warp_sum(fall + (u64)(all * (float)kFix));
-  fabove = warp_sum(fabove + (u64)(above * (float)kFix));
-  u64 before;
-  const Slot sum = cluster_total<NT>(fall, fabove, 0, sh, 31, before);
-  const double total = (double)sum.a / kFix, ahead = (double)sum.b / kFix;
+  sum_all += (double)all;
+  sum_above += (double)above;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum_all += __shfl_xor_sync(0xffffffffu, sum_all, o);
+    sum_above += __shfl_xor_sync(0xffffffffu, sum_above, o);
+    best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  }
+  const double c = 1.4426950408889634 / (double)t;
+  bool far = best > -INFINITY && !((best - m0) * c32 < kOctaves && cutoff > -3e38f && cutoff < m0);
+  double e = m0 > -INFINITY && !far ? (double)m0 * c : -INFINITY;
+  if (lane == 0) {
+    sh.warp_a[warp] = as_bits(sum_all);
+    sh.warp_b[warp] = as_bits(e);
+    sh.warp_c[warp] = (u64)__float_as_uint(best) | (far ? 1ull << 32 : 0);
+    sh.seg[warp] = as_bits(sum_above);
+  }
+  __syncthreads();
+  double inc, own;
+  if (warp == 0) {
+    const bool in = lane < NT / 32;
+    sum_all = in ? as_double(sh.warp_a[lane]) : 0.0;
+    sum_above = in ? as_double(sh.seg[lane]) : 0.0;
+    own = e = in ? as_double(sh.warp_b[lane]) : -INFINITY;
+    best = in ? __uint_as_float((uint32_t)sh.warp_c[lane]) : -INFINITY;
+    far = __any_sync(0xffffffffu, in && (sh.warp_c[lane] >> 32) != 0);
+    join(sum_all, e, inc, lane);
+    const double whole = __shfl_sync(0xffffffffu, inc, 31);
+    double g = own;
+    join(sum_above, g, inc, lane);
+    const double ahead = __shfl_sync(0xffffffffu, inc, 31);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) {
+      sh.slot[0].a = as_bits(whole);
+      sh.slot[0].b = as_bits(e);
+      sh.slot[0].c = (u64)__float_as_uint(best) | (far ? 1ull << 32 : 0);
+      sh.slot[1].a = as_bits(ahead);
+    }
+  }
+  cluster_sync();
+  const bool in = lane < (int)cluster_size();
+  sum_all = in ? as_double(ld_remote64(remote(&sh.slot[0].a, lane))) : 0.0;
+  own = e = in ? as_double(ld_remote64(remote(&sh.slot[0].b, lane))) : -INFINITY;
+  const u64 z = in ? ld_remote64(remote(&sh.slot[0].c, lane)) : (u64)__float_as_uint(-INFINITY);
+  sum_above = in ? as_double(ld_remote64(remote(&sh.slot[1].a, lane))) : 0.0;
+  join(sum_all, e, inc, lane);
+  const double total = __shfl_sync(0xffffffffu, inc, 31);
+  double g = own;
+  join(sum_above, g, inc, lane);
+  const double ahead = __shfl_sync(0xffffffffu, inc, 31);
+  best = __uint_as_float((uint32_t)z);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  top = best;
+  if (__any_sync(0xffffffffu, (z >> 32) != 0) || top == INFINITY || top < -1e38f) return -1;
+  const double wx = power((double)lx * c - e);
   double least = total;  // of Z
   if (cut) {
     least = total * fmax((double)top_p, 0.0);
     if (ahead * (1 - kGuard) > least * (1 + kGuard)) return 0;      // not in the nucleus
-    if (!(ahead * (1 + kGuard) <= least * (1 - kGuard))) return -1;  // (and its first token when top_p is 0)
+    if (!(ahead * (1 + kGuard) <= least * (1 - kGuard))) return -1;
   }
   if (uq * total * (1 + kGuard) < wx) return 1;
   if (uq * least * (1 - kGuard) >= wx) return 0;
@@ -1075,22 +1407,23 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Sample
   const float lx = token ? to_f32(row[x]) : -INFINITY;
   const double q = p.draft_probs == nullptr || !token ? 1.0 : (double)__ldg(p.draft_probs + (int64_t)r * p.draft_stride + x);
   const double uq = (double)__ldg(p.uniform + r) * q;
-  float best;
   int ok = 0;
-  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, slice_of<NT>(dyn, p), best, sh);
-  const float top = row_top(sl, best, sh), l = rewritten(lx, sl.how);
-  if (l > -INFINITY) {  // a token (and so the row has a top)
+  if (lx > -INFINITY) {  // a token
+    uint4* buf = slice_of<NT>(dyn, p);
+    Slice<T, NT, kShared> sl = make_slice<T, NT, kShared>(row, p.vocab, p.slice, buf, sh);
+    float top;
     if (!(t > 0.f)) {
-      ok = l == top && row_first(sl, top, sh) == x && uq < 1.0;
+      ok = greedy_walk(sl, buf, top, sh) == x && uq < 1.0;
     } else {
-      const RowScale s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
-      const double wx = weight(l, s);
-      ok = quick_test(sl, s, top_p, x, l, wx, uq, sh);
+      ok = quick_walk(sl, buf, t, top_p, x, lx, uq, top, sh);
       if (ok < 0) {
+        top = settle(sl, top);
+        const float l = rewritten(lx, sl.how);
+        const RowScale s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
         u64 mine;
         Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
-        const Kept k = find_kept(sl, s, top_p, near, sh, mine);
-        ok = k.holds(l, x) && uq < wx * (top_weight(s) / (double)k.total);
+        const Kept k = find_kept(sl, s, top_p, -1.0, near, sh, mine);
+        ok = k.holds(l, x) && uq < weight(l, s) * (top_weight(s) / (double)k.total);
       }
     }
   }
@@ -1120,24 +1453,32 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
   const bool rejected = r + 1 < end;
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const float t = __ldg(p.temperature + req), top_p = __ldg(p.top_p + req), u = __ldg(p.uniform + end - 1);
-  float best;
-  Slice<T, NT, kShared> sl = load_slice<T, NT, kShared>(row, p.vocab, p.slice, slice_of<NT>(dyn, p), best, sh);
-  const float top = row_top(sl, best, sh);
+  uint4* buf = slice_of<NT>(dyn, p);
+  Slice<T, NT, kShared> sl = make_slice<T, NT, kShared>(row, p.vocab, p.slice, buf, sh);
+  const bool greedy = !(t > 0.f), cut = top_p < 1.f;
+  Walk walk;
+  int first = -1;
+  if (greedy) first = greedy_walk(sl, buf, walk.top, sh);
+  else walk = weight_walk(sl, buf, t, sh);
   if (lead) p.accepted[req] = r - begin;
-  if (!(t > 0.f) || top == -INFINITY) {
-    const int first = top == -INFINITY ? 0 : row_first(sl, top, sh);
-    if (lead) p.tokens[req] = first;
+  if (greedy || walk.top == -INFINITY) {
+    if (lead) p.tokens[req] = max(first, 0);
+  } else if (!cut && !rejected && !walk.far && u >= kLeastU) {
+    settle(sl, walk.top);
+    draw_all(sl, walk, t, u, p.tokens + req, sh);
   } else {
+    const float top = settle(sl, walk.top);
     Mass mass;
     mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
     u64 mine;
     Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
-    mass.kept = find_kept(sl, mass.s, top_p, near, sh, mine);
+    const double known = cut || rejected ? in_fixed_units(walk, mass.s) : -1.0;
+    mass.kept = find_kept(sl, mass.s, top_p, known, near, sh, mine);
     mass.inv_z = 1.0 / (double)mass.kept.total;
     mass.residual = rejected;
     mass.minus = rejected && p.draft_probs != nullptr ? p.draft_probs + (int64_t)r * p.draft_stride : nullptr;
     mass.one_hot = rejected ? __ldg(p.draft + r + 1) : -1;
-    if (!draw(sl, mass, near, u, !rejected && !(top_p < 1.f), mine, 33, p.tokens + req, sh)) {
+    if (!draw(sl, mass, near, u, !rejected && !cut, mine, 33, p.tokens + req, sh)) {
       mass.residual = false;  // nothing left above the draft's distribution: the target's own
       draw(sl, mass, near, u, false, 0, 34, p.tokens + req, sh);
     }

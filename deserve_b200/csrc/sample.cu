@@ -274,6 +274,7 @@ struct Slice {
   int n_vec, first;
   int seg, sub;    // vectors of a warp's contiguous segment, of a subsegment
   int lead, tail;  // entries of the first and of the last vector that lie outside
+  int limit;       // entries of the row
   int how;
   __device__ __forceinline__ void mask(int i, float (&f)[N]) const {
     if (i == 0 || i == n_vec - 1) {
@@ -404,6 +405,7 @@ __device__ __forceinline__ Slice<T, NT, kShared> make_slice(const T* row, int vo
   sl.tail = sl.n_vec * N - sl.lead - n;
   sl.seg = ((sl.n_vec + W * 32 - 1) / (W * 32)) * 32;
   sl.sub = ((sl.seg + kSub * 32 - 1) / (kSub * 32)) * 32;
+  sl.limit = vocab;
   sl.how = kAsIs;
   return sl;
 }
@@ -414,6 +416,7 @@ template <typename T, int NT, bool kShared, typename F>
 __device__ __forceinline__ void first_walk(const Slice<T, NT, kShared>& sl, uint4* buf, F of) {
   constexpr int N = Vec16<T>::N, DEPTH = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, a = sl.begin(warp), b = sl.end(warp);
+  const unsigned inner = (unsigned)max(min(b, sl.n_vec - 1) - 1, 0);  // vectors 1 .. inner need no mask
   uint4 u[DEPTH];
 #pragma unroll
   for (int k = 0; k < DEPTH; ++k) {
@@ -430,10 +433,10 @@ __device__ __forceinline__ void first_walk(const Slice<T, NT, kShared>& sl, uint
       if (kShared && i < b) buf[i] = now;
       float f[N];
       Vec16<T>::unpack(now, f);
-      sl.mask(i, f);
-      if (i >= b) {
+      if ((unsigned)(i - 1) >= inner) {  // the slice's first or last vector, or behind the segment
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = -INFINITY;
+        for (int j = 0; j < N; ++j)
+          if (i >= b || (i == 0 && j < sl.lead) || (i == sl.n_vec - 1 && j >= N - sl.tail)) f[j] = -INFINITY;
       }
       of(f, sl.first + i * N, at);
     }
@@ -1212,6 +1215,131 @@ __device__ __forceinline__ uint4* slice_of(unsigned char* dyn, const SampleParam
   return reinterpret_cast<uint4*>(dyn + (size_t)p.cap * (NT / 32) * sizeof(Entry));
 }
 
+// The draw of a row without a cut from max(p - q, 0), in double like weight_walk: masses of the subsegments, then the one that holds
+// the target again. false: no mass. Slot 33.
+template <typename T, int NT, bool kShared>
+__device__ bool draw_rest(const Slice<T, NT, kShared>& sl, const Walk& walk, float temperature, const float* q, int one_hot, float u,
+                          int32_t* out, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float t = fminf(fmaxf(temperature, 1e-30f), 1e36f), lowest = walk.top - 31.2f * t;
+  const double c = 92.332482616893657 / (double)t, magic = 6755399441055744.0 - 64.0 * walk.e, inv = 1.0 / walk.total;
+  const bool wide = q != nullptr && ((reinterpret_cast<uintptr_t>(q + sl.first) & 15) == 0);
+  auto rest_of = [&](const float (&f)[N], int i0, double (&m)[N]) {
+    float d[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = i0 + i == one_hot ? 1.f : 0.f;
+    if (q != nullptr) {
+      const bool inside = i0 >= 0 && i0 + N <= sl.limit;
+      if (wide && inside) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const float4 x = __ldg(reinterpret_cast<const float4*>(q + i0 + i));
+          d[i] = x.x; d[i + 1] = x.y; d[i + 2] = x.z; d[i + 3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) d[i] = f[i] >= lowest ? __ldg(q + i0 + i) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {  // as in weight_walk
+      const double x = (double)fmaxf(f[i], lowest), w = fma(x, c, magic), r = fma(x, c, magic - w);
+      constexpr double a = 0.010830424696249145;
+      double y = fma(r, a * a * a * a / 24.0, a * a * a / 6.0);
+      y = fma(r, y, a * a / 2.0);
+      y = fma(r, y, a);
+      y = fma(r, y, 1.0);
+      const int n = __double2loint(w);
+      const double p = sh.table[n & (kTable - 1)];
+      y = fma(__hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p)) * y, inv, -(double)d[i]);
+      m[i] = f[i] >= lowest && y > 0.0 ? y : 0.0;
+    }
+  };
+  double mass = 0.0;
+  const int e = sl.end(warp);
+  int at = sl.begin(warp);
+  __syncthreads();  // weight_walk's masses in sh.seg are no longer needed
+  for (int k = 0; k < kSub; ++k) {
+    const int stop = min(at + sl.sub, e);
+    double x = 0.0;
+    sl.each(at + lane, stop, 32, [&](const float (&f)[N], int i0) {
+      double m[N];
+      rest_of(f, i0, m);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x += m[i];
+    });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (lane == 0) sh.seg[warp * kSub + k] = as_bits(x);
+    mass += x;
+    at = stop;
+  }
+  if (lane == 0) sh.warp_a[warp] = as_bits(mass);
+  __syncthreads();
+  double inc, same = 0.0;
+  if (warp == 0) {
+    mass = lane < NT / 32 ? as_double(sh.warp_a[lane]) : 0.0;
+    same = 0.0;
+    join(mass, same, inc, lane);
+    const double all = __shfl_sync(0xffffffffu, inc, 31);
+    if (lane == 0) sh.slot[33].a = as_bits(all);
+  }
+  cluster_sync();
+  mass = lane < (int)cluster_size() ? as_double(ld_remote64(remote(&sh.slot[33].a, lane))) : 0.0;
+  same = 0.0;
+  join(mass, same, inc, lane);
+  const double all = __shfl_sync(0xffffffffu, inc, 31);
+  if (!(all > 0.0)) return false;
+  if (warp != 0) return true;
+  double rest;
+  if (pick(inc, u > 0.f ? fmin((double)u, 1.0) * all : 0.0, rest) != (int)cluster_rank()) return true;
+  mass = lane < NT / 32 ? as_double(sh.warp_a[lane]) : 0.0;
+  join(mass, same, inc, lane);
+  const int w = pick(inc, rest, rest);
+  mass = lane < kSub ? as_double(sh.seg[w * kSub + lane]) : 0.0;
+  join(mass, same, inc, lane);
+  const int k = pick(inc, rest, rest), a = min(sl.begin(w) + k * sl.sub, sl.end(w)), b = min(a + sl.sub, sl.end(w));
+  int last = -1;
+  for (int v0 = a; v0 < b; v0 += 32) {
+    const int v = v0 + lane;
+    float f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = -INFINITY;
+    if (v < b) sl.get(v, f);
+    double m[N], total = 0.0;
+    int mine = -1;
+    rest_of(f, sl.first + min(v, b - 1) * N, m);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      total += m[i];
+      if (m[i] > 0.0) mine = sl.first + v * N + i;
+    }
+    mass = total;
+    join(mass, same, inc, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, inc > rest);
+    if (hit) {
+      const int who = __ffs(hit) - 1;
+      const double before = __shfl_up_sync(0xffffffffu, inc, 1);
+      if (lane == who) {
+        double run = lane > 0 ? before : 0.0;
+        int i = -1;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (m[j] > 0.0 && (i < 0 || run <= rest)) i = j;
+          run += m[j];
+        }
+        *out = sl.first + v * N + i;
+      }
+      return true;
+    }
+    last = max(last, __reduce_max_sync(0xffffffffu, mine));
+    rest = fmax(rest - __shfl_sync(0xffffffffu, inc, 31), 0.0);
+  }
+  if (lane == 0) *out = max(last, 0);
+  return true;
+}
+
 // The sum of weight_walk in units of the fixed-point weights, -1 where it does not hold.
 __device__ __forceinline__ double in_fixed_units(const Walk& w, const RowScale& s) {
   return w.far ? -1.0 : w.total * exp2(44.0 + (w.e - (6755399441055744.0 - s.magic) * 0.015625));
@@ -1285,18 +1413,20 @@ __device__ __forceinline__ int owner_of(const int32_t* __restrict__ indptr, int 
 
 // Does the draft x of a row pass, u q(x) < p(x)? The answer needs p(x) only to one side of u q(x): sums in fp32 from the first
 // walk decide unless they come too close, or the nucleus' exact mass is needed (Z lies between top_p and 1 times the whole sum).
-// Relative error of the sums: 2^-22 of ex2.approx, 2^-22 for each of at most 80 factors of two of the exponent, 2^-24 for each of a
-// subsegment's additions: below 3e-5. 1: yes, 0: no, -1: not known. Also the row's top. Slots 0 and 1.
+// Relative error of the sums: 2^-22 of ex2.approx, 2^-24 of an exponent below 2^14 (kept to 80 above the first entries, what lies far
+// below does not count), 2^-24 of c for the same, 2^-24 for each of 128 additions: below 5e-5 up to exponents of 300; larger ones are
+// left to the exact way. 1: yes, 0: no, -1: not known. Also the row's top. Slots 0 and 1.
 template <typename T, int NT, bool kShared>
 __device__ int quick_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float temperature, float top_p, int x, float lx, double uq, float& top,
                           Shared& sh) {
   constexpr int N = Vec16<T>::N;
-  constexpr double kGuard = 6e-5;
+  constexpr double kGuard = 1e-4;
   constexpr float kOctaves = 80.f;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float t = fminf(fmaxf(temperature, 1e-30f), 1e36f), c32 = 1.442695041f / t;
   const bool cut = top_p < 1.f;
-  float m0 = -INFINITY, cutoff = 0.f, best = -INFINITY, all = 0.f, above = 0.f;
+  float m0 = -INFINITY, shift = 0.f, best = -INFINITY, all = 0.f, above = 0.f;
+  const float below = lx == 0.f ? -1.4e-45f : __uint_as_float(__float_as_uint(lx) + (lx > 0.f ? -1 : 1));
   double sum_all = 0.0, sum_above = 0.0;
   int turn = 0;
   first_walk(sl, buf, [&](const float (&f)[N], int i0, int) {
@@ -1306,14 +1436,21 @@ __device__ int quick_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float tem
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       m0 = m;
-      cutoff = m - fminf(0.69f * 120.f * t, 1e37f);
+      shift = -m0 * c32;
     }
     if (m0 > -INFINITY) {
+      // Entries of lower index rank ahead of x among equals: they are compared with the number just below lx.
+      const float bar = i0 < x ? below : lx;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float w = ex2((fmaxf(f[i], cutoff) - m0) * c32);
+        const float w = ex2(fmaf(f[i], c32, shift));  // (NaN makes the sums NaN: not known)
         all += w;
-        if (cut) above += f[i] > lx || (f[i] == lx && i0 + i < x) ? w : 0.f;
+        if (cut && f[i] > bar) above += w;
+      }
+      if (cut && i0 <= x && x < i0 + N) {  // the vector of x itself: what ranks behind it was counted
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (i0 + i >= x && f[i] == lx) above -= i0 < x ? ex2(fmaf(f[i], c32, shift)) : 0.f;
       }
     }
     if (++turn == 16) {
@@ -1332,8 +1469,8 @@ __device__ int quick_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float tem
     best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
   }
   const double c = 1.4426950408889634 / (double)t;
-  bool far = best > -INFINITY && !((best - m0) * c32 < kOctaves && cutoff > -3e38f && cutoff < m0);
-  double e = m0 > -INFINITY && !far ? (double)m0 * c : -INFINITY;
+  bool far = best > -INFINITY && !((best - m0) * c32 < kOctaves && fabsf(shift) < 300.f);
+  double e = m0 > -INFINITY && !far ? -(double)shift : -INFINITY;  // (shift as rounded: one factor for all)
   if (lane == 0) {
     sh.warp_a[warp] = as_bits(sum_all);
     sh.warp_b[warp] = as_bits(e);
@@ -1463,9 +1600,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
   if (lead) p.accepted[req] = r - begin;
   if (greedy || walk.top == -INFINITY) {
     if (lead) p.tokens[req] = max(first, 0);
-  } else if (!cut && !rejected && !walk.far && u >= kLeastU) {
-    settle(sl, walk.top);
-    draw_all(sl, walk, t, u, p.tokens + req, sh);
+  } else if (!cut && !walk.far && u >= kLeastU &&
+             (!rejected || draw_rest(sl, walk, t, p.draft_probs == nullptr ? nullptr : p.draft_probs + (int64_t)r * p.draft_stride,
+                                     p.draft_probs == nullptr ? __ldg(p.draft + r + 1) : -1, u, p.tokens + req, sh))) {
+    if (!rejected) draw_all(sl, walk, t, u, p.tokens + req, sh);
   } else {
     const float top = settle(sl, walk.top);
     Mass mass;
@@ -1492,15 +1630,20 @@ struct Shape {
   bool shared;  // rows in shared memory, 512 threads; else in L2, 256 threads
   size_t smem;
 };
-// Few rows: as many CTAs (up to 8) per row as the SMs have room for, the row in shared memory. Many rows: one CTA per
-// row and four per SM, later passes from L2 (592 rows at once, so 128,256 entries of 16 bits for each just about fill
-// its 126 MB); the CTAs of a cluster wait for one another at every exchange, which costs more than reading L2.
+// Few rows: as many CTAs (up to 8) per row as two per SM have room for, the row in shared memory. Many rows: CTAs of 256
+// threads, four per SM, later walks from L2; up to 8 CTAs per row while there are not more than about four rounds of them.
+// (128 rows of 128,256: 8 CTAs from L2 and 4 from shared memory the same within 5 %, 1 from L2 three times as long; 1024 rows: 1 or 2
+// from L2 the same, 4 from shared memory twice as long, since the CTAs of a cluster wait for one another at every exchange.)
 Shape pick_shape(int rows, int vocab, int es) {
   Shape s;
   s.ctas = 1;
   while (s.ctas < kMaxCtas && (int64_t)rows * s.ctas * 2 <= 296 && vocab / (s.ctas * 2) >= 2048) s.ctas *= 2;
+  s.shared = (int64_t)rows * s.ctas <= 296 && (int64_t)(vocab / s.ctas + 64) * es <= 72 * 1024;
+  if (!s.shared) {
+    s.ctas = 1;
+    while (s.ctas < kMaxCtas && (int64_t)rows * s.ctas * 2 <= 2400 && vocab / (s.ctas * 2) >= 2048) s.ctas *= 2;
+  }
   s.slice = ((vocab + s.ctas - 1) / s.ctas + 63) & ~63;
-  s.shared = (int64_t)rows * s.ctas <= 296 && (int64_t)s.slice * es <= 72 * 1024;
   s.cap = s.shared ? 64 : 176;
   s.smem = (s.shared ? (size_t)s.slice * es + 32 : 0) + (size_t)s.cap * (s.shared ? 16 : 8) * sizeof(Entry);
   return s;

@@ -101,6 +101,11 @@ struct Shared {
   u64 border, kept;
 };
 
+struct QuickShared {
+  Slot slot[2];
+  u64 warp_a[kMaxWarps], warp_b[kMaxWarps], warp_c[kMaxWarps], warp_d[kMaxWarps];
+};
+
 // ---- cluster plumbing ------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -390,10 +395,8 @@ __device__ __forceinline__ void marked(const float (&f)[N], unsigned in, F of) {
 
 // Geometry of the slice; `first_walk` brings it in.
 template <typename T, int NT, bool kShared>
-__device__ __forceinline__ Slice<T, NT, kShared> make_slice(const T* row, int vocab, int slice, uint4* buf, Shared& sh) {
+__device__ __forceinline__ Slice<T, NT, kShared> make_slice(const T* row, int vocab, int slice, uint4* buf) {
   constexpr int N = Vec16<T>::N, W = NT / 32;
-  if (threadIdx.x < kTable) sh.table[threadIdx.x] = kPowers[threadIdx.x];
-  if (threadIdx.x == 0) sh.n_list = 0;
   const int begin = min((int)cluster_rank() * slice, vocab), n = min(begin + slice, vocab) - begin;
   const T* src = row + begin;
   Slice<T, NT, kShared> sl;
@@ -451,8 +454,8 @@ __device__ __forceinline__ float settle(Slice<T, NT, kShared>& sl, float top) {
 }
 
 // Greedy walk: the row's largest entry that is a number and its lowest index (-1: there is none). Slot 0.
-template <typename T, int NT, bool kShared>
-__device__ int greedy_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float& top, Shared& sh) {
+template <typename T, int NT, bool kShared, typename S>
+__device__ int greedy_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float& top, S& sh) {
   constexpr int N = Vec16<T>::N;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float best = -INFINITY;
@@ -519,7 +522,9 @@ __device__ Walk weight_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float t
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float t = fminf(fmaxf(temperature, 1e-30f), 1e36f);
   const double c = 92.332482616893657 / (double)t;
-  __syncthreads();  // the table
+  if (threadIdx.x < kTable) sh.table[threadIdx.x] = kPowers[threadIdx.x];
+  if (threadIdx.x == 0) sh.n_list = 0;
+  __syncthreads();
   float top = -INFINITY, cutoff = 0.f;
   double e = -INFINITY, magic = 0.0, mass = 0.0, part = 0.0;
   bool far = false;
@@ -1355,7 +1360,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const float t = __ldg(p.temperature + r), top_p = __ldg(p.top_p + r), u = __ldg(p.uniform + r);
   uint4* buf = slice_of<NT>(dyn, p);
-  Slice<T, NT, kShared> sl = make_slice<T, NT, kShared>(row, p.vocab, p.slice, buf, sh);
+  Slice<T, NT, kShared> sl = make_slice<T, NT, kShared>(row, p.vocab, p.slice, buf);
   const int begin = min((int)cluster_rank() * p.slice, p.vocab), end = min(begin + p.slice, p.vocab);
   float* probs = p.probs == nullptr ? nullptr : p.probs + (int64_t)r * p.probs_stride;
   const bool greedy = !(t > 0.f);
@@ -1415,10 +1420,9 @@ __device__ __forceinline__ int owner_of(const int32_t* __restrict__ indptr, int 
 // walk decide unless they come too close, or the nucleus' exact mass is needed (Z lies between top_p and 1 times the whole sum).
 // Relative error of the sums: 2^-22 of ex2.approx, 2^-24 of an exponent below 2^14 (kept to 80 above the first entries, what lies far
 // below does not count), 2^-24 of c for the same, 2^-24 for each of 128 additions: below 5e-5 up to exponents of 300; larger ones are
-// left to the exact way. 1: yes, 0: no, -1: not known. Also the row's top. Slots 0 and 1.
-template <typename T, int NT, bool kShared>
-__device__ int quick_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float temperature, float top_p, int x, float lx, double uq, float& top,
-                          Shared& sh) {
+// left to the exact way. 1: yes, 0: no, -1: not known. Slots 0 and 1.
+template <typename T, int NT>
+__device__ int quick_walk(const Slice<T, NT, false>& sl, float temperature, float top_p, int x, float lx, double uq, QuickShared& sh) {
   constexpr int N = Vec16<T>::N;
   constexpr double kGuard = 1e-4;
   constexpr float kOctaves = 80.f;
@@ -1429,7 +1433,7 @@ __device__ int quick_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float tem
   const float below = lx == 0.f ? -1.4e-45f : __uint_as_float(__float_as_uint(lx) + (lx > 0.f ? -1 : 1));
   double sum_all = 0.0, sum_above = 0.0;
   int turn = 0;
-  first_walk(sl, buf, [&](const float (&f)[N], int i0, int) {
+  first_walk(sl, nullptr, [&](const float (&f)[N], int i0, int) {
     float m = largest(f);
     best = fmaxf(best, m);
     if (m0 == -INFINITY) {  // warp-uniform
@@ -1475,14 +1479,14 @@ __device__ int quick_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float tem
     sh.warp_a[warp] = as_bits(sum_all);
     sh.warp_b[warp] = as_bits(e);
     sh.warp_c[warp] = (u64)__float_as_uint(best) | (far ? 1ull << 32 : 0);
-    sh.seg[warp] = as_bits(sum_above);
+    sh.warp_d[warp] = as_bits(sum_above);
   }
   __syncthreads();
   double inc, own;
   if (warp == 0) {
     const bool in = lane < NT / 32;
     sum_all = in ? as_double(sh.warp_a[lane]) : 0.0;
-    sum_above = in ? as_double(sh.seg[lane]) : 0.0;
+    sum_above = in ? as_double(sh.warp_d[lane]) : 0.0;
     own = e = in ? as_double(sh.warp_b[lane]) : -INFINITY;
     best = in ? __uint_as_float((uint32_t)sh.warp_c[lane]) : -INFINITY;
     far = __any_sync(0xffffffffu, in && (sh.warp_c[lane] >> 32) != 0);
@@ -1514,25 +1518,26 @@ __device__ int quick_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float tem
   best = __uint_as_float((uint32_t)z);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-  top = best;
-  if (__any_sync(0xffffffffu, (z >> 32) != 0) || top == INFINITY || top < -1e38f) return -1;
+  if (__any_sync(0xffffffffu, (z >> 32) != 0) || best == INFINITY || best < -1e38f) return -1;
   const double wx = power((double)lx * c - e);
-  double least = total;  // of Z
+  double least = total, most = total;  // bounds of Z
   if (cut) {
     least = total * fmax((double)top_p, 0.0);
     if (ahead * (1 - kGuard) > least * (1 + kGuard)) return 0;      // not in the nucleus
     if (!(ahead * (1 + kGuard) <= least * (1 - kGuard))) return -1;
+    most = fmin(total, least + wx);  // the border's weight is at most that of a kept token
   }
-  if (uq * total * (1 + kGuard) < wx) return 1;
+  if (uq * most * (1 + kGuard) < wx) return 1;
   if (uq * least * (1 - kGuard) >= wx) return 0;
   return -1;
 }
 
-// One cluster per row that has a draft behind it: is the draft accepted?
-template <typename T, int NT, bool kShared>
-__global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const SampleParams p) {
-  extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ __align__(16) Shared sh;
+// One cluster per row that has a draft behind it: is the draft accepted? Reads its row once and keeps nothing of it.
+enum : uint8_t { kRejected = 0, kAccepted = 1, kUnknown = 2 };
+constexpr int kQuickThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kQuickThreads, 4) verify_rows_kernel(const SampleParams p) {
+  __shared__ QuickShared sh;
   const int r = blockIdx.x / cluster_size();
   const int req = owner_of(p.indptr, p.batch, r);
   const int begin = __ldg(p.indptr + req), end = __ldg(p.indptr + req + 1);
@@ -1546,30 +1551,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_rows_kernel(const Sample
   const double uq = (double)__ldg(p.uniform + r) * q;
   int ok = 0;
   if (lx > -INFINITY) {  // a token
-    uint4* buf = slice_of<NT>(dyn, p);
-    Slice<T, NT, kShared> sl = make_slice<T, NT, kShared>(row, p.vocab, p.slice, buf, sh);
+    const Slice<T, kQuickThreads, false> sl = make_slice<T, kQuickThreads, false>(row, p.vocab, p.slice, nullptr);
     float top;
-    if (!(t > 0.f)) {
-      ok = greedy_walk(sl, buf, top, sh) == x && uq < 1.0;
-    } else {
-      ok = quick_walk(sl, buf, t, top_p, x, lx, uq, top, sh);
-      if (ok < 0) {
-        top = settle(sl, top);
-        const float l = rewritten(lx, sl.how);
-        const RowScale s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
-        u64 mine;
-        Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
-        const Kept k = find_kept(sl, s, top_p, -1.0, near, sh, mine);
-        ok = k.holds(l, x) && uq < weight(l, s) * (top_weight(s) / (double)k.total);
-      }
-    }
+    if (!(t > 0.f)) ok = greedy_walk(sl, nullptr, top, sh) == x && uq < 1.0;
+    else ok = quick_walk(sl, t, top_p, x, lx, uq, sh);
   }
-  if (cluster_rank() == 0 && threadIdx.x == 0) p.ok[r] = (uint8_t)ok;
+  if (cluster_rank() == 0 && threadIdx.x == 0) p.ok[r] = ok < 0 ? kUnknown : ok ? kAccepted : kRejected;
   cluster_sync();
 }
 
-// One cluster per request: the accepted prefix, then a draw from the residual of the first rejected row or
-// from the last row.
+// One cluster per request: the accepted prefix (drafts that the sums of the rows kernel did not decide are tested exactly), then a
+// draw from the residual of the first rejected row or from the last row.
 template <typename T, int NT, bool kShared>
 __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -1585,41 +1577,62 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
     }
     return;
   }
-  int r = begin;
-  while (r + 1 < end && p.ok[r]) ++r;
-  const bool rejected = r + 1 < end;
-  const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const float t = __ldg(p.temperature + req), top_p = __ldg(p.top_p + req), u = __ldg(p.uniform + end - 1);
-  uint4* buf = slice_of<NT>(dyn, p);
-  Slice<T, NT, kShared> sl = make_slice<T, NT, kShared>(row, p.vocab, p.slice, buf, sh);
   const bool greedy = !(t > 0.f), cut = top_p < 1.f;
-  Walk walk;
-  int first = -1;
-  if (greedy) first = greedy_walk(sl, buf, walk.top, sh);
-  else walk = weight_walk(sl, buf, t, sh);
-  if (lead) p.accepted[req] = r - begin;
-  if (greedy || walk.top == -INFINITY) {
-    if (lead) p.tokens[req] = max(first, 0);
-  } else if (!cut && !walk.far && u >= kLeastU &&
-             (!rejected || draw_rest(sl, walk, t, p.draft_probs == nullptr ? nullptr : p.draft_probs + (int64_t)r * p.draft_stride,
-                                     p.draft_probs == nullptr ? __ldg(p.draft + r + 1) : -1, u, p.tokens + req, sh))) {
-    if (!rejected) draw_all(sl, walk, t, u, p.tokens + req, sh);
-  } else {
-    const float top = settle(sl, walk.top);
+  uint4* buf = slice_of<NT>(dyn, p);
+  for (int r = begin;; ++r) {
+    const uint8_t said = r + 1 < end ? p.ok[r] : kRejected;
+    if (said == kAccepted) continue;
+    const bool last = r + 1 == end;
+    const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
+    const float* q_row = p.draft_probs == nullptr ? nullptr : p.draft_probs + (int64_t)r * p.draft_stride;
+    const int x = last ? -1 : __ldg(p.draft + r + 1);
+    Slice<T, NT, kShared> sl = make_slice<T, NT, kShared>(row, p.vocab, p.slice, buf);
+    Walk walk;
+    int first = -1;
+    if (greedy) first = greedy_walk(sl, buf, walk.top, sh);
+    else walk = weight_walk(sl, buf, t, sh);
     Mass mass;
-    mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
-    u64 mine;
+    u64 mine = 0;
     Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
-    const double known = cut || rejected ? in_fixed_units(walk, mass.s) : -1.0;
-    mass.kept = find_kept(sl, mass.s, top_p, known, near, sh, mine);
-    mass.inv_z = 1.0 / (double)mass.kept.total;
-    mass.residual = rejected;
-    mass.minus = rejected && p.draft_probs != nullptr ? p.draft_probs + (int64_t)r * p.draft_stride : nullptr;
-    mass.one_hot = rejected ? __ldg(p.draft + r + 1) : -1;
-    if (!draw(sl, mass, near, u, !rejected && !cut, mine, 33, p.tokens + req, sh)) {
-      mass.residual = false;  // nothing left above the draft's distribution: the target's own
-      draw(sl, mass, near, u, false, 0, 34, p.tokens + req, sh);
+    const bool plain = !greedy && !cut && !walk.far && u >= kLeastU;  // sums in double will do
+    const bool none = walk.top == -INFINITY;
+    if (!greedy && !none) {
+      const float top = settle(sl, walk.top);
+      mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
+      const double known = cut || !last ? in_fixed_units(walk, mass.s) : -1.0;
+      if (plain) {
+        mass.kept.value = -INFINITY;
+        mass.kept.index = -1;
+        mass.kept.total = (u64)fmax(in_fixed_units(walk, mass.s), 1.0);
+      } else {
+        mass.kept = find_kept(sl, mass.s, top_p, known, near, sh, mine);
+      }
+      if (said == kUnknown) {
+        const float l = rewritten(to_f32(row[x]), sl.how);
+        const double qx = q_row == nullptr ? 1.0 : (double)__ldg(q_row + x);
+        if (mass.kept.holds(l, x) && (double)__ldg(p.uniform + r) * qx < weight(l, mass.s) * (top_weight(mass.s) / (double)mass.kept.total)) {
+          cluster_sync();  // the others may still read this CTA's slots
+          continue;
+        }
+      }
     }
+    if (lead) p.accepted[req] = r - begin;
+    if (greedy || none) {
+      if (lead) p.tokens[req] = max(first, 0);
+    } else if (plain && last) {
+      draw_all(sl, walk, t, u, p.tokens + req, sh);
+    } else if (!plain || !draw_rest(sl, walk, t, q_row, q_row == nullptr ? x : -1, u, p.tokens + req, sh)) {
+      mass.inv_z = 1.0 / (double)mass.kept.total;
+      mass.residual = !last && !plain;  // (plain: nothing is left above the draft's distribution, the target's own is drawn from)
+      mass.minus = last ? nullptr : q_row;
+      mass.one_hot = q_row == nullptr ? x : -1;
+      if (!draw(sl, mass, near, u, last && !cut && !plain, mine, 31, p.tokens + req, sh) && mass.residual) {
+        mass.residual = false;
+        draw(sl, mass, near, u, false, 0, 34, p.tokens + req, sh);
+      }
+    }
+    break;
   }
   cluster_sync();
 }
@@ -1723,10 +1736,12 @@ int dsv_verify_draft(const void* logits, int64_t row_stride, int nnz, int vocab,
   auto go = [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
     if (nnz > 0) {
-      const Shape shape = pick_shape(nnz, vocab, elem_size(dtype));
-      p.slice = shape.slice; p.cap = shape.cap;
-      const cudaError_t er = shape.shared ? launch<512>(verify_rows_kernel<T, 512, true>, nnz, shape, p, st)
-                                        : launch<256>(verify_rows_kernel<T, 256, false>, nnz, shape, p, st);
+      // one round of CTAs, four per SM, where there are enough rows for it
+      Shape shape = {};
+      shape.ctas = 1;
+      while (shape.ctas < kMaxCtas && (int64_t)nnz * shape.ctas < 592 && vocab / (shape.ctas * 2) >= 2048) shape.ctas *= 2;
+      p.slice = ((vocab + shape.ctas - 1) / shape.ctas + 63) & ~63;
+      const cudaError_t er = launch<kQuickThreads>(verify_rows_kernel<T>, nnz, shape, p, st);
       if (er != cudaSuccess) return er;
     }
     const Shape shape = pick_shape(batch, vocab, elem_size(dtype));

@@ -142,3 +142,14 @@ class FlashPrefillCtx(FlashForwardCtx):
     def init_paged_prefill_ctx(task_datas, kvcaches, wrapper) -> "FlashPrefillCtx":
         c = FlashForwardCtx.init_paged_forward_ctx(task_datas, kvcaches)
         return FlashPrefillCtx(**{k: getattr(c, k) for k in c.__dataclass_fields__}, prefill_wrapper=wrapper)
+
+
+@dataclass
+class FlashVerifyCtx(FlashPrefillCtx):
+    """A speculative step: every request feeds its last token and its drafts, attention runs on the chunk
+    wrapper (kv axis split over the GPU), and the last stage keeps the logits of every row."""
+
+    @staticmethod
+    def init_paged_verify_ctx(task_datas, kvcaches, wrapper) -> "FlashVerifyCtx":
+        c = FlashForwardCtx.init_paged_forward_ctx(task_datas, kvcaches)
+        return FlashVerifyCtx(**{k: getattr(c, k) for k in c.__dataclass_fields__}, prefill_wrapper=wrapper)

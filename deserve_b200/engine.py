@@ -318,7 +318,7 @@ class RingPipeline:
 # =================================================================================================
 from dataclasses import field as _field  # noqa: E402
 
-from .context import FlashPrefillCtx  # noqa: E402
+from .context import FlashPrefillCtx, FlashVerifyCtx  # noqa: E402
 from .kvcache import ChunkHandle, KVCacheManager, PageTableAllocator, VirtualPagedKVCache, CopiedPinnedMemory  # noqa: E402
 from .task import SamplingParams, TaskManager  # noqa: E402
 
@@ -444,6 +444,65 @@ class BatchPrefill(BatchExec):
             return self.post_process(result, ignore_eos)
 
 
+_VERIFY_WRAPPERS: dict = {}
+
+
+def verify_wrapper(device) -> ops.BatchChunkWithPagedKVCacheWrapper:
+    """One 128 MiB workspace and chunk wrapper per device, beside those of stage_wrappers."""
+    key = torch.device(device).index or 0
+    if key not in _VERIFY_WRAPPERS:
+        _VERIFY_WRAPPERS[key] = ops.BatchChunkWithPagedKVCacheWrapper(torch.empty(128 << 20, dtype=torch.uint8, device=device))
+    return _VERIFY_WRAPPERS[key]
+
+
+@dataclass
+class VerifyResult:
+    """What the last stage says to a speculative step: request i (task_ids[i]) keeps the first accepted[i] of its
+    drafts and goes on with tokens[i]. logits: the target's, one row per token fed."""
+
+    task_ids: list
+    accepted: torch.Tensor
+    tokens: torch.Tensor
+    logits: torch.Tensor
+
+
+@dataclass
+class BatchVerify(BatchExec):
+    """A speculative step: row block i is request i's last token followed by its drafts (TaskData.seqlen of them
+    together). It has no counterpart in the reference, whose requests advance one token per step. tokens: the ids
+    that were fed, where xs holds activations (a later stage); draft_probs and uniform as in LlamaStage.verify."""
+
+    tokens: Optional[torch.Tensor] = None
+    draft_probs: Optional[torch.Tensor] = None
+    uniform: Optional[torch.Tensor] = None
+    verify_ctx: Optional[FlashVerifyCtx] = None
+
+    def prepare(self) -> None:
+        for t in self.task_datas:
+            if not t.is_prefill():
+                raise ValueError(f"task {t.task_id}: drafts are verified behind the whole prompt ({t.start_pos} of {t.initial_seqlen} "
+                                 "tokens are in the cache)")
+        wrapper = verify_wrapper(self.kvcaches[0].pool.main_device)
+        self.verify_ctx = FlashVerifyCtx.init_paged_verify_ctx(self.task_datas, self.kvcaches, wrapper)
+        a, c = self.layer_storage.model_args, self.verify_ctx
+        wrapper.begin_forward(c.indptr, c.kv_page_indptr, c.kv_page_indices, c.kv_last_page_lens, a.n_heads, a.n_kv_heads,
+                              a.dim // a.n_heads, c.page_pool.page_size, c.page_pool.main_dtype,
+                              qo_indptr_host=c.host["indptr"], kv_indptr_host=c.host["kv_page_indptr"])
+
+    def step(self, ignore_eos: bool):
+        """BatchResult of activations, on the stage that samples a VerifyResult."""
+        ids = [t.task_id for t in self.task_datas]
+        with torch.inference_mode():
+            result = self.layer_storage.forward(self.xs, self.verify_ctx)
+            self.verify_ctx.prefill_wrapper.end_forward()
+            if not self.layer_storage.need_sample:
+                return BatchResult(result, ids, result, ids, [], {})
+            tokens = self.xs if self.tokens is None else self.tokens
+            accepted, following = self.layer_storage.verify(result, tokens, self.verify_ctx.indptr, self.task_datas,
+                                                            self.draft_probs, self.uniform)
+            return VerifyResult(ids, accepted, following, result)
+
+
 class MicroBatchProcessor:
     """One microbatch: its tasks' KV caches and the pinned image of its swap
     region (deserve_worker/engine/microbatch/processor.py:24-149)."""
@@ -503,6 +562,28 @@ class MicroBatchProcessor:
         batch = self._batch(task_ids, xs)
         batch.prepare()
         return batch.step(self.ignore_eos)
+
+    def verify(self, task_ids: list, xs: torch.Tensor, tokens: torch.Tensor | None = None,
+               draft_probs: torch.Tensor | None = None, uniform: torch.Tensor | None = None):
+        """A speculative step of these tasks, whose TaskData.init was given 1 + drafts each; see BatchVerify. The caller
+        ends it with commit() on every stage."""
+        batch = BatchVerify(xs, self.layer_storage, [self.task_data_manager.get(t) for t in task_ids],
+                            [self.ongoing_paged_kvcaches[t] for t in task_ids], tokens=tokens, draft_probs=draft_probs, uniform=uniform)
+        batch.prepare()
+        return batch.step(self.ignore_eos)
+
+    def commit(self, task_ids: list, accepted: list) -> list:
+        """End of a speculative step: the tasks move on by their accepted drafts and the token drawn behind them. Returns the
+        tasks that are done by their token or length limits."""
+        done = []
+        for task_id, n in zip(task_ids, accepted):
+            task = self.task_data_manager.get(task_id)
+            task.step_verified(int(n))
+            sp = task.sampling_params
+            sp.max_new_tokens -= int(n) + 1
+            if sp.max_new_tokens <= 0 or task.start_pos >= sp.max_seq_len:
+                done.append(task_id)
+        return done
 
     def step(self, task_ids: list, xs: torch.Tensor, prev_group: "MicroBatchProcessor",
              next_group: "MicroBatchProcessor") -> BatchResult:

@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ops
-from .context import FlashDecodeCtx, FlashForwardCtx, FlashPrefillCtx
+from .context import FlashDecodeCtx, FlashForwardCtx, FlashPrefillCtx, FlashVerifyCtx
 from .task import TaskData
 
 
@@ -65,8 +65,11 @@ class LlamaStage:
     tokens, the last one also applies the final norm and the output projection."""
 
     def __init__(self, args: ModelArgs, layer_begin: int, layer_end: int, device, dtype, seed: int = 0,
-                 first: bool | None = None, last: bool | None = None, split_head: bool = False):
-        """split_head: the output projection is cut in two halves of the vocabulary. The LAST stage
+                 first: bool | None = None, last: bool | None = None, split_head: bool = False,
+                 sample_seed: int | None = None):
+        """sample_seed: requests with a temperature above 0 are sampled (temperature, top_p) with random
+        numbers of a generator of this seed; None: every request is greedy.
+        split_head: the output projection is cut in two halves of the vocabulary. The LAST stage
         applies the final norm, computes the logits of the lower half and their row maxima, and hands
         on the normed rows together with (max, argmax) of its half (`pack_partial`); the FIRST stage
         computes the upper half, combines the two (`finish_head`) and embeds the tokens for the next
@@ -83,6 +86,7 @@ class LlamaStage:
         self.need_sample = is_last and not split_head  # with a split head nobody samples inside forward()
         self.vocab_lo = (args.vocab_size // 2 + 7) // 8 * 8
         self.main_device, self.dtype = torch.device(device), dtype
+        self.generator = None if sample_seed is None else torch.Generator(device=device).manual_seed(sample_seed)
         a, hd = args, args.head_dim
         qkv_rows = (a.n_heads + 2 * a.n_kv_heads) * hd
         self.layers = []
@@ -167,14 +171,14 @@ class LlamaStage:
     def forward(self, h: torch.Tensor, ctx: FlashForwardCtx) -> torch.Tensor:
         """h: token ids [nnz] on the first stage, activations [nnz, dim] otherwise.
         Returns activations, or on the last stage the logits of every request's
-        last row [bsz, vocab]."""
+        last row [bsz, vocab] (of every row in a speculative step, [nnz, vocab])."""
         if self.need_tokenize:
             h = self.tok_embeddings[h.long()]
         for w in self.layers:
             h = self._block(w, h, ctx)
             ctx.layer_id += 1
         if self.need_sample or self.head_lo:
-            if h.shape[0] != ctx.bsz:  # prompt chunks: only every request's last row is sampled
+            if h.shape[0] != ctx.bsz and not isinstance(ctx, FlashVerifyCtx):  # prompt chunks: only last rows are sampled
                 h = h[(ctx.indptr[1:] - 1).long()]
             hn = rmsnorm(h, self.norm, self.model_args.norm_eps)
             h = self.pack_partial(hn) if self.head_lo else torch.mm(hn, self.output.t())
@@ -182,11 +186,15 @@ class LlamaStage:
 
     @torch.inference_mode()
     def sample(self, logits: torch.Tensor, task_datas: list[TaskData], ignore_eos: bool):
-        """Greedy next token of every request that finished its prompt (one batched
-        argmax and one device->host copy instead of the reference's per-task
-        argmax + cat, layer_storage.py:219-253). Returns (tokens [bsz] int32 on the
+        """Next token of every request that finished its prompt (one batched argmax, or
+        one sampling launch where a generator was given and a request has a temperature
+        above 0, instead of the reference's per-task loop, layer_storage.py:219-253). Returns (tokens [bsz] int32 on the
         device, mask of requests that produced a token, ids done)."""
-        tokens = ops.greedy_sample(logits)
+        if self.generator is not None and any(t.sampling_params.temperature > 0 for t in task_datas):
+            temperature, top_p = self._sampling_params(task_datas, logits.device)
+            tokens = ops.sample_top_p(logits, temperature, top_p, self.uniform(len(task_datas), logits.device))
+        else:
+            tokens = ops.greedy_sample(logits)
         produced, done = [], []
         for t in task_datas:
             fin = t.finished_prefill()
@@ -196,3 +204,32 @@ class LlamaStage:
                 if t.sampling_params.max_new_tokens <= 0 or t.start_pos >= t.sampling_params.max_seq_len:
                     done.append(t.task_id)
         return tokens, produced, done
+
+    # ---- sampling and speculative verification -----------------------------------------------------
+    def _sampling_params(self, task_datas: list[TaskData], device) -> tuple[torch.Tensor, torch.Tensor]:
+        host = torch.tensor([[t.sampling_params.temperature for t in task_datas], [t.sampling_params.top_p for t in task_datas]],
+                            dtype=torch.float32)
+        if torch.device(device).type == "cuda":
+            host = host.pin_memory()
+        return host.to(device, non_blocking=True).unbind(0)
+
+    def uniform(self, n: int, device) -> torch.Tensor:
+        """n random numbers in [0, 1) of this stage's generator (0.5 for a greedy stage, which does not look at them)."""
+        if self.generator is None:
+            return torch.full((n,), 0.5, device=device)
+        return torch.rand(n, generator=self.generator, device=device)
+
+    @torch.inference_mode()
+    def verify(self, logits: torch.Tensor, tokens: torch.Tensor, indptr: torch.Tensor, task_datas: list[TaskData],
+               draft_probs: torch.Tensor | None = None, uniform: torch.Tensor | None = None):
+        """The target's verdict on the drafted tokens of a speculative step: (accepted drafts, next token) per
+        request, int32 on the device. tokens [nnz] are the ids that were fed (every request's last token and its
+        drafts), logits [nnz, vocab] the stage's answer; draft_probs [nnz, vocab] the draft model's probabilities
+        row by row (None: drafts without a distribution). A request is greedy unless it has a temperature above 0
+        and the stage a generator."""
+        temperature, top_p = self._sampling_params(task_datas, logits.device)
+        if self.generator is None:
+            temperature = torch.zeros_like(temperature)
+        if uniform is None:
+            uniform = self.uniform(logits.shape[0], logits.device)
+        return ops.verify_draft(logits, tokens, indptr, uniform, temperature, top_p, draft_probs)

@@ -52,6 +52,14 @@ class TaskData:
         self.seqlen = 1 if self.start_pos >= self.initial_seqlen else 0
         self.round += 1
 
+    def step_verified(self, accepted: int) -> None:
+        """A speculative step is over: the last token and `accepted` of the drafts fed with it are in the cache for
+        good (the next step writes over the rejected ones), and one token drawn by the target is fed next."""
+        assert self.is_prefill() and 0 <= accepted < self.seqlen
+        self.start_pos += accepted + 1
+        self.seqlen = 1
+        self.round += 1
+
 
 class TaskManager:
     """Registry of TaskData plus the page arithmetic the schedulers use."""

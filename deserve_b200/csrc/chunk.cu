@@ -327,10 +327,9 @@ cudaError_t launch_simple(const ChunkParams& p, int n_items, int tile_tokens, cu
   const int row_blocks = (tile_tokens * (p.n_q_heads / p.n_kv_heads) + kSimpleRows - 1) / kSimpleRows;
   const int64_t grid = (int64_t)n_items * p.n_kv_heads * row_blocks;
   const size_t smem = ((size_t)(kSimpleRows + 2 * kSimpleTok) * (DMAX + 4) + kSimpleRows * 33) * sizeof(float);
-  auto kernel = chunk_simple_kernel<T, DMAX>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem<chunk_simple_kernel<T, DMAX>>(smem);
   if (e != cudaSuccess) return e;
-  kernel<<<(unsigned)grid, kSimpleThreads, smem, st>>>(p, row_blocks);
+  chunk_simple_kernel<T, DMAX><<<(unsigned)grid, kSimpleThreads, smem, st>>>(p, row_blocks);
   return cudaGetLastError();
 }
 int ilog2_exact(int x) {  // log2 of a power of two, -1 otherwise
@@ -350,20 +349,18 @@ int heads_per_cta(int n_kv_heads) {
 template <typename T, int D>
 cudaError_t launch_tma(const CUtensorMap& map, const ChunkParams& p, const chunk_tma::Split& sp, int n_items, cudaStream_t st) {
   const size_t smem = (size_t)512 * D * chunk_tma::kStages + 1024 + 64;
-  auto kernel = chunk_tma::chunk_tma_kernel<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem<chunk_tma::chunk_tma_kernel<T, D>>(smem);
   if (e != cudaSuccess) return e;
-  kernel<<<(unsigned)(n_items * (p.n_kv_heads >> sp.hb_log2)), chunk_tma::kThreads, smem, st>>>(map, p, sp);
+  chunk_tma::chunk_tma_kernel<T, D><<<(unsigned)(n_items * (p.n_kv_heads >> sp.hb_log2)), chunk_tma::kThreads, smem, st>>>(map, p, sp);
   return cudaGetLastError();
 }
 
 template <typename T, int D, bool MERGED>
 cudaError_t launch_tc(const chunk_tc::Maps& m, const ChunkParams& p, int ps_log2, int n_items, cudaStream_t st) {
   const size_t smem = (size_t)2 * 128 * D * 2 + (size_t)(2 + chunk_tc::kVStages) * chunk_tc::kBN * D * 2 + 256 + 1024;
-  auto kernel = chunk_tc::chunk_tc_kernel<T, D, MERGED>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem<chunk_tc::chunk_tc_kernel<T, D, MERGED>>(smem);
   if (e != cudaSuccess) return e;
-  kernel<<<(unsigned)(n_items * p.n_kv_heads), chunk_tc::kThreads, smem, st>>>(m.q, m.k, m.v, p, ps_log2);
+  chunk_tc::chunk_tc_kernel<T, D, MERGED><<<(unsigned)(n_items * p.n_kv_heads), chunk_tc::kThreads, smem, st>>>(m.q, m.k, m.v, p, ps_log2);
   return cudaGetLastError();
 }
 template <typename T>

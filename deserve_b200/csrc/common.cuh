@@ -38,6 +38,20 @@ inline bool dtype_ok(int dtype) { return dtype == DSV_F32 || dtype == DSV_F16 ||
 // of faulting. Address resolved once per device (api.cu).
 int* device_status_ptr();
 
+// Dynamic shared memory that kernel kKernel may be launched with, `bytes` at every call: raised once per device. (The
+// attribute call costs a microsecond or two, as much as a small kernel.)
+template <auto kKernel>
+inline cudaError_t allow_smem(size_t bytes) {
+  static int done[64] = {0};  // per device; threads that race set the same value
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+  if (__atomic_load_n(&done[dev], __ATOMIC_ACQUIRE)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) __atomic_store_n(&done[dev], 1, __ATOMIC_RELEASE);
+  return e;
+}
+
 // detail codes written by kernels
 enum : int {
   ST_BAD_PAGE_ID = 1,   // page id outside [0, num_pages) when the caller gave num_pages

@@ -1638,6 +1638,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
 }
 
 // ---- host --------------------------------------------------------------------------------------------
+constexpr size_t kMostSmem = 96 * 1024;  // of pick_shape: a slice of 72 KB and its alignment, 16 KB of lists
 struct Shape {
   int ctas, slice, cap;
   bool shared;  // rows in shared memory, 512 threads; else in L2, 256 threads
@@ -1662,10 +1663,12 @@ Shape pick_shape(int rows, int vocab, int es) {
   return s;
 }
 
-template <int NT, typename K>
-cudaError_t launch(K kernel, int rows, const Shape& s, const SampleParams& p, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.smem);
-  if (e != cudaSuccess) return e;
+template <auto kKernel, int NT>
+cudaError_t launch(int rows, const Shape& s, const SampleParams& p, cudaStream_t st) {
+  if (s.smem > 0) {
+    const cudaError_t e = allow_smem<kKernel>(kMostSmem);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * s.ctas);
   cfg.blockDim = dim3(NT);
@@ -1677,7 +1680,7 @@ cudaError_t launch(K kernel, int rows, const Shape& s, const SampleParams& p, cu
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return cudaLaunchKernelEx(&cfg, kKernel, p);
 }
 
 }  // namespace
@@ -1704,8 +1707,8 @@ int dsv_sample_top_p(const void* logits, int64_t row_stride, int rows, int vocab
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
-    return shape.shared ? launch<512>(sample_kernel<T, 512, true>, rows, shape, p, st)
-                        : launch<256>(sample_kernel<T, 256, false>, rows, shape, p, st);
+    return shape.shared ? launch<sample_kernel<T, 512, true>, 512>(rows, shape, p, st)
+                        : launch<sample_kernel<T, 256, false>, 256>(rows, shape, p, st);
   };
   const cudaError_t e = dtype == DSV_F32 ? go(float{}) : dtype == DSV_F16 ? go(__half{}) : go(__nv_bfloat16{});
   if (e != cudaSuccess) return fail(DSV_E_CUDA, "sample_top_p launch failed: %s", cudaGetErrorString(e));
@@ -1741,13 +1744,13 @@ int dsv_verify_draft(const void* logits, int64_t row_stride, int nnz, int vocab,
       shape.ctas = 1;
       while (shape.ctas < kMaxCtas && (int64_t)nnz * shape.ctas < 592 && vocab / (shape.ctas * 2) >= 2048) shape.ctas *= 2;
       p.slice = ((vocab + shape.ctas - 1) / shape.ctas + 63) & ~63;
-      const cudaError_t er = launch<kQuickThreads>(verify_rows_kernel<T>, nnz, shape, p, st);
+      const cudaError_t er = launch<verify_rows_kernel<T>, kQuickThreads>(nnz, shape, p, st);
       if (er != cudaSuccess) return er;
     }
     const Shape shape = pick_shape(batch, vocab, elem_size(dtype));
     p.slice = shape.slice; p.cap = shape.cap;
-    return shape.shared ? launch<512>(verify_draw_kernel<T, 512, true>, batch, shape, p, st)
-                      : launch<256>(verify_draw_kernel<T, 256, false>, batch, shape, p, st);
+    return shape.shared ? launch<verify_draw_kernel<T, 512, true>, 512>(batch, shape, p, st)
+                      : launch<verify_draw_kernel<T, 256, false>, 256>(batch, shape, p, st);
   };
   const cudaError_t e = dtype == DSV_F32 ? go(float{}) : dtype == DSV_F16 ? go(__half{}) : go(__nv_bfloat16{});
   if (e != cudaSuccess) return fail(DSV_E_CUDA, "verify_draft launch failed: %s", cudaGetErrorString(e));

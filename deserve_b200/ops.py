@@ -27,20 +27,25 @@ def _i32_dev(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
-def _same_device(what: str, first: torch.Tensor, *others) -> None:
-    _lib.require_cuda(first)
+def _same_device(what: str, first: torch.Tensor, *others) -> int:
+    """Device index of tensors that have to share one."""
+    dev = first.get_device()
+    if dev < 0:
+        _lib.require_cuda(first)
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             _lib.require_cuda(t)
             raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+    return dev
 
 
-def _device_of(t: torch.Tensor):
-    """Context in which the tensor's device is the current one (kernels launch on the current device)."""
-    return _NO_SWITCH if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _on(dev: int):
+    """Context in which device `dev` is the current one (kernels launch on the current device)."""
+    return _NO_SWITCH if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 _NO_SWITCH = contextlib.nullcontext()
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.current_stream_ptr)  # the current stream without an object
 
 
 def _row_stride(t: torch.Tensor, heads: int, dim: int, name: str) -> int:
@@ -438,8 +443,8 @@ def paged_chunk_attention(q: torch.Tensor, qo_indptr: torch.Tensor, paged_kv_cac
     """Causal attention of a few new tokens per request over the paged cache, the kv axis split over the
     GPU. Functional form: every buffer explicit. Rows behind the last request are left as they are; lse,
     if given ([nnz, n_q_heads] fp32), receives the natural-log sum-exp of the scaled scores."""
-    _same_device("chunk attention", q, qo_indptr, paged_kv_cache, kv_indices, kv_indptr, kv_last_page_len, plan_dev,
-                 workspace, out, lse)
+    dev = _same_device("chunk attention", q, qo_indptr, paged_kv_cache, kv_indices, kv_indptr, kv_last_page_len, plan_dev,
+                       workspace, out, lse)
     ps, hkv, d, page_stride = _pages_view(paged_kv_cache)
     if q.dtype != paged_kv_cache.dtype or (out is not None and out.dtype != q.dtype):
         raise ValueError("chunk attention: dtypes of q, out and the pages differ")
@@ -454,18 +459,27 @@ def paged_chunk_attention(q: torch.Tensor, qo_indptr: torch.Tensor, paged_kv_cac
         raise ValueError(f"chunk attention: lse must be a contiguous float32 tensor [{nnz}, {hq}]")
     if qo_indptr.shape[0] != batch + 1 or kv_indptr.shape[0] != batch + 1:
         raise ValueError("chunk attention: qo_indptr and kv_indptr must have batch + 1 entries")
-    if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(d)
-    with _device_of(q):
-        _lib.check(_lib.lib.dsv_paged_chunk_attention(
-            q.data_ptr(), qs, _i32_dev(qo_indptr, "qo_indptr").data_ptr(), paged_kv_cache.data_ptr(), page_stride,
-            paged_kv_cache.shape[0], _i32_dev(kv_indices, "kv_indices").data_ptr(),
-            _i32_dev(kv_indptr, "kv_indptr").data_ptr(), _i32_dev(kv_last_page_len, "kv_last_page_len").data_ptr(),
-            out.data_ptr(), os_, _lib.ptr(lse), plan_host.ctypes.data, _i32_dev(plan_dev, "plan_dev").data_ptr(),
-            _lib.ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), batch, nnz, hq,
-            hkv, d, ps, _lib.dtype_code(q.dtype), float(sm_scale), _lib.current_stream_ptr(q.device)))
-    _lib.LAUNCHES[0] += int(plan_host[1] > 0) + int(plan_host[2] > 0)  # the attention kernel, the merge of split tiles
+    descriptors = (_i32_dev(qo_indptr, "qo_indptr").data_ptr(), _i32_dev(kv_indices, "kv_indices").data_ptr(),
+                   _i32_dev(kv_indptr, "kv_indptr").data_ptr(), _i32_dev(kv_last_page_len, "kv_last_page_len").data_ptr())
+    _launch_chunk(dev, q, qs, descriptors, paged_kv_cache, (ps, hkv, d, page_stride), out, os_, lse, plan_host,
+                  _i32_dev(plan_dev, "plan_dev").data_ptr(), _lib.ptr(workspace),
+                  0 if workspace is None else workspace.numel() * workspace.element_size(), batch, sm_scale)
     return out
+
+
+def _launch_chunk(dev, q, q_stride, descriptors, pages, page_shape, out, out_stride, lse, plan_host, plan_ptr, ws_ptr, ws_bytes,
+                  batch, sm_scale) -> None:
+    ps, hkv, d, page_stride = page_shape
+    qo, indices, indptr, last = descriptors
+    with _on(dev):
+        rc = _lib.lib.dsv_paged_chunk_attention(
+            q.data_ptr(), q_stride, qo, pages.data_ptr(), page_stride, pages.shape[0], indices, indptr, last, out.data_ptr(),
+            out_stride, None if lse is None else lse.data_ptr(), plan_host.ctypes.data, plan_ptr, ws_ptr, ws_bytes, batch,
+            q.shape[0], q.shape[1], hkv, d, ps, _lib.dtype_code(q.dtype), 1.0 / math.sqrt(d) if sm_scale is None else sm_scale,
+            _raw_stream(dev))
+    if rc:
+        _lib.check(rc)
+    _lib.LAUNCHES[0] += int(plan_host[1] > 0) + int(plan_host[2] > 0)  # the attention kernel, the merge of split tiles
 
 
 class BatchChunkWithPagedKVCacheWrapper:
@@ -510,8 +524,14 @@ class BatchChunkWithPagedKVCacheWrapper:
         _pinned_ring("chunk_plan").done(slot)
         _COUNTERS["h2d_bytes"] += used * 4
         self._plan_host = plan[:16].copy()  # the header is all that a call reads on the host
-        self._plan_dev, self._partials = self._ws[: self._PLAN_BYTES].view(torch.int32), self._ws[self._PLAN_BYTES :]
-        self._desc = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len, num_qo_heads, head_dim)
+        batch = len(qo_indptr_host) - 1
+        dev = _same_device("chunk attention", self._ws, qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
+        if paged_kv_last_page_len.shape[0] != batch or qo_indptr.shape[0] != batch + 1 or paged_kv_indptr.shape[0] != batch + 1:
+            raise ValueError("chunk attention: qo_indptr and kv_indptr must have batch + 1 entries, kv_last_page_len batch")
+        pointers = (_i32_dev(qo_indptr, "qo_indptr").data_ptr(), _i32_dev(paged_kv_indices, "kv_indices").data_ptr(),
+                    _i32_dev(paged_kv_indptr, "kv_indptr").data_ptr(), _i32_dev(paged_kv_last_page_len, "kv_last_page_len").data_ptr())
+        self._desc = (dev, batch, num_qo_heads, num_kv_heads, head_dim, page_size, pointers)
+        self._keep = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)  # alive while planned
 
     def forward(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, causal: bool = True, sm_scale: float | None = None,
                 out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
@@ -519,14 +539,32 @@ class BatchChunkWithPagedKVCacheWrapper:
             raise RuntimeError("forward() called outside begin_forward()/end_forward()")
         if not causal:
             raise ValueError("chunk attention is causal: a row sees the cache up to its own position")
-        qo, kv_indptr, kv_indices, last, hq, d = self._desc
+        dev, batch, hq, hkv, d, ps, pointers = self._desc
         if q.dim() == 2:
             q = q.view(-1, hq, d)
-        return paged_chunk_attention(q, qo, paged_kv_cache, kv_indices, kv_indptr, last, self._plan_host, self._plan_dev,
-                                     self._partials, out, sm_scale, lse)
+        _same_device("chunk attention", self._ws, q, paged_kv_cache, out, lse)
+        shape = _pages_view(paged_kv_cache)
+        if shape[:3] != (ps, hkv, d):
+            raise ValueError(f"chunk attention: pages of {shape[:3]} (page size, kv heads, head_dim), planned for {(ps, hkv, d)}")
+        if q.dtype != paged_kv_cache.dtype or (out is not None and out.dtype != q.dtype):
+            raise ValueError("chunk attention: dtypes of q, out and the pages differ")
+        qs = _row_stride(q, hq, d, "q")
+        nnz = q.shape[0]
+        if out is None:
+            out, os_ = torch.empty((nnz, hq, d), dtype=q.dtype, device=q.device), hq * d
+        else:
+            os_ = _row_stride(out, hq, d, "out")
+            if out.shape[0] != nnz:
+                raise ValueError("chunk attention: out must have as many rows as q")
+        if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (nnz, hq) or not lse.is_contiguous()):
+            raise ValueError(f"chunk attention: lse must be a contiguous float32 tensor [{nnz}, {hq}]")
+        at = self._ws.data_ptr()
+        _launch_chunk(dev, q, qs, pointers, paged_kv_cache, shape, out, os_, lse, self._plan_host, at, at + self._PLAN_BYTES,
+                      self._ws.numel() - self._PLAN_BYTES, batch, sm_scale)
+        return out
 
     def end_forward(self) -> None:
-        self._desc = None
+        self._desc = self._keep = None
 
 
 def rope_append_paged_kv_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, indptr: torch.Tensor,
@@ -593,10 +631,9 @@ def greedy_sample(logits: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def _f32_rows(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
+def _f32_rows(t: torch.Tensor, n: int, name: str) -> None:
+    if t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float32 tensor [{n}]")
-    return t
 
 
 def _rows_of(t: torch.Tensor, name: str) -> int:
@@ -613,11 +650,12 @@ def sample_top_p(logits: torch.Tensor, temperature: torch.Tensor, top_p: torch.T
     is the shortest prefix of the tokens by probability (lower index first among equals) whose mass exceeds
     top_p; the draw walks it in index order. probs, if given ([rows, vocab] float32), receives the kept,
     renormalised probabilities: what verify_draft takes as draft_probs."""
-    _same_device("sample_top_p", logits, temperature, top_p, uniform, probs, out)
+    dev = _same_device("sample_top_p", logits, temperature, top_p, uniform, probs, out)
     stride = _rows_of(logits, "sample_top_p: logits")
     rows, vocab = logits.shape
-    for t, name in ((temperature, "temperature"), (top_p, "top_p"), (uniform, "uniform")):
-        _f32_rows(t, rows, f"sample_top_p: {name}")
+    _f32_rows(temperature, rows, "sample_top_p: temperature")
+    _f32_rows(top_p, rows, "sample_top_p: top_p")
+    _f32_rows(uniform, rows, "sample_top_p: uniform")
     probs_stride = 0
     if probs is not None:
         probs_stride = _rows_of(probs, "sample_top_p: probs")
@@ -627,11 +665,12 @@ def sample_top_p(logits: torch.Tensor, temperature: torch.Tensor, top_p: torch.T
         out = torch.empty(rows, dtype=torch.int32, device=logits.device)
     elif out.dtype != torch.int32 or out.shape != (rows,) or not out.is_contiguous():
         raise ValueError(f"sample_top_p: out must be a contiguous int32 tensor [{rows}]")
-    with _device_of(logits):
-        _lib.check(_lib.lib.dsv_sample_top_p(
+    with _on(dev):
+        rc = _lib.lib.dsv_sample_top_p(
             logits.data_ptr(), stride, rows, vocab, temperature.data_ptr(), top_p.data_ptr(), uniform.data_ptr(),
-            out.data_ptr(), _lib.ptr(probs), probs_stride, _lib.dtype_code(logits.dtype),
-            _lib.current_stream_ptr(logits.device)))
+            out.data_ptr(), _lib.ptr(probs), probs_stride, _lib.dtype_code(logits.dtype), _raw_stream(dev))
+    if rc:
+        _lib.check(rc)
     _lib.LAUNCHES[0] += int(rows > 0)
     return out
 
@@ -647,7 +686,7 @@ def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, indptr: torch.Tenso
     without draft_probs, 1 at the draft. Returns int32 [batch] tensors (accepted drafts, next token); the next
     token is drawn from max(p - q, 0) of the first rejected row, or from p of the last row, with the uniform
     number of the request's last row. A request without rows gets (0, -1)."""
-    _same_device("verify_draft", logits, tokens, indptr, uniform, temperature, top_p, draft_probs)
+    dev = _same_device("verify_draft", logits, tokens, indptr, uniform, temperature, top_p, draft_probs)
     stride = _rows_of(logits, "verify_draft: logits")
     nnz, vocab = logits.shape
     batch = indptr.shape[0] - 1
@@ -661,13 +700,17 @@ def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, indptr: torch.Tenso
         draft_stride = _rows_of(draft_probs, "verify_draft: draft_probs")
         if draft_probs.dtype != torch.float32 or draft_probs.shape != logits.shape:
             raise ValueError(f"verify_draft: draft_probs must be float32 {tuple(logits.shape)}")
-    accepted, following = torch.empty((2, batch), dtype=torch.int32, device=logits.device).unbind(0)
-    workspace = torch.empty(nnz, dtype=torch.uint8, device=logits.device)
-    with _device_of(logits):
-        _lib.check(_lib.lib.dsv_verify_draft(
+    # one allocation: accepted, next tokens, and a byte per row of scratch
+    buf = torch.empty(2 * batch + (nnz + 3) // 4, dtype=torch.int32, device=logits.device)
+    accepted, following = buf[:batch], buf[batch : 2 * batch]
+    at = buf.data_ptr()
+    with _on(dev):
+        rc = _lib.lib.dsv_verify_draft(
             logits.data_ptr(), stride, nnz, vocab, _i32_dev(tokens, "tokens").data_ptr(),
             _i32_dev(indptr, "indptr").data_ptr(), batch, uniform.data_ptr(), temperature.data_ptr(), top_p.data_ptr(),
-            _lib.ptr(draft_probs), draft_stride, workspace.data_ptr(), nnz, accepted.data_ptr(), following.data_ptr(),
-            _lib.dtype_code(logits.dtype), _lib.current_stream_ptr(logits.device)))
+            _lib.ptr(draft_probs), draft_stride, at + 8 * batch, nnz, at, at + 4 * batch, _lib.dtype_code(logits.dtype),
+            _raw_stream(dev))
+    if rc:
+        _lib.check(rc)
     _lib.LAUNCHES[0] += int(nnz > 0) + 1 if batch > 0 else 0
     return accepted, following

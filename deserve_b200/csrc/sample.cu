@@ -322,6 +322,25 @@ struct Slice {
       u1 = u2;
     }
   }
+  // of(vector, its number): the 16-byte vectors themselves, neighbours' entries in the first and the last one included.
+  template <typename F>
+  __device__ __forceinline__ void each_raw(int a, int b, F of) const {
+    if (kShared) {
+      for (int i = a; i < b; i += 32) of(v[i], i);
+      return;
+    }
+    uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0, u2 = u0, u3 = u0;
+    if (a < b) u0 = ld_stream16(v + a);
+    if (a + 32 < b) u1 = ld_stream16(v + a + 32);
+    if (a + 64 < b) u2 = ld_stream16(v + a + 64);
+    for (int i = a; i < b; i += 32) {
+      if (i + 96 < b) u3 = ld_stream16(v + i + 96);
+      of(u0, i);
+      u0 = u1;
+      u1 = u2;
+      u2 = u3;
+    }
+  }
   // The same for the warp's 32 lanes together: of(values, first index) runs in all of them, with -inf behind the end.
   template <typename F>
   __device__ __forceinline__ void each_warp(int a, int b, F of) const {
@@ -753,9 +772,10 @@ __device__ __forceinline__ void hist_clear(Shared& sh) {
 }
 
 // First bin of the cluster's summed histogram whose inclusive running sum exceeds a limit, the sum before it and its own
-// mass; -1: none, `before` is the whole. Each CTA sums its share of the bins over the cluster. Slots s to s + 2.
-template <int NT>
-__device__ int hist_find(Shared& sh, int s, u64 limit, u64& before, u64& mass) {
+// mass; -1: none, `before` is the whole. Each CTA sums its share of the bins over the cluster; mass_of(bin, sum) makes a mass of a
+// bin's sum. Slots s to s + 2.
+template <int NT, typename F>
+__device__ int hist_find(Shared& sh, int s, u64 limit, u64& before, u64& mass, F mass_of) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = cluster_size(), rank = cluster_rank();
   constexpr int MAX = kBins / NT;
   const int bins = kBins / c, per = max(1, bins / NT);  // bins of this CTA, of a thread
@@ -779,6 +799,7 @@ __device__ int hist_find(Shared& sh, int s, u64 limit, u64& before, u64& mass) {
 #pragma unroll
         for (int r = 0; r < kMaxCtas; ++r) v[i] += ((u64)hi[r] << 32) + lo[r];
       }
+      v[i] = mass_of(b, v[i]);
     }
     mine += v[i];
   }
@@ -900,6 +921,79 @@ __device__ u64 locate(const Slice<T, NT, kShared>& sl, Shared& sh, int slot, u64
   return all;
 }
 
+// The border falls among `count` entries equal to `value`: the ones with the lowest indices are kept, as many as begin within the
+// limit. k.total comes with what ranks before them. Slots 14 and 15.
+template <typename T, int NT, bool kShared>
+__device__ void keep_ties(const Slice<T, NT, kShared>& sl, float value, u64 limit, u64 count, const RowScale& s, Kept& k, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
+  const u64 w = raw_weight(value, s, sh.table) - kRaw, n = limit / w + 1;
+  k.value = value;
+  k.total += n * w;
+  if (n >= count) {
+    k.index = kMaxVocab;
+    return;
+  }
+  if (threadIdx.x == 0) sh.tie = -1;
+  const u64 mine = sl.sum(sh, [&](const float (&f)[N], int) {
+    int x = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x += f[i] == value ? 1 : 0;
+    return (u64)x;
+  });
+  locate(sl, sh, 14, mine, [&](float l, int) { return l == value ? (u64)1 : 0; }, [&](u64) { return n - 1; }, &sh.tie);
+  __syncthreads();
+  if (threadIdx.x == 0) sh.slot[15].a = (u64)(sh.tie + 1);
+  cluster_sync();
+  k.index = (int)cluster_max(&sh.slot[15].a) - 1;
+}
+
+// Border of a row of 16-bit logits that lies behind the list: entries are counted by their very value, 2048 order keys (16 factors
+// of two in bf16, 2 in fp16) at a time, and a bin's mass is its count times one weight. Eight instructions per entry instead of the 45
+// of weighing each; the members of a bin are equal, so only their indices are left to look at. false: the border lies on a zero, whose
+// two signs are one value. Slots 3 to 8 in turn.
+template <typename T, int NT, bool kShared>
+__device__ bool count_border(const Slice<T, NT, kShared>& sl, const RowScale& s, u64 limit, Kept& k, Shared& sh) {
+  constexpr int N = Vec16<T>::N;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  k.total = 0;
+  int key0 = (int)order_key<T>(s.top);
+  for (int round = 0; key0 >= 0; ++round, key0 -= kBins) {
+    hist_clear<NT>(sh);
+    __syncthreads();
+    sl.each_raw(sl.begin(warp) + lane, sl.end(warp), [&](const uint4& u, int i) {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      const bool edge = i == 0 || i == sl.n_vec - 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t neg = (w[j] >> 15) & 0x00010001u;               // signs
+        const uint32_t key = w[j] ^ (neg * 0xffffu | 0x80008000u);     // order keys of both halves
+        const uint32_t a = (uint32_t)key0 - (key & 0xffffu), b = (uint32_t)key0 - (key >> 16);
+        bool in_a = a < (uint32_t)kBins, in_b = b < (uint32_t)kBins;
+        if (edge) {
+          const int at = i * N + 2 * j;
+          in_a = in_a && at >= sl.lead && at < sl.n_vec * N - sl.tail;
+          in_b = in_b && at + 1 >= sl.lead && at + 1 < sl.n_vec * N - sl.tail;
+        }
+        if (in_a) atomicAdd(&sh.hist_lo[a], 1u);
+        if (in_b) atomicAdd(&sh.hist_lo[b], 1u);
+      }
+    });
+    u64 before, mass;
+    const int bin = hist_find<NT>(sh, 3 + 3 * (round & 1), limit, before, mass,
+                                  [&](int b, u64 n) { return n ? n * (raw_weight(key_value<T>((uint32_t)(key0 - b)), s, sh.table) - kRaw) : 0; });
+    limit -= before;
+    k.total += before;
+    if (bin >= 0) {
+      const float value = key_value<T>((uint32_t)(key0 - bin));
+      if (value == 0.f) return false;
+      keep_ties(sl, value, limit, mass / (raw_weight(value, s, sh.table) - kRaw), s, k, sh);
+      return true;
+    }
+    cluster_sync();  // the slots of the round before last are free
+  }
+  return false;  // cannot happen with top_p < 1
+}
+
 // Top-p border of the row. `known`: the sum of its weights in units of the fixed-point weights, or -1. Without a cut and
 // with an unknown sum the masses of the subsegments are left in sh.seg (`mine`: the warp's). Slots 2 to 30.
 template <typename T, int NT, bool kShared>
@@ -971,8 +1065,15 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
   k.total = whole.b;
   u64 limit = (u64)((double)fmaxf(top_p, 0.f) * (double)whole.b), mass, kept = 0;
   near.usable = limit < whole.a && whole.c < 1ull << 40;
+  if constexpr (sizeof(T) == 2) {
+    if (!near.usable && sl.how == kAsIs && count_border(sl, s, limit, k, sh)) return k;
+    k.value = -INFINITY;
+    k.index = -1;
+    k.total = whole.b;
+  }
   int bin = -1, window = 0;
   if (!(near.usable && whole.c <= kList)) {
+    cluster_sync();
     // Histograms over windows of kWindow nats, the last one to where weights end. (The tail of a vocabulary is most of its
     // entries and seldom holds the border.)
     for (; bin < 0; ++window) {
@@ -1004,7 +1105,7 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
           marked(f, in, [&](float l, int) { count(l, raw_weight(l, s, sh.table) - kRaw); });
         });
       }
-      bin = hist_find<NT>(sh, 3 + 3 * window, limit, before, mass);
+      bin = hist_find<NT>(sh, 3 + 3 * window, limit, before, mass, [](int, u64 w) { return w; });
       limit -= before;
       kept += before;
     }
@@ -1085,23 +1186,9 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
     k.total = kept + sh.kept;
     return k;
   }
-  if ((lo >> kIndexBits) == (hi >> kIndexBits)) {  // many, but of one value (16-bit logits): the ones with the lowest indices
-    set_border<T>(k, lo);
-    const u64 w = raw_weight(k.value, s, sh.table) - kRaw, n = limit / w + 1;
-    k.total = kept + n * w;
-    if (threadIdx.x == 0) sh.tie = -1;
-    const float value = k.value;
-    const u64 count = sl.sum(sh, [&](const float (&f)[N], int) {
-      int x = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) x += f[i] == value ? 1 : 0;
-      return (u64)x;
-    });
-    locate(sl, sh, 14, count, [&](float l, int) { return l == value ? (u64)1 : 0; }, [&](u64) { return n - 1; }, &sh.tie);
-    __syncthreads();
-    if (threadIdx.x == 0) sh.slot[15].a = (u64)(sh.tie + 1);
-    cluster_sync();
-    k.index = (int)cluster_max(&sh.slot[15].a) - 1;
+  if ((lo >> kIndexBits) == (hi >> kIndexBits)) {  // many, but of one value (16-bit logits)
+    k.total = kept;
+    keep_ties(sl, key_value<T>((uint32_t)(lo >> kIndexBits)), limit, members, s, k, sh);
     return k;
   }
   for (int s0 = 16;; s0 += 3) {  // 50 bits of rank key, 11 a round: five rounds at most
@@ -1122,7 +1209,7 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
         if (key >= lo && key <= hi) hist_add(sh, (int)((hi - key) >> shift), raw_weight(l, s, sh.table) - kRaw);
       }
     });
-    bin = hist_find<NT>(sh, s0, limit, before, mass);
+    bin = hist_find<NT>(sh, s0, limit, before, mass, [](int, u64 w) { return w; });
     if (bin < 0) {  // cannot happen: the members' mass exceeds the limit
       k.total = kept + before;
       return k;

@@ -426,7 +426,7 @@ __device__ __forceinline__ Slice<T, NT, kShared> make_slice(const T* row, int vo
   sl.n_vec = n > 0 ? (sl.lead + n + N - 1) / N : 0;
   sl.tail = sl.n_vec * N - sl.lead - n;
   sl.seg = ((sl.n_vec + W * 32 - 1) / (W * 32)) * 32;
-  sl.sub = ((sl.seg + kSub * 32 - 1) / (kSub * 32)) * 32;
+  sl.sub = max(64, ((sl.seg + kSub * 32 - 1) / (kSub * 32)) * 32);
   sl.limit = vocab;
   sl.how = kAsIs;
   return sl;
@@ -504,7 +504,23 @@ __device__ int greedy_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float& t
 
 __device__ __forceinline__ double as_double(u64 v) { return __longlong_as_double((long long)v); }
 __device__ __forceinline__ u64 as_bits(double v) { return (u64)__double_as_longlong(v); }
-__device__ __forceinline__ double power(double n) { return exp2(fmax(n, -2000.0)); }  // of an integer; 0 far below
+// 2^n of an integer below 1024; 0 far below.
+__device__ __forceinline__ double power(double n) {
+  return n > -1022.0 ? __hiloint2double((1023 + (int)n) << 20, 0) : 0.0;
+}
+
+// 2^(l c / 64 - e) as the product of two doubles, magic = 1.5 * 2^52 - 64 e: raw_weight without the fixed point.
+__device__ __forceinline__ void double_weight(float l, double c, double magic, const double* __restrict__ table, double& scaled, double& series) {
+  const double x = (double)l, w = fma(x, c, magic), r = fma(x, c, magic - w);
+  constexpr double a = 0.010830424696249145;
+  double y = fma(r, a * a * a * a / 24.0, a * a * a / 6.0);
+  y = fma(r, y, a * a / 2.0);
+  y = fma(r, y, a);
+  series = fma(r, y, 1.0);
+  const int n = __double2loint(w);
+  const double p = table[n & (kTable - 1)];
+  scaled = __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));  // the weight is scaled * series
+}
 
 // Sum of the row's weights in double, and its top, from the first walk. Every warp measures against a power of two of its
 // own, 2^E near its first entries' maximum (a double's range leaves 600 factors of two to both sides), so nothing has to be known
@@ -519,12 +535,13 @@ struct Walk {
 };
 constexpr double kReach = 600.0;
 
-// Joins (mass, power) over the lanes below n: the larger power, the running sums in it.
+// Joins (mass, power) over the warp: the largest power, the masses and their running sums in it. Powers are integers, or (kReal) not.
+template <bool kReal = false>
 __device__ __forceinline__ void join(double& mass, double& e, double& inc, int lane) {
   double g = e;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) g = fmax(g, __shfl_xor_sync(0xffffffffu, g, o));
-  mass = g > -INFINITY && e > -INFINITY ? mass * power(e - g) : 0.0;
+  mass = g > -INFINITY && e > -INFINITY ? mass * (kReal ? (double)exp2f((float)(e - g)) : power(e - g)) : 0.0;
   e = g;
   inc = mass;
 #pragma unroll
@@ -545,15 +562,18 @@ __device__ Walk weight_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float t
   if (threadIdx.x == 0) sh.n_list = 0;
   __syncthreads();
   float top = -INFINITY, cutoff = 0.f;
-  double e = -INFINITY, magic = 0.0, mass = 0.0, part = 0.0;
+  double e = -INFINITY, magic = 0.0, mass = 0.0, part = 0.0, odd = 0.0;
   bool far = false;
   int sub = 0, next = sl.begin(warp) + sl.sub;
+  if (lane < kSub) sh.seg[warp * kSub + lane] = 0;
+  __syncwarp();
   auto close = [&]() {  // end of a subsegment
+    part += odd;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
     if (lane == 0) sh.seg[warp * kSub + sub] = as_bits(part);
     mass += part;
-    part = 0.0;
+    part = odd = 0.0;
     ++sub;
   };
   first_walk(sl, buf, [&](const float (&f)[N], int, int at) {
@@ -577,21 +597,15 @@ __device__ Walk weight_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float t
     }
     if (e > -INFINITY && !far) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {  // as in raw_weight, summed as a double
-        const double x = (double)fmaxf(f[i], cutoff);
-        const double w = fma(x, c, magic), r = fma(x, c, magic - w);
-        constexpr double a = 0.010830424696249145;
-        double y = fma(r, a * a * a * a / 24.0, a * a * a / 6.0);
-        y = fma(r, y, a * a / 2.0);
-        y = fma(r, y, a);
-        y = fma(r, y, 1.0);
-        const int n = __double2loint(w);
-        const double p = sh.table[n & (kTable - 1)];
-        part = fma(__hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p)), y, part);
+      for (int i = 0; i < N; ++i) {
+        double scaled, series;
+        double_weight(fmaxf(f[i], cutoff), c, magic, sh.table, scaled, series);
+        if (i & 1) odd = fma(scaled, series, odd);
+        else part = fma(scaled, series, part);
       }
     }
   });
-  while (sub < kSub) close();
+  close();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   // An entry more than kReach above the warp's first ones makes the sum meaningless (it may have wrapped an exponent).
@@ -690,9 +704,9 @@ __device__ void draw_all(const Slice<T, NT, kShared>& sl, const Walk& walk, floa
     for (int i = 0; i < N; ++i) {
       m[i] = 0.0;
       if (f[i] >= lowest) {
-        const double x = (double)f[i], y = fma(x, c, magic), r = fma(x, c, magic - y);
-        const int n = __double2loint(y);
-        m[i] = sh.table[n & (kTable - 1)] * exp2(r * 0.015625) * power((double)(n >> 6));
+        double scaled, series;
+        double_weight(f[i], c, magic, sh.table, scaled, series);
+        m[i] = scaled * series;
         mine = sl.first + v * N + i;
       }
       total += m[i];
@@ -921,6 +935,36 @@ __device__ u64 locate(const Slice<T, NT, kShared>& sl, Shared& sh, int slot, u64
   return all;
 }
 
+// The border among the entries that the CTAs' lists hold (kList at most, behind a cluster barrier): every CTA fetches them all, a thread
+// weighs what ranks before its entry.
+template <typename T>
+__device__ void rank_members(u64 limit, u64 kept, const RowScale& s, Kept& k, Shared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = cluster_size();
+  const int mine = lane < c ? (int)ld_remote32(remote(&sh.n_list, lane)) : 0;
+  const int upto = (int)warp_scan((u64)mine, lane), members = __shfl_sync(0xffffffffu, upto, 31);
+  if (warp < c) {  // warp r fetches CTA r's
+    const int n = __shfl_sync(0xffffffffu, mine, warp), first = __shfl_sync(0xffffffffu, upto, warp) - n;
+    for (int i = lane; i < n; i += 32) {
+      const u64 key = ld_remote64(remote(&sh.list[i], warp));
+      sh.all_key[first + i] = key;
+      sh.all_w[first + i] = raw_weight(key_value<T>((uint32_t)(key >> kIndexBits)), s, sh.table) - kRaw;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < members; i += blockDim.x) {
+    const u64 key = sh.all_key[i];
+    u64 above = 0;
+    for (int j = 0; j < members; ++j) above += sh.all_key[j] > key ? sh.all_w[j] : 0;
+    if (above <= limit && above + sh.all_w[i] > limit) {  // the last kept one
+      sh.border = key;
+      sh.kept = above + sh.all_w[i];
+    }
+  }
+  __syncthreads();
+  set_border<T>(k, sh.border);
+  k.total = kept + sh.kept;
+}
+
 // The border falls among `count` entries equal to `value`: the ones with the lowest indices are kept, as many as begin within the
 // limit. k.total comes with what ranks before them. Slots 14 and 15.
 template <typename T, int NT, bool kShared>
@@ -1060,6 +1104,11 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
     }
   });
   if (lane == 0) sh.near_n[warp] = near.n;
+  int put = 0;  // the cluster's entries, should they be few
+  if (lane == 0 && near.n > 0) put = atomicAdd(&sh.n_list, near.n);
+  put = __shfl_sync(0xffffffffu, put, 0);
+  for (int i = lane; i < min(near.n, near.cap); i += 32)
+    if (put + i < kList) sh.list[put + i] = rank_key<T>(list[i].l, list[i].i);
   Slot whole = cluster_total<NT>(warp_sum(sum), warp_sum(whole_mass), (u64)near.n + (near.n > near.cap ? 1ull << 40 : 0), sh, 2, before);
   if (known >= 0.0) whole.b = (u64)known;
   k.total = whole.b;
@@ -1110,14 +1159,19 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
       kept += before;
     }
   }
-  // Members of the border's bin (all that are near, where those are few): listed, and the range of their rank keys. In the row
-  // the values around the bin are found by two comparisons, with room for the rounding of the bin's arithmetic, the members
-  // among them by their bin.
+  if (near.usable && whole.c <= kList) {  // few: every CTA ranks all of them
+    rank_members<T>(limit, kept, s, k, sh);
+    return k;
+  }
+  // Members of the border's bin: listed, and the range of their rank keys. In the row the values around the bin are found by two
+  // comparisons, with room for the rounding of the bin's arithmetic, the members among them by their bin.
+  if (threadIdx.x == 0) sh.n_list = 0;
+  __syncthreads();
   const float width = 1.f / scale, slack = 1e-6f * (fabsf(base) + (float)(bin + 1) * width);
   const float v_hi = base - (float)bin * width + slack, v_lo = bin == kBins - 1 ? to : base - (float)(bin + 1) * width - slack;
   u64 lo = ~0ull, hi = 0;
   auto member = [&](float l, int i) {
-    if (bin >= 0 && min((int)((base - l) * scale), kBins - 1) != bin) return;
+    if (min((int)((base - l) * scale), kBins - 1) != bin) return;
     const u64 key = rank_key<T>(l, i);
     lo = min(lo, key);
     hi = max(hi, key);
@@ -1162,28 +1216,8 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
   hi = cluster_max(&sh.slot[12].b);
   const int c = cluster_size();
   const int members = (int)cluster_sum(&sh.slot[13].a, c);
-  if (members <= kList) {  // few: every CTA ranks all of them
-    if (warp < c) {  // warp r fetches CTA r's
-      const int n = (int)ld_remote64(remote(&sh.slot[13].a, warp)), first = (int)cluster_sum(&sh.slot[13].a, warp);
-      for (int i = lane; i < n; i += 32) {
-        const u64 key = ld_remote64(remote(&sh.list[i], warp));
-        sh.all_key[first + i] = key;
-        sh.all_w[first + i] = raw_weight(key_value<T>((uint32_t)(key >> kIndexBits)), s, sh.table) - kRaw;
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < members; i += NT) {
-      const u64 key = sh.all_key[i];
-      u64 above = 0;
-      for (int j = 0; j < members; ++j) above += sh.all_key[j] > key ? sh.all_w[j] : 0;
-      if (above <= limit && above + sh.all_w[i] > limit) {  // the last kept one
-        sh.border = key;
-        sh.kept = above + sh.all_w[i];
-      }
-    }
-    __syncthreads();
-    set_border<T>(k, sh.border);
-    k.total = kept + sh.kept;
+  if (members <= kList) {
+    rank_members<T>(limit, kept, s, k, sh);
     return k;
   }
   if ((lo >> kIndexBits) == (hi >> kIndexBits)) {  // many, but of one value (16-bit logits)
@@ -1335,16 +1369,10 @@ __device__ bool draw_rest(const Slice<T, NT, kShared>& sl, const Walk& walk, flo
       }
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {  // as in weight_walk
-      const double x = (double)fmaxf(f[i], lowest), w = fma(x, c, magic), r = fma(x, c, magic - w);
-      constexpr double a = 0.010830424696249145;
-      double y = fma(r, a * a * a * a / 24.0, a * a * a / 6.0);
-      y = fma(r, y, a * a / 2.0);
-      y = fma(r, y, a);
-      y = fma(r, y, 1.0);
-      const int n = __double2loint(w);
-      const double p = sh.table[n & (kTable - 1)];
-      y = fma(__hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p)) * y, inv, -(double)d[i]);
+    for (int i = 0; i < N; ++i) {
+      double scaled, series;
+      double_weight(fmaxf(f[i], lowest), c, magic, sh.table, scaled, series);
+      const double y = fma(scaled * series, inv, -(double)d[i]);
       m[i] = f[i] >= lowest && y > 0.0 ? y : 0.0;
     }
   };
@@ -1577,10 +1605,10 @@ __device__ int quick_walk(const Slice<T, NT, false>& sl, float temperature, floa
     own = e = in ? as_double(sh.warp_b[lane]) : -INFINITY;
     best = in ? __uint_as_float((uint32_t)sh.warp_c[lane]) : -INFINITY;
     far = __any_sync(0xffffffffu, in && (sh.warp_c[lane] >> 32) != 0);
-    join(sum_all, e, inc, lane);
+    join<true>(sum_all, e, inc, lane);
     const double whole = __shfl_sync(0xffffffffu, inc, 31);
     double g = own;
-    join(sum_above, g, inc, lane);
+    join<true>(sum_above, g, inc, lane);
     const double ahead = __shfl_sync(0xffffffffu, inc, 31);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -1597,16 +1625,16 @@ __device__ int quick_walk(const Slice<T, NT, false>& sl, float temperature, floa
   own = e = in ? as_double(ld_remote64(remote(&sh.slot[0].b, lane))) : -INFINITY;
   const u64 z = in ? ld_remote64(remote(&sh.slot[0].c, lane)) : (u64)__float_as_uint(-INFINITY);
   sum_above = in ? as_double(ld_remote64(remote(&sh.slot[1].a, lane))) : 0.0;
-  join(sum_all, e, inc, lane);
+  join<true>(sum_all, e, inc, lane);
   const double total = __shfl_sync(0xffffffffu, inc, 31);
   double g = own;
-  join(sum_above, g, inc, lane);
+  join<true>(sum_above, g, inc, lane);
   const double ahead = __shfl_sync(0xffffffffu, inc, 31);
   best = __uint_as_float((uint32_t)z);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (__any_sync(0xffffffffu, (z >> 32) != 0) || best == INFINITY || best < -1e38f) return -1;
-  const double wx = power((double)lx * c - e);
+  const double wx = exp2(fmax((double)lx * c - e, -2000.0));
   double least = total, most = total;  // bounds of Z
   if (cut) {
     least = total * fmax((double)top_p, 0.0);

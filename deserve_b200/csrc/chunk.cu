@@ -21,16 +21,17 @@ constexpr int32_t kChunkMagic = 0x44534331;  // "DSC1"
 // header: magic, items, merge rows, q tokens per tile, batch, offset of the items, offset of the merge
 // rows, q heads, kv heads, head_dim, partial rows, page size, dtype, nnz, kernel, most parts of a tile
 constexpr int kPlanHeader = 16;
-constexpr int kItemInts = 8;  // request, first q token, q tokens, first page, end page, partial row or -1, 2 unused
+// request, first q token, q tokens, first page | end page, partial row or -1, first q row, first entry of the page list |
+// pages of the request, first q token behind which the request's tokens lie (n_new - q0), 2 unused: all that a CTA needs but the last
+// page's length, so that it begins after two dependent loads instead of four
+constexpr int kItemInts = 12;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct ChunkParams {
   const void* q;
   const void* pages;
-  const int32_t* qo_indptr;
   const int32_t* kv_indices;
-  const int32_t* kv_indptr;
   const int32_t* kv_last_page_len;
   void* out;
   float* lse;
@@ -55,23 +56,19 @@ struct Item {
 };
 
 __device__ __forceinline__ bool load_item(const ChunkParams& p, int index, Item& it) {
-  const int32_t* raw = p.items + (int64_t)index * kItemInts;
-  const int4 a = __ldg(reinterpret_cast<const int4*>(raw));
-  const int2 b = __ldg(reinterpret_cast<const int2*>(raw + 4));
-  const int req = a.x, q0 = a.y, nq = a.z, pb = a.w, pe = b.x;
-  const int q_begin = __ldg(p.qo_indptr + req), n_new = __ldg(p.qo_indptr + req + 1) - q_begin;
-  const int ip0 = __ldg(p.kv_indptr + req), n_pages = __ldg(p.kv_indptr + req + 1) - ip0;
-  if (q0 < 0 || nq < 1 || q0 + nq > n_new || q_begin < 0 || q_begin + n_new > p.nnz || pb < 0 || pe > n_pages || pb > pe)
-    return false;
+  const int4* raw = reinterpret_cast<const int4*>(p.items + (int64_t)index * kItemInts);
+  const int4 a = __ldg(raw), b = __ldg(raw + 1), c = __ldg(raw + 2);
+  const int req = a.x, nq = a.z, pb = a.w, pe = b.x, n_pages = c.x, left = c.y;
+  if (nq < 1 || nq > left || b.z < 0 || b.z + nq > p.nnz || pb < 0 || pe > n_pages || pb > pe) return false;
   const int kv_len = n_pages > 0 ? (n_pages - 1) * p.page_size + __ldg(p.kv_last_page_len + req) : 0;
-  it.q_row0 = q_begin + q0;
+  it.q_row0 = b.z;
   it.nq = nq;
   it.n_rows = nq * (p.n_q_heads / p.n_kv_heads);
-  it.ip0 = ip0;
-  it.limit0 = kv_len - n_new + q0;
+  it.ip0 = b.w;
+  it.limit0 = kv_len - left;
   it.tok_begin = pb * p.page_size;
   // what lies behind the last token's limit is not needed by any row of the tile
-  it.tok_end = max(it.tok_begin, min(min(pe * p.page_size, kv_len), it.limit0 + nq));
+  it.tok_end = max(it.tok_begin, min(pe * p.page_size, it.limit0 + nq));
   it.slot = b.y;
   return true;
 }
@@ -517,7 +514,12 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
   for (int64_t k = 0; k < n_items; ++k) {
     int32_t* it = plan_host + kPlanHeader + kItemInts * k;
     for (int j = 0; j < 6; ++j) it[j] = items[k].v[j];
-    it[6] = it[7] = 0;
+    const int req = it[0], q0 = it[1];
+    it[6] = qo_indptr_host[req] + q0;
+    it[7] = kv_indptr_host[req];
+    it[8] = kv_indptr_host[req + 1] - kv_indptr_host[req];
+    it[9] = qo_indptr_host[req + 1] - qo_indptr_host[req] - q0;
+    it[10] = it[11] = 0;
   }
   return DSV_OK;
 }
@@ -560,7 +562,7 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
     return fail(DSV_E_WORKSPACE, "chunk: workspace needs %lld bytes, got %lld", (long long)ws_need, (long long)workspace_bytes);
   DSV_REQUIRE(ws_need == 0 || aligned16(workspace), "chunk: workspace must be 16-byte aligned");
   ChunkParams p;
-  p.q = q; p.pages = pages_layer; p.qo_indptr = qo_indptr; p.kv_indices = kv_indices; p.kv_indptr = kv_indptr;
+  p.q = q; p.pages = pages_layer; p.kv_indices = kv_indices;
   p.kv_last_page_len = kv_last_page_len; p.out = out; p.lse = lse; p.items = plan_dev + plan_host[5];
   DSV_REQUIRE(aligned16(p.items) && aligned16(plan_dev + plan_host[6]), "chunk: device plan must be 16-byte aligned");
   p.part_o = static_cast<float*>(workspace);

@@ -58,6 +58,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
   const int kv_head = blockIdx.x % p.n_kv_heads;  // the kv heads of an item are adjacent CTAs
   const int ps = 1 << ps_log, bt = min(ps, 16), n_boxes = kBN / bt;
 
+  if (warp == 9 && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];\n prefetch.tensormap [%1];\n prefetch.tensormap [%2];\n" ::"l"(&q_map), "l"(&k_map), "l"(&v_map));
+  }
   Item it;
   if (!load_item(p, blockIdx.x / p.n_kv_heads, it) || it.nq > 2 * tq) {
     if (tid == 0) record_status(p.status, ST_BAD_PLAN);

@@ -416,7 +416,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
 
 def chunk_plan_capacity(nnz: int, batch: int, sm_count: int = 148) -> int:
     """int32 entries that a chunk plan for `nnz` new tokens of `batch` requests can need."""
-    return 16 + 8 * (4 * sm_count + 2 * (nnz + batch)) + 4 * nnz
+    return 16 + 12 * (4 * sm_count + 2 * (nnz + batch)) + 4 * nnz
 
 
 def make_chunk_plan(qo_indptr_host: np.ndarray, kv_indptr_host: np.ndarray, n_q_heads: int, n_kv_heads: int,

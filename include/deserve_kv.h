@@ -269,7 +269,7 @@ int dsv_paged_prefill(const void* q, int64_t q_stride_tok, const int32_t* qo_ind
  * Host-side planning of attention of a few new tokens per request over the paged cache
  * (dsv_paged_chunk_attention). Reads qo_indptr_host[batch+1] and kv_indptr_host[batch+1]
  * (HOST memory), cuts every request into q tiles and the page list of a tile into parts
- * so that the whole GPU streams K/V, and writes the int32 plan (opaque: a header, eight
+ * so that the whole GPU streams K/V, and writes the int32 plan (opaque: a header, twelve
  * integers per item, four per q row whose tile was split) with its size and the bytes of
  * device workspace that the partial states need. Pure host arithmetic. sm_count <= 0
  * means 148. One plan serves all layers of a step.

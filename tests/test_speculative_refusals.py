@@ -29,15 +29,16 @@ def _plan(new, pages, hq=32, hkv=8, d=128, ps=16, dtype=torch.bfloat16, sms=148)
 def test_chunk_plan_covers_every_row_and_page_once(dtype, hq, hkv, d, ps, new, pages):
     plan, ws, qo = _plan(new, pages, hq, hkv, d, ps, dtype)
     n_items, n_merge, tile, batch, parts_total = plan[1], plan[2], plan[3], plan[4], plan[10]
-    assert batch == len(new) and plan[5] == 16 and plan[6] == 16 + 8 * n_items and len(plan) == plan[6] + 4 * n_merge
+    assert batch == len(new) and plan[5] == 16 and plan[6] == 16 + 12 * n_items and len(plan) == plan[6] + 4 * n_merge
     assert ws == parts_total * hq * (d + 2) * 4 and plan[13] == qo[-1]
-    items = plan[16: 16 + 8 * n_items].reshape(-1, 8)
+    items = plan[16: 16 + 12 * n_items].reshape(-1, 12)
     merge = {int(m[0]): m[1:].tolist() for m in plan[plan[6]:].reshape(-1, 4)}
     assert len(merge) == n_merge
     cover = [np.zeros((n, p), dtype=int) for n, p in zip(new, pages)]
     rows = [np.zeros(n, dtype=int) for n in new]
     part = np.zeros(parts_total, dtype=int)
-    for req, q0, nq, pb, pe, slot, *_ in items:
+    for req, q0, nq, pb, pe, slot, row, first, n_pages, left, *_ in items:
+        assert row == qo[req] + q0 and left == new[req] - q0 and n_pages == pages[req] and first == sum(pages[:req])
         assert 0 <= q0 and 1 <= nq <= tile and q0 + nq <= new[req] and 0 <= pb <= pe <= pages[req]
         cover[req][q0: q0 + nq, pb:pe] += 1
         rows[req][q0: q0 + nq] += 1

@@ -1,12 +1,14 @@
-// Chunk attention for 16-bit K/V on the tensor cores (mma.sync), K/V staged by TMA.
+// Chunk attention for 16-bit K/V and at most 16 rows ((token, q head) pairs of a kv head) per item, on the
+// tensor cores (mma.sync), K/V staged by TMA.
 //
 // A CTA owns one item of the plan for `hb` kv heads: 8 consumer warps and a producer warp, 1 CTA per SM,
 // a 3-deep ring of 512 * D bytes per stage (128 (head, token) rows of K and of V). The warps are split over
-// heads first, then over the item's 16-row blocks (rw of them), then over 16-token groups of a stage (ts):
-// hb * rw * ts = 8. A K/V tile is read from HBM once for all rows; each row block reads it from shared
-// memory again, which costs rw * 23 bytes per clock and SM at full HBM speed, of 128 available.
-// Per 16 tokens and 16 rows: S = Q K^T as 16 mma.sync.m16n8k16, causal / length mask where a row's limit
-// falls into the group, online softmax on the fragments, O += P V as 16 more.
+// heads first, then over the 16-token groups of a stage (ts): hb * ts = 8; the ts warps of a head merge at the end.
+// Per 16 tokens: S = Q K^T as mma.sync.m16n8k16, causal / length mask where a row's limit falls into the group,
+// online softmax on the fragments, O += P V. One 16-row MMA tile covers all rows, so the arithmetic is a few
+// percent of the time that the tile's bytes take. With 17 rows and more it would read its tile from shared
+// memory once per 16 rows: those go to the tcgen05 kernel.
+// Two requests of about 100 kv tokens, 2-4 of them new, 8 q / 2 kv heads of 64: 6.5 us, the latency of one launch and one ring fill.
 #pragma once
 
 #include <cuda.h>
@@ -140,22 +142,18 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
   const int kv_group = blockIdx.x % n_groups;                 // the kv heads of an item are adjacent CTAs
 
   Item it;
-  if (!load_item(p, blockIdx.x / n_groups, it)) {
+  if (!load_item(p, blockIdx.x / n_groups, it) || it.n_rows > 16) {
     if (tid == 0) record_status(p.status, ST_BAD_PLAN);
     return;
   }
   const int n_tiles = (it.tok_end - it.tok_begin + ttok - 1) / ttok;
-  // The item's own row blocks (a request with one new token needs one, whatever the plan's tile holds):
-  // the warps that are left over split the 16-token groups of a stage. A warp has rw groups per stage.
-  const int live_blocks = (it.n_rows + 15) >> 4;
-  const int rw_log = live_blocks <= 1 ? 0 : live_blocks <= 2 ? 1 : live_blocks <= 4 ? 2 : 3;
-  const int rw = 1 << rw_log, ts = kConsumerWarps >> (hb_log + rw_log);
+  const int ts = ng;  // warps of a kv head: one 16-token group of a stage each
 
   if (tid == 0) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1);
-      mbar_init(bar_empty + 8 * s, live_blocks * hb * ts);  // warps without a live row take no part
+      mbar_init(bar_empty + 8 * s, kConsumerWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -195,15 +193,14 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
 
   // ============================ consumer warps ===========================================
   const int g = lane >> 2, tg = lane & 3;
-  const int head_local = warp & (hb - 1), block = (warp >> hb_log) & (rw - 1), sub = warp >> (hb_log + rw_log);
+  const int head_local = warp & (hb - 1), sub = warp >> hb_log;
   const int kv_head = kv_group * hb + head_local;
-  const int r0 = block * 16 + g, r1 = r0 + 8;  // this lane's rows
+  const int r0 = g, r1 = r0 + 8;  // this lane's rows
   const int t_r0 = r0 / G, t_r1 = r1 / G;
   // last kv position that a row sees in this part; -1 for rows that are not there
   const int lim0 = r0 < it.n_rows ? min(it.limit0 + t_r0, it.tok_end - 1) : -1;
   const int lim1 = r1 < it.n_rows ? min(it.limit0 + t_r1, it.tok_end - 1) : -1;
-  const int lim_first = min(it.limit0 + (block * 16) / G, it.tok_end - 1);  // smallest limit of the block's live rows
-  const int lim_last = min(it.limit0 + min(block * 16 + 15, it.n_rows - 1) / G, it.tok_end - 1);
+  const int lim_first = min(it.limit0, it.tok_end - 1);  // smallest limit of the live rows; the largest is tok_end - 1
 
   uint32_t qa[KSTEPS][4];
   {
@@ -244,50 +241,44 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
     v_off[dh] = HALF + vr * 128 + ((v_cx ^ (vr & 7)) << 4);
   }
 
-  // One step: NG groups of 16 tokens (32 where a warp has more than one group: four independent chains
-  // of S products, one maximum and one rescale test for all).
-  auto step = [&](auto ng_tag, const int stage, const int grp, const int wt0) {
-    constexpr int NG = decltype(ng_tag)::value;
+  // One step: a group of 16 tokens.
+  auto step = [&](const int stage, const int grp, const int wt0) {
     const uint32_t kbase = smem_base + stage * STAGE + (uint32_t)(grp * bpg * box_bytes);
     const uint32_t vbase = kbase + HALF;
-    const uint32_t group_bytes = (uint32_t)(bpg * box_bytes);
-    const bool masked = wt0 + 16 * NG - 1 > lim_first;
+    const bool masked = wt0 + 15 > lim_first;
     bool poisoned = false;  // V of a token that some row does not see is not a number
     if (masked) {
       unsigned char* vg = smem + (vbase - smem_base);
       const int live = it.tok_end - wt0;
-      if (live < 16 * NG) {
+      if (live < 16) {
         // whole boxes were brought (or none): tokens past the end hold whatever was there. Clear them in V so
         // that 0 * garbage cannot produce a NaN (every warp that reads them writes the same zeros).
-        for (int x = lane; x < (16 * NG - live) * DH * 8; x += 32) {
+        for (int x = lane; x < (16 - live) * DH * 8; x += 32) {
           const int ch = x & 7, dh = (x >> 3) % DH, tl = live + (x >> 3) / DH;
-          *reinterpret_cast<uint4*>(vg + (tl >> 4) * group_bytes + row_of(tl & 15, dh) * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(vg + row_of(tl, dh) * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
       }
-      for (int x = lane; x < 16 * NG * DH * 8; x += 32) {
+      for (int x = lane; x < 16 * DH * 8; x += 32) {
         const int ch = x & 7, dh = (x >> 3) % DH, tl = (x >> 3) / DH;
-        const uint4 v = *reinterpret_cast<const uint4*>(vg + (tl >> 4) * group_bytes + row_of(tl & 15, dh) * 128 + ch * 16);
+        const uint4 v = *reinterpret_cast<const uint4*>(vg + row_of(tl, dh) * 128 + ch * 16);
         poisoned |= (not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w)) != 0;
       }
       poisoned = __any_sync(0xffffffffu, poisoned);
     }
-    float s[2 * NG][4];  // [8-token column block][row g: 2 tokens, row g + 8: 2 tokens]
+    float s[2][4];  // [8-token column block][row g: 2 tokens, row g + 8: 2 tokens]
 #pragma unroll
-    for (int i = 0; i < 2 * NG; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < KSTEPS; ++kk) {
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        uint32_t b[4];
-        ldmatrix_x4(b, (kbase + i * group_bytes + k_off[kk >> 2]) ^ ((kk & 3) << 5));
-        mma16816<T>(s[2 * i], qa[kk], b[0], b[1]);
-        mma16816<T>(s[2 * i + 1], qa[kk], b[2], b[3]);
-      }
+      uint32_t b[4];
+      ldmatrix_x4(b, (kbase + k_off[kk >> 2]) ^ ((kk & 3) << 5));
+      mma16816<T>(s[0], qa[kk], b[0], b[1]);
+      mma16816<T>(s[1], qa[kk], b[2], b[3]);
     }
     if (masked) {
 #pragma unroll
-      for (int i = 0; i < 2 * NG; ++i) {
+      for (int i = 0; i < 2; ++i) {
         const int c = wt0 + 8 * i + 2 * tg;
         if (c > lim0) s[i][0] = -INFINITY;
         if (c + 1 > lim0) s[i][1] = -INFINITY;
@@ -297,7 +288,7 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
     }
     float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 2 * NG; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mx0 = fmaxf(mx0, fmaxf(s[i][0], s[i][1]));
       mx1 = fmaxf(mx1, fmaxf(s[i][2], s[i][3]));
     }
@@ -320,55 +311,49 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
     }
     const float off0 = m0 == -INFINITY ? 0.f : -m0, off1 = m1 == -INFINITY ? 0.f : -m1;
     // P is rounded to the 16-bit type of V, as the tensor core needs it; the sum l is not
-    uint32_t pa[NG][4];
+    uint32_t pa[4];
 #pragma unroll
-    for (int i = 0; i < 2 * NG; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const float a = ex2(fmaf(s[i][0], sc, off0)), b = ex2(fmaf(s[i][1], sc, off0));
       const float c = ex2(fmaf(s[i][2], sc, off1)), d = ex2(fmaf(s[i][3], sc, off1));
       l0 += a + b;
       l1 += c + d;
-      pa[i >> 1][(i & 1) * 2] = pack2<T>(a, b);
-      pa[i >> 1][(i & 1) * 2 + 1] = pack2<T>(c, d);
+      pa[i * 2] = pack2<T>(a, b);
+      pa[i * 2 + 1] = pack2<T>(c, d);
     }
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
+    for (int jn = 0; jn < D / 16; ++jn) {
+      uint32_t v[4];
+      ldmatrix_x4_trans(v, (kbase + v_off[jn >> 2]) ^ ((jn & 3) << 5));
+      if (poisoned) {  // a zero weight must not meet an infinity: such values are added below
 #pragma unroll
-      for (int jn = 0; jn < D / 16; ++jn) {
-        uint32_t v[4];
-        ldmatrix_x4_trans(v, (kbase + i * group_bytes + v_off[jn >> 2]) ^ ((jn & 3) << 5));
-        if (poisoned) {  // a zero weight must not meet an infinity: such values are added below
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] &= ~not_finite<T>(v[k]);
-        }
-        mma16816<T>(o[2 * jn], pa[i], v[0], v[1]);
-        mma16816<T>(o[2 * jn + 1], pa[i], v[2], v[3]);
+        for (int k = 0; k < 4; ++k) v[k] &= ~not_finite<T>(v[k]);
       }
+      mma16816<T>(o[2 * jn], pa, v[0], v[1]);
+      mma16816<T>(o[2 * jn + 1], pa, v[2], v[3]);
     }
     if (poisoned) {  // the rest, token by token, only into the rows that see it
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
 #pragma unroll 1
-        for (int tl = 0; tl < 16; ++tl) {
-          const int from = g * 4 + ((tl & 7) >> 1);
-          const float2 w0 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[i][0] : pa[i][2], from));
-          const float2 w1 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[i][1] : pa[i][3], from));
-          const float a = (tl & 1) ? w0.y : w0.x, b = (tl & 1) ? w1.y : w1.x;
-          const bool see0 = wt0 + 16 * i + tl <= lim0, see1 = wt0 + 16 * i + tl <= lim1;
+      for (int tl = 0; tl < 16; ++tl) {
+        const int from = g * 4 + ((tl & 7) >> 1);
+        const float2 w0 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[0] : pa[2], from));
+        const float2 w1 = unpack2<T>(__shfl_sync(0xffffffffu, tl < 8 ? pa[1] : pa[3], from));
+        const float a = (tl & 1) ? w0.y : w0.x, b = (tl & 1) ? w1.y : w1.x;
+        const bool see0 = wt0 + tl <= lim0, see1 = wt0 + tl <= lim1;
 #pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            const int d = j * 8 + tg * 2, row = row_of(tl, d >> 6);
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + (vbase - smem_base) + i * group_bytes + row * 128 +
-                                                                  ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2);
-            const uint32_t odd = not_finite<T>(w);
-            const float2 v = unpack2<T>(w);
-            if (odd & 0xffffu) {
-              if (see0) o[j][0] = fmaf(a, v.x, o[j][0]);
-              if (see1) o[j][2] = fmaf(b, v.x, o[j][2]);
-            }
-            if (odd >> 16) {
-              if (see0) o[j][1] = fmaf(a, v.y, o[j][1]);
-              if (see1) o[j][3] = fmaf(b, v.y, o[j][3]);
-            }
+        for (int j = 0; j < D / 8; ++j) {
+          const int d = j * 8 + tg * 2, row = row_of(tl, d >> 6);
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + (vbase - smem_base) + row * 128 +
+                                                                ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2);
+          const uint32_t odd = not_finite<T>(w);
+          const float2 v = unpack2<T>(w);
+          if (odd & 0xffffu) {
+            if (see0) o[j][0] = fmaf(a, v.x, o[j][0]);
+            if (see1) o[j][2] = fmaf(b, v.x, o[j][2]);
+          }
+          if (odd >> 16) {
+            if (see0) o[j][1] = fmaf(a, v.y, o[j][1]);
+            if (see1) o[j][3] = fmaf(b, v.y, o[j][3]);
           }
         }
       }
@@ -376,24 +361,16 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
   };
 
   bool ok = true;
-  if (block < live_blocks) {
-    for (int tile = 0; tile < n_tiles; ++tile) {
-      const int s = tile % kStages;
-      if (!mbar_wait(bar_full + 8 * s, (tile / kStages) & 1, p.status)) {
-        ok = false;
-        break;
-      }
-      // this warp's groups of the stage: [sub * rw, sub * rw + rw); nothing behind lim_last is seen by its rows
-      const int t0 = it.tok_begin + tile * ttok + 16 * (sub << rw_log);
-      if (rw == 1) {
-        if (t0 <= lim_last) step(std::integral_constant<int, 1>{}, s, sub, t0);
-      } else {
-        for (int i = 0; i < rw && t0 + 16 * i <= lim_last; i += 2)
-          step(std::integral_constant<int, 2>{}, s, (sub << rw_log) + i, t0 + 16 * i);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_empty + 8 * s);  // this warp is done with the stage
+  for (int tile = 0; tile < n_tiles; ++tile) {
+    const int s = tile % kStages;
+    if (!mbar_wait(bar_full + 8 * s, (tile / kStages) & 1, p.status)) {
+      ok = false;
+      break;
     }
+    const int t0 = it.tok_begin + tile * ttok + 16 * sub;  // this warp's group of the stage
+    if (t0 < it.tok_end) step(s, sub, t0);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_empty + 8 * s);  // this warp is done with the stage
   }
   if (!ok) return;
 
@@ -403,7 +380,7 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
   l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
 
   // ---- merge the warps that share rows and write, through shared memory ---------------------
-  // every issued copy has been waited for above (by a warp with live rows), so the ring is free
+  // every issued copy has been waited for above so the ring is free
   asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumerThreads) : "memory");
   constexpr int LD = D + 4;
   float* sc_o = reinterpret_cast<float*>(smem);        // [warp][16][LD]
@@ -423,14 +400,13 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
   const int quads = D / 4;
   for (int x = tid; x < hb * it.n_rows * quads; x += kConsumerThreads) {
     const int d = (x % quads) * 4, y = x / quads, r = y % it.n_rows, hl = y / it.n_rows;
-    const int w0 = hl + ((r >> 4) << hb_log), step = 1 << (hb_log + rw_log);
     float mx = -INFINITY;
-    for (int s2 = 0; s2 < ts; ++s2) mx = fmaxf(mx, sc_ml[((w0 + s2 * step) * 16 + (r & 15)) * 2]);
+    for (int s2 = 0; s2 < ts; ++s2) mx = fmaxf(mx, sc_ml[((hl + s2 * hb) * 16 + r) * 2]);
     const float off = mx == -INFINITY ? 0.f : mx;
     float lsum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s2 = 0; s2 < ts; ++s2) {
-      const int at = (w0 + s2 * step) * 16 + (r & 15);
+      const int at = (hl + s2 * hb) * 16 + r;
       const float a = ex2(sc_ml[at * 2] - off);
       lsum = fmaf(sc_ml[at * 2 + 1], a, lsum);
       const float4 v = *reinterpret_cast<const float4*>(&sc_o[at * LD + d]);

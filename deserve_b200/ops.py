@@ -510,6 +510,14 @@ class BatchChunkWithPagedKVCacheWrapper:
             qo_indptr_host = qo_indptr.cpu().numpy()
         if kv_indptr_host is None:
             kv_indptr_host = paged_kv_indptr.cpu().numpy()
+        batch = len(qo_indptr_host) - 1
+        dev = _same_device("chunk attention", self._ws, qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
+        if paged_kv_last_page_len.shape[0] != batch or qo_indptr.shape[0] != batch + 1 or paged_kv_indptr.shape[0] != batch + 1:
+            raise ValueError("chunk attention: qo_indptr and kv_indptr must have batch + 1 entries, kv_last_page_len batch")
+        if paged_kv_indices.shape[0] < int(kv_indptr_host[-1]):
+            raise ValueError(f"chunk attention: {paged_kv_indices.shape[0]} kv_indices, kv_indptr covers {int(kv_indptr_host[-1])}")
+        pointers = (_i32_dev(qo_indptr, "qo_indptr").data_ptr(), _i32_dev(paged_kv_indices, "kv_indices").data_ptr(),
+                    _i32_dev(paged_kv_indptr, "kv_indptr").data_ptr(), _i32_dev(paged_kv_last_page_len, "kv_last_page_len").data_ptr())
         cap = chunk_plan_capacity(int(qo_indptr_host[-1]), len(qo_indptr_host) - 1, self._sm_count)
         pinned, slot = _pinned_ring("chunk_plan").take(cap)
         plan = pinned.numpy()
@@ -524,12 +532,6 @@ class BatchChunkWithPagedKVCacheWrapper:
         _pinned_ring("chunk_plan").done(slot)
         _COUNTERS["h2d_bytes"] += used * 4
         self._plan_host = plan[:16].copy()  # the header is all that a call reads on the host
-        batch = len(qo_indptr_host) - 1
-        dev = _same_device("chunk attention", self._ws, qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
-        if paged_kv_last_page_len.shape[0] != batch or qo_indptr.shape[0] != batch + 1 or paged_kv_indptr.shape[0] != batch + 1:
-            raise ValueError("chunk attention: qo_indptr and kv_indptr must have batch + 1 entries, kv_last_page_len batch")
-        pointers = (_i32_dev(qo_indptr, "qo_indptr").data_ptr(), _i32_dev(paged_kv_indices, "kv_indices").data_ptr(),
-                    _i32_dev(paged_kv_indptr, "kv_indptr").data_ptr(), _i32_dev(paged_kv_last_page_len, "kv_last_page_len").data_ptr())
         self._desc = (dev, batch, num_qo_heads, num_kv_heads, head_dim, page_size, pointers)
         self._keep = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)  # alive while planned
 

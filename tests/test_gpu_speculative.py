@@ -153,6 +153,21 @@ def test_chunk_attention_matches_prefill_and_decode():
     assert (one.wrapper.forward(one.q, one.pages).float() - dec.forward(one.q, one.pages).float()).abs().max() <= 2e-2
 
 
+def test_chunk_attention_refuses_a_plan_that_its_tensors_do_not_cover():
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    ws = torch.zeros(4 << 20, dtype=torch.uint8, device=DEV)
+    w = dk.BatchChunkWithPagedKVCacheWrapper(ws)
+    with pytest.raises(ValueError, match="kv_indices"):
+        w.begin_forward(i32([0, 2]), i32([0, 3]), i32([0, 1]), i32([4]), 8, 2, 64, 16, torch.bfloat16)
+    with pytest.raises(ValueError, match="batch"):
+        w.begin_forward(i32([0, 2]), i32([0, 3]), i32([0, 1, 2]), i32([4, 4]), 8, 2, 64, 16, torch.bfloat16)
+    assert not ws.any()  # a refused batch leaves the workspace, and the plan in it, alone
+    w.begin_forward(i32([0, 2]), i32([0, 3]), i32([0, 1, 2]), i32([4]), 8, 2, 64, 16, torch.bfloat16)
+    pages = torch.zeros(3, 2, 16, 2, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="rows"):
+        w.forward(torch.zeros(1, 8, 64, dtype=torch.bfloat16, device=DEV), pages)
+
+
 def test_chunk_attention_on_a_side_stream_and_in_a_graph():
     b = Batch(11, [5000, 40], [5, 2], 32, 8, 128, 16, torch.bfloat16).begin()
     want = b.wrapper.forward(b.q, b.pages)

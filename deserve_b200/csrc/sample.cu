@@ -667,18 +667,39 @@ __device__ __forceinline__ int pick(double inc, double target, double& rest) {
   return who;
 }
 
+// How far a running sum in double, or u times the whole, may lie from the one in fixed-point weights, in the walk's units: an entry's
+// two masses differ by at most 2^-45 of the top (its rounding, or all of a smaller one), which makes 2^-44 an entry for a running sum
+// and a target together, taken twice; 2^-32 of the whole covers the additions (2^18 roundings of 2^-53) and the series (2^-43).
+__device__ __forceinline__ double sum_margin(const Walk& w, float temperature, int vocab) {
+  const double c = 92.332482616893657 / (double)fminf(fmaxf(temperature, 1e-30f), 1e36f);
+  return (double)vocab * 0x1p-43 * exp2((double)w.top * c * 0.015625 - w.e) + w.total * 0x1p-32;
+}
+
+// floor(x all) for x in [0, 1], exact (24 bits times 63); 0 for NaN and below, all above.
+__device__ __forceinline__ u64 fraction_of(float x, u64 all) {
+  if (!(x > 0.f)) return 0;
+  if (x >= 1.f) return all;
+  const uint32_t b = __float_as_uint(x), e = b >> 23;
+  const u64 m = e ? (b & 0x7fffffu) | 0x800000u : b;
+  const int shift = 150 - (int)max(e, 1u);  // x = m 2^-shift, 24 <= shift <= 149
+  const u64 hi = __umul64hi(m, all), lo = m * all;  // hi < 2^24
+  return shift < 64 ? (hi << (64 - shift)) | (lo >> shift) : hi >> min(shift - 64, 63);
+}
+
 // The draw of a row without a cut from the sums that weight_walk left: only the subsegment that holds the target is read again.
-// (Every CTA joins the same numbers in the same order, so exactly one of them finds the target its own.)
+// (Every CTA joins the same numbers in the same order, so exactly one of them finds the target its own.) The sums are grouped by the
+// launch and count weights that cannot be drawn, so they decide only where the target lies farther than `sum_margin` from both ends
+// of the token's mass; there the fixed-point sums give the same token. false (in all threads of the cluster): they do not. Slot 35.
 template <typename T, int NT, bool kShared>
-__device__ void draw_all(const Slice<T, NT, kShared>& sl, const Walk& walk, float temperature, float u, int32_t* out, Shared& sh) {
+__device__ __forceinline__ bool draw_in_subsegment(const Slice<T, NT, kShared>& sl, const Walk& walk, float temperature, float u, int32_t* out,
+                                                   Shared& sh) {
   constexpr int N = Vec16<T>::N;
   const int lane = threadIdx.x & 31;
-  if (threadIdx.x >= 32) return;
   const float t = fminf(fmaxf(temperature, 1e-30f), 1e36f);
   const double c = 92.332482616893657 / (double)t;
-  double rest, inc;
-  const int owner = pick(walk.inc, fmin((double)u, 1.0) * walk.total, rest);
-  if (owner != (int)cluster_rank()) return;
+  double rest, inc, margin = sum_margin(walk, temperature, sl.limit);
+  const int owner = pick(walk.inc, u > 0.f ? fmin((double)u, 1.0) * walk.total : 0.0, rest);
+  if (owner != (int)cluster_rank()) return true;
   const bool in = lane < NT / 32;
   const double own_e = in ? as_double(sh.warp_b[lane]) : -INFINITY;
   double mass = in ? as_double(sh.warp_a[lane]) : 0.0, e = own_e;
@@ -686,6 +707,7 @@ __device__ void draw_all(const Slice<T, NT, kShared>& sl, const Walk& walk, floa
   const int w = pick(inc, rest * power(walk.e - e), rest);
   const double e_w = __shfl_sync(0xffffffffu, own_e, w);
   rest *= power(e - e_w);
+  margin *= power(walk.e - e) * power(e - e_w);
   inc = lane < kSub ? as_double(sh.seg[w * kSub + lane]) : 0.0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -696,7 +718,6 @@ __device__ void draw_all(const Slice<T, NT, kShared>& sl, const Walk& walk, floa
   const float lowest = walk.top - 31.2f * t;  // weights below 2^-45 of the largest cannot be drawn
   const double magic = 6755399441055744.0 - 64.0 * e_w;
   const int a = min(sl.begin(w) + k * sl.sub, sl.end(w)), b = min(a + sl.sub, sl.end(w));
-  int last = -1;
   for (int v0 = a; v0 < b; v0 += 32) {
     const int v = v0 + lane;
     double m[N], total = 0.0;
@@ -704,7 +725,6 @@ __device__ void draw_all(const Slice<T, NT, kShared>& sl, const Walk& walk, floa
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = -INFINITY;
     if (v < b) sl.get(v, f);
-    int mine = -1;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       m[i] = 0.0;
@@ -712,7 +732,6 @@ __device__ void draw_all(const Slice<T, NT, kShared>& sl, const Walk& walk, floa
         double scaled, series;
         double_weight(f[i], c, magic, sh.table, scaled, series);
         m[i] = scaled * series;
-        mine = sl.first + v * N + i;
       }
       total += m[i];
     }
@@ -726,23 +745,36 @@ __device__ void draw_all(const Slice<T, NT, kShared>& sl, const Walk& walk, floa
     if (hit) {
       const int who = __ffs(hit) - 1;
       const double before = __shfl_up_sync(0xffffffffu, inc, 1);
+      bool sure = false;
       if (lane == who) {
-        double run = lane > 0 ? before : 0.0;
+        double run = lane > 0 ? before : 0.0, to_low = 0.0, to_high = 0.0;
         int i = -1;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          if (m[j] > 0.0 && (i < 0 || run <= rest)) i = j;
+          if (m[j] > 0.0 && (i < 0 || run <= rest)) {
+            i = j;
+            to_low = rest - run;
+            to_high = m[j] - to_low;
+          }
           run += m[j];
         }
-        *out = sl.first + v * N + i;
+        sure = to_low > margin && to_high > margin;
+        if (sure) *out = sl.first + v * N + i;
       }
-      return;
+      return __any_sync(0xffffffffu, sure);
     }
-    mine = __reduce_max_sync(0xffffffffu, mine);
-    last = max(last, mine);
     rest = fmax(rest - __shfl_sync(0xffffffffu, inc, 31), 0.0);
   }
-  if (lane == 0) *out = max(last, 0);  // (a last unit of rounding left nothing: its last entry)
+  return false;  // among weights that cannot be drawn
+}
+template <typename T, int NT, bool kShared>
+__device__ bool draw_all(const Slice<T, NT, kShared>& sl, const Walk& walk, float temperature, float u, int32_t* out, Shared& sh) {
+  if (threadIdx.x < 32) {
+    const bool sure = draw_in_subsegment(sl, walk, temperature, u, out, sh);
+    if (threadIdx.x == 0) sh.slot[35].a = sure ? 0 : 1;
+  }
+  cluster_sync();
+  return cluster_max(&sh.slot[35].a) == 0;
 }
 
 // Sums over the cluster of up to three integers per warp (in its lane 0), through slot `s`: the wholes, and what the CTAs
@@ -1043,8 +1075,8 @@ __device__ bool count_border(const Slice<T, NT, kShared>& sl, const RowScale& s,
   return false;  // cannot happen with top_p < 1
 }
 
-// Top-p border of the row. `known`: the sum of its weights in units of the fixed-point weights, or -1. Without a cut and
-// with an unknown sum the masses of the subsegments are left in sh.seg (`mine`: the warp's). Slots 2 to 30.
+// Top-p border of the row. `known`: the sum of its weights in units of the fixed-point weights, or -1. Without a cut the masses of
+// the subsegments are left in sh.seg (`mine`: the warp's). Slots 2 to 30.
 template <typename T, int NT, bool kShared>
 __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, float top_p, double known, Near& near, Shared& sh, u64& mine) {
   constexpr int N = Vec16<T>::N;
@@ -1057,10 +1089,6 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
   mine = 0;
   near.n = 0;
   near.usable = false;
-  if (!(top_p < 1.f) && known >= 0.0) {
-    k.total = (u64)known;
-    return k;
-  }
   if (!(top_p < 1.f)) {  // NaN: no cut
     mine = sl.sum(sh, [&](const float (&f)[N], int) {
       u64 x = 0;
@@ -1292,10 +1320,7 @@ __device__ bool draw(const Slice<T, NT, kShared>& sl, const Mass& mass, const Ne
                      Shared& sh) {
   constexpr int N = Vec16<T>::N;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto target_of = [&](u64 all) {
-    const double x = u > 0.f ? (double)u * (double)all : 0.0;  // NaN: 0
-    return x < (double)all ? min((u64)x, all - 1) : all - 1;
-  };
+  auto target_of = [&](u64 all) { return min(fraction_of(u, all), all - 1); };
   if (near.usable) {  // every kept token is in the lists
     auto of = [&](const Entry& e) { return mass.kept.holds(e.l, e.i) ? mass.of_weight(e.w, e.i) : 0; };
     const Entry* list = near.mine();
@@ -1469,7 +1494,6 @@ __device__ bool draw_rest(const Slice<T, NT, kShared>& sl, const Walk& walk, flo
 __device__ __forceinline__ double in_fixed_units(const Walk& w, const RowScale& s) {
   return w.far ? -1.0 : w.total * exp2(44.0 + (w.e - (6755399441055744.0 - s.magic) * 0.015625));
 }
-constexpr float kLeastU = 1e-7f;  // random numbers below go the exact way: what cannot be drawn must not be met there
 
 template <typename T, int NT, bool kShared>
 __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParams p) {
@@ -1499,8 +1523,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     mass.kept.value = -INFINITY;
     mass.kept.index = -1;
     double z;  // the kept weights' sum, in units of the top's
-    if (!(top_p < 1.f) && !walk.far && u >= kLeastU) {
-      draw_all(sl, walk, t, u, p.tokens + r, sh);
+    if (!(top_p < 1.f) && !walk.far && draw_all(sl, walk, t, u, p.tokens + r, sh)) {
       z = in_fixed_units(walk, mass.s);
     } else {
       u64 mine;
@@ -1715,18 +1738,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
     Mass mass;
     u64 mine = 0;
     Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
-    const bool plain = !greedy && !cut && !walk.far && u >= kLeastU;  // sums in double will do
     const bool none = walk.top == -INFINITY;
-    if (!greedy && !none) {
+    bool done = greedy || none;
+    if (done) {
+      if (lead) p.tokens[req] = max(first, 0);
+    } else {
       const float top = settle(sl, walk.top);
       mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
       const double known = cut || !last ? in_fixed_units(walk, mass.s) : -1.0;
-      if (plain) {
+      const bool plain = !cut && !walk.far;  // sums in double will do
+      if (plain && !last) {
         mass.kept.value = -INFINITY;
         mass.kept.index = -1;
-        mass.kept.total = (u64)fmax(in_fixed_units(walk, mass.s), 1.0);
+        mass.kept.total = (u64)fmax(known, 1.0);
       } else {
-        mass.kept = find_kept(sl, mass.s, top_p, known, near, sh, mine);
+        if (plain) done = draw_all(sl, walk, t, u, p.tokens + req, sh);
+        if (!done) mass.kept = find_kept(sl, mass.s, top_p, known, near, sh, mine);
       }
       if (said == kUnknown) {
         const float l = rewritten(to_f32(row[x]), sl.how);
@@ -1736,22 +1763,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
           continue;
         }
       }
-    }
-    if (lead) p.accepted[req] = r - begin;
-    if (greedy || none) {
-      if (lead) p.tokens[req] = max(first, 0);
-    } else if (plain && last) {
-      draw_all(sl, walk, t, u, p.tokens + req, sh);
-    } else if (!plain || !draw_rest(sl, walk, t, q_row, q_row == nullptr ? x : -1, u, p.tokens + req, sh)) {
-      mass.inv_z = 1.0 / (double)mass.kept.total;
-      mass.residual = !last && !plain;  // (plain: nothing is left above the draft's distribution, the target's own is drawn from)
-      mass.minus = last ? nullptr : q_row;
-      mass.one_hot = q_row == nullptr ? x : -1;
-      if (!draw(sl, mass, near, u, last && !cut && !plain, mine, 31, p.tokens + req, sh) && mass.residual) {
-        mass.residual = false;
-        draw(sl, mass, near, u, false, 0, 34, p.tokens + req, sh);
+      if (!done && plain && !last) done = draw_rest(sl, walk, t, q_row, q_row == nullptr ? x : -1, u, p.tokens + req, sh);
+      if (!done) {
+        mass.inv_z = 1.0 / (double)mass.kept.total;
+        mass.residual = !last && !plain;  // (plain: nothing is left above the draft's distribution, the target's own is drawn from)
+        mass.minus = last ? nullptr : q_row;
+        mass.one_hot = q_row == nullptr ? x : -1;
+        if (!draw(sl, mass, near, u, last && !cut, mine, 31, p.tokens + req, sh) && mass.residual) {
+          mass.residual = false;
+          draw(sl, mass, near, u, false, 0, 34, p.tokens + req, sh);
+        }
       }
     }
+    if (lead) p.accepted[req] = r - begin;
     break;
   }
   cluster_sync();

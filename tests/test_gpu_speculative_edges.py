@@ -1,0 +1,64 @@
+"""Speculative operators where a border is met exactly, at the ends of the number range, and on calls that are allowed but
+unusual. Expected tokens follow from the definition by counting: equal logits have equal weights, so running sums are whole
+multiples of one weight and a dyadic random number meets a border exactly."""
+import numpy as np
+import pytest
+import torch
+
+import deserve_b200 as dk
+from deserve_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+INF = float("inf")
+
+
+@pytest.fixture(autouse=True)
+def _device_status_clean():
+    yield
+    assert _lib.read_device_status() == 0, "a kernel self-check fired"
+
+
+def _full(n, value):
+    return torch.full((n,), float(value), device=DEV)
+
+
+def _sample(row, rows, temperature, top_p, u, **kw):
+    """Tokens of `rows` copies of one row."""
+    x = row.to(DEV).expand(rows, -1).contiguous()
+    return dk.sample_top_p(x, _full(rows, temperature), _full(rows, top_p), _full(rows, u), **kw).cpu()
+
+
+def _last_row(row, requests, temperature, top_p, u):
+    """The token that verification draws for requests without drafts."""
+    x = row.to(DEV).expand(requests, -1).contiguous()
+    n, tok = dk.verify_draft(x, torch.zeros(requests, dtype=torch.int32, device=DEV),
+                             torch.arange(requests + 1, dtype=torch.int32, device=DEV), _full(requests, u),
+                             _full(requests, temperature), _full(requests, top_p))
+    assert (n == 0).all()
+    return tok.cpu()
+
+
+# ---- draws without a cut -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature,far", [(1.0, -32.0), (0.6, -20.0)])
+@pytest.mark.parametrize("rows", [1, 128, 1024])
+def test_a_draw_never_ends_among_weights_that_cannot_be_drawn(dtype, temperature, far, rows):
+    """Two equal tokens, between them a vocabulary of weights below 2^-45 of theirs, no token at 0: a draw at one half meets
+    the end of the first token's mass and takes the second."""
+    row = torch.full((128256,), far, dtype=dtype)
+    row[0], row[5000], row[128255] = -INF, 0.0, 0.0
+    for draw in (_sample, _last_row):
+        assert (draw(row, rows, temperature, 1.0, 0.5) == 128255).all()
+        assert (draw(row, rows, temperature, 1.0, 0.5 - 2.0**-25) == 5000).all()
+
+
+@pytest.mark.parametrize("vocab,value", [(1000, 0.0), (1000, 5.0), (5000, 5.0), (5000, -3.75), (4096, 0.3125), (32000, 7.5)])
+@pytest.mark.parametrize("rows", [1, 40, 299, 1024])
+def test_draws_at_exact_borders_do_not_depend_on_the_launch(vocab, value, rows):
+    """All tokens equal: u of the whole is exactly the mass of the first u * vocab tokens, and the next one is drawn."""
+    row = torch.full((vocab,), value)
+    for u in (0.125, 0.25, 0.5, 0.75, 0.875):
+        for draw in (_sample, _last_row):
+            assert (draw(row, rows, 0.7, 1.0, u) == int(u * vocab)).all(), u

@@ -230,7 +230,7 @@ __device__ __forceinline__ RowScale row_scale(float top, float temperature) {
   // A temperature so small that one unit in the last place of the top already gives weight 0 gives the same weights
   // as 2^37 / |top|, which keeps the exponents in range.
   if (fabs((double)top * s.c) > 137438953472.0) s.c = 137438953472.0 / fabs((double)top);
-  const float ulp = __uint_as_float(__float_as_uint(fabsf(top)) + 1u) - fabsf(top);
+  const float a = fabsf(top), ulp = a > 0.f ? a - __uint_as_float(__float_as_uint(a) - 1u) : 1.4e-45f;  // (finite for the largest number too)
   s.cutoff = top - fmaxf(64.f * s.t, 2.f * ulp);
   s.magic = 6755399441055744.0 - rint((double)top * s.c);
   return s;

@@ -62,3 +62,33 @@ def test_draws_at_exact_borders_do_not_depend_on_the_launch(vocab, value, rows):
     for u in (0.125, 0.25, 0.5, 0.75, 0.875):
         for draw in (_sample, _last_row):
             assert (draw(row, rows, 0.7, 1.0, u) == int(u * vocab)).all(), u
+
+
+# ---- the ends of the number range ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("top_p", [0.9, 1.0])
+@pytest.mark.parametrize("rest", ["ordinary", "masked", "lowest"])
+def test_a_token_forced_by_the_largest_number_is_always_drawn(dtype, top_p, rest):
+    info = torch.finfo(dtype)
+    row = torch.randn(1000, generator=torch.Generator().manual_seed(1)) * 3
+    row[::5] = -INF
+    if rest != "ordinary":
+        row[:] = -INF if rest == "masked" else info.min
+    row[7], row[1:4] = info.max, torch.tensor([0.0, 1.0, -5.0])
+    row = row.to(dtype)
+    probs = torch.empty(3, 1000, device=DEV)
+    for u in (0.0, 0.3, 0.999):
+        for t in (1.0, 1e-3):
+            assert (_sample(row, 3, t, top_p, u, probs=probs) == 7).all()
+            assert (probs[:, 7] == 1).all() and probs.sum() == 3
+            assert (_last_row(row, 3, t, top_p, u) == 7).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_two_tokens_at_the_largest_number_share_a_row(dtype):
+    row = torch.zeros(1000, dtype=dtype)
+    row[7] = row[900] = torch.finfo(dtype).max
+    for top_p in (0.9, 1.0):
+        for u, want in ((0.25, 7), (0.5, 900), (0.75, 900)):
+            assert (_sample(row, 2, 1.0, top_p, u) == want).all()
+    assert (_sample(row, 2, 1.0, 0.25, 0.99) == 7).all()  # the nucleus ends with the first

@@ -595,8 +595,9 @@ __device__ Walk weight_walk(const Slice<T, NT, kShared>& sl, uint4* buf, float t
       if (m > -INFINITY) {
         e = fabs(x) < 1e6 ? rint(x) : 0.0;
         far |= !(fabs(x) < 1e6);
-        cutoff = m - fminf(0.69f * (float)kReach * t, 1e37f);
-        far |= !(cutoff > -3e38f && cutoff < m);
+        const float reach = 0.69f * (float)kReach * t;  // what lies farther below counts as much as that: less than can be drawn
+        cutoff = m - reach;
+        far |= !(reach < 1e37f && cutoff > -3e38f && cutoff < m);
         magic = 6755399441055744.0 - 64.0 * e;
       }
     }

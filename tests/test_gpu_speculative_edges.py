@@ -92,3 +92,19 @@ def test_two_tokens_at_the_largest_number_share_a_row(dtype):
         for u, want in ((0.25, 7), (0.5, 900), (0.75, 900)):
             assert (_sample(row, 2, 1.0, top_p, u) == want).all()
     assert (_sample(row, 2, 1.0, 0.25, 0.99) == 7).all()  # the nucleus ends with the first
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature", [1e34, 1e36, 3e38, INF])
+@pytest.mark.parametrize("hidden", [-INF, float("nan")])
+def test_masked_entries_have_no_weight_at_any_temperature(dtype, temperature, hidden):
+    """64 tokens among 131,072 entries, evenly likely: half of them side by side, half of them far apart."""
+    at = list(range(100, 132)) + list(range(1000, 131072, 4096))
+    row = torch.full((131072,), hidden, dtype=dtype)
+    row[at] = torch.linspace(-3, 3, 64).to(dtype)
+    for rows in (1, 300):
+        for u in (0.0, 0.26, 0.51, 0.99):
+            want = at[int(64 * u)]
+            for top_p in (1.0, 1 - 2.0**-24):
+                assert (_sample(row, rows, temperature, top_p, u) == want).all()
+                assert (_last_row(row, rows, temperature, top_p, u) == want).all()

@@ -1685,7 +1685,11 @@ __global__ void __launch_bounds__(kQuickThreads, 4) verify_rows_kernel(const Sam
   const int r = blockIdx.x / cluster_size();
   const int req = owner_of(p.indptr, p.batch, r);
   const int begin = __ldg(p.indptr + req), end = __ldg(p.indptr + req + 1);
-  if (r < begin || r + 1 >= end || end > p.nnz) return;  // a last row, or behind the last request (the whole cluster)
+  if (r < begin || r + 1 >= end || end > p.nnz) {  // a last row, or behind the last request (the whole cluster)
+    // With an indptr that is not monotone the draw kernel may take it for another request's: nothing there is left undefined.
+    if (cluster_rank() == 0 && threadIdx.x == 0) p.ok[r] = kRejected;
+    return;
+  }
   const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)r * p.row_stride;
   const int x = __ldg(p.draft + r + 1);
   const float t = __ldg(p.temperature + req), top_p = __ldg(p.top_p + req);

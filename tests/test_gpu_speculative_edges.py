@@ -108,3 +108,29 @@ def test_masked_entries_have_no_weight_at_any_temperature(dtype, temperature, hi
             for top_p in (1.0, 1 - 2.0**-24):
                 assert (_sample(row, rows, temperature, top_p, u) == want).all()
                 assert (_last_row(row, rows, temperature, top_p, u) == want).all()
+
+
+# ---- calls that are refused on the device --------------------------------------------------------------------------------------
+def test_verify_draft_with_an_indptr_that_is_not_monotone_reads_nothing_it_should_not():
+    """Requests whose rows belong to no request of the search, drafts that are no tokens, and scratch full of old verdicts: the bad
+    request is reported, the others end."""
+    vocab, nnz = 5000, 8
+    indptr = torch.tensor([0, 5, 3, 8], dtype=torch.int32, device=DEV)
+    logits = torch.randn(nnz, vocab, generator=torch.Generator().manual_seed(1)).to(DEV)
+    tokens = torch.full((nnz,), 2**31 - 1, dtype=torch.int32, device=DEV)
+    tokens[1], tokens[4] = logits[0].argmax(), logits[3].argmax()
+    u, one = _full(nnz, 1e-6), _full(3, 1.0)
+    torch.cuda.synchronize()
+    _lib.read_device_status()
+    for old in (0x00, 0x01, 0x02):
+        accepted, following = (torch.empty(3, dtype=torch.int32, device=DEV) for _ in range(2))
+        scratch = torch.full((nnz,), old, dtype=torch.uint8, device=DEV)
+        rc = _lib.lib.dsv_verify_draft(logits.data_ptr(), vocab, nnz, vocab, tokens.data_ptr(), indptr.data_ptr(), 3, u.data_ptr(),
+                                       one.data_ptr(), one.data_ptr(), None, 0, scratch.data_ptr(), nnz, accepted.data_ptr(),
+                                       following.data_ptr(), _lib.dtype_code(torch.float32), _lib.current_stream_ptr())
+        assert rc == 0
+        torch.cuda.synchronize()
+        assert _lib.read_device_status() == 2  # inconsistent indptr
+        assert (scratch <= 2).all() and following[1] == -1
+        assert accepted.tolist() == [1, 0, 1]  # the last request gets to row 4, which the search gives to the first one
+        assert ((following[[0, 2]] >= 0) & (following[[0, 2]] < vocab)).all()

@@ -1146,7 +1146,7 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
   Slot whole = cluster_total<NT>(warp_sum(sum), warp_sum(whole_mass), (u64)near.n + (near.n > near.cap ? 1ull << 40 : 0), sh, 2, before);
   if (known >= 0.0) whole.b = (u64)known;
   k.total = whole.b;
-  u64 limit = (u64)((double)fmaxf(top_p, 0.f) * (double)whole.b), mass, kept = 0;
+  u64 limit = fraction_of(top_p, whole.b), mass, kept = 0;
   near.usable = limit < whole.a && whole.c < 1ull << 40;
   if constexpr (sizeof(T) == 2) {
     if (!near.usable && sl.how == kAsIs && count_border(sl, s, limit, k, sh)) return k;
@@ -1292,6 +1292,25 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
       k.total = kept + mass;
       return k;
     }
+  }
+}
+
+// The same with a border that does not depend on the launch. `known` comes from sums in double, so that the limit top_p * known may lie to
+// the other side of a token's mass than the one of the fixed-point sum: a border that close to an end of its token's mass (the two
+// sums differ by 2^-45 of the top, half a unit, an entry, and 2^-33 of the whole, see sum_margin) is searched again with that sum.
+template <typename T, int NT, bool kShared>
+__device__ __forceinline__ Kept settled_border(const Slice<T, NT, kShared>& sl, const RowScale& s, float top_p, double known, Near& near, Shared& sh,
+                                               u64& mine) {
+  for (;;) {
+    const Kept k = find_kept(sl, s, top_p, known, near, sh, mine);
+    if (!(top_p < 1.f) || known < 0.0) return k;
+    const u64 limit = fraction_of(top_p, (u64)known), margin = (u64)sl.limit + (u64)(known * 0x1p-32);
+    const u64 below = k.total - (raw_weight(k.value, s, sh.table) - kRaw);  // ranked before the last kept token
+    if (limit > below + margin && limit + margin < k.total) return k;
+    known = -1.0;
+    cluster_sync();  // the others may still read this CTA's slots and list
+    if (threadIdx.x == 0) sh.n_list = 0;
+    __syncthreads();
   }
 }
 
@@ -1529,7 +1548,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleParam
     } else {
       u64 mine;
       Near near = {reinterpret_cast<Entry*>(dyn), p.cap, 0, false};
-      mass.kept = find_kept(sl, mass.s, top_p, top_p < 1.f ? in_fixed_units(walk, mass.s) : -1.0, near, sh, mine);
+      mass.kept = settled_border(sl, mass.s, top_p, top_p < 1.f ? in_fixed_units(walk, mass.s) : -1.0, near, sh, mine);
       mass.residual = false;
       mass.inv_z = 0.0; mass.minus = nullptr; mass.one_hot = -1;
       draw(sl, mass, near, u, !(top_p < 1.f), mine, 32, p.tokens + r, sh);
@@ -1758,7 +1777,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
         mass.kept.total = (u64)fmax(known, 1.0);
       } else {
         if (plain) done = draw_all(sl, walk, t, u, p.tokens + req, sh);
-        if (!done) mass.kept = find_kept(sl, mass.s, top_p, known, near, sh, mine);
+        if (!done) mass.kept = settled_border(sl, mass.s, top_p, known, near, sh, mine);
       }
       if (said == kUnknown) {
         const float l = rewritten(to_f32(row[x]), sl.how);

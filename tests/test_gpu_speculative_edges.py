@@ -64,6 +64,37 @@ def test_draws_at_exact_borders_do_not_depend_on_the_launch(vocab, value, rows):
             assert (draw(row, rows, 0.7, 1.0, u) == int(u * vocab)).all(), u
 
 
+# ---- the nucleus' border -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,value", [(1000, 0.0), (1000, 0.3125), (1000, -3.75), (5000, 5.0), (32000, 7.5)])
+@pytest.mark.parametrize("rows", [1, 40, 299, 1024])
+def test_nucleus_borders_met_exactly_do_not_depend_on_the_launch(dtype, vocab, value, rows):
+    """All tokens equal, top_p of the whole is exactly the mass of the first top_p * vocab tokens: the one behind them is kept too
+    (the mass ranked before it is not more than top_p), and no other."""
+    row = torch.full((vocab,), value, dtype=dtype)
+    probs = torch.empty(rows, vocab, device=DEV)
+    for top_p in (0.0, 0.125, 0.25, 0.5, 0.75):
+        kept = int(top_p * vocab) + 1
+        assert (_sample(row, rows, 0.7, top_p, 1 - 2.0**-24, probs=probs) == kept - 1).all()
+        assert (probs[:, :kept] > 0).all() and (probs[:, kept:] == 0).all()
+        assert (_last_row(row, rows, 0.7, top_p, 1 - 2.0**-24) == kept - 1).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 128, 700])
+def test_nucleus_borders_between_the_values_of_a_row(dtype, rows):
+    """Eight tokens at the top, the other 1,016 entries at a 64th of their weight (their border lies behind the listed entries, or among
+    them, depending on the launch): 8 + 1016 / 64 = 23.875 of the top's mass. top_p 0.5 keeps 11.9375 of it: 8 + 3.9375 * 64 = 252
+    of the others rank before the border exactly, one more is kept."""
+    row = torch.full((1024,), -6.0, dtype=dtype)
+    row[500:508] = 0.0
+    temperature = 1 / float(np.log(2.0))  # weights of 2^l; as fp32 off by up to 2^-25, the border by 6 * 2^-25 * 11 << 1 / 64
+    probs = torch.empty(rows, 1024, device=DEV)
+    _sample(row, rows, temperature, 0.5, 0.5, probs=probs)
+    assert ((probs > 0).sum(1) - 8 - 252).abs().max() <= 1  # to the side on which the rounded temperature puts the border
+    assert (probs == probs[0]).all()
+
+
 # ---- the ends of the number range ----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("top_p", [0.9, 1.0])

@@ -668,12 +668,16 @@ __device__ __forceinline__ int pick(double inc, double target, double& rest) {
   return who;
 }
 
+// The top's weight in the walk's units.
+__device__ __forceinline__ double top_units(const Walk& w, float temperature) {
+  const double c = 92.332482616893657 / (double)fminf(fmaxf(temperature, 1e-30f), 1e36f);
+  return exp2((double)w.top * c * 0.015625 - w.e);
+}
 // How far a running sum in double, or u times the whole, may lie from the one in fixed-point weights, in the walk's units: an entry's
 // two masses differ by at most 2^-45 of the top (its rounding, or all of a smaller one), which makes 2^-44 an entry for a running sum
 // and a target together, taken twice; 2^-32 of the whole covers the additions (2^18 roundings of 2^-53) and the series (2^-43).
 __device__ __forceinline__ double sum_margin(const Walk& w, float temperature, int vocab) {
-  const double c = 92.332482616893657 / (double)fminf(fmaxf(temperature, 1e-30f), 1e36f);
-  return (double)vocab * 0x1p-43 * exp2((double)w.top * c * 0.015625 - w.e) + w.total * 0x1p-32;
+  return (double)vocab * 0x1p-43 * top_units(w, temperature) + w.total * 0x1p-32;
 }
 
 // floor(x all) for x in [0, 1], exact (24 bits times 63); 0 for NaN and below, all above.
@@ -685,6 +689,26 @@ __device__ __forceinline__ u64 fraction_of(float x, u64 all) {
   const int shift = 150 - (int)max(e, 1u);  // x = m 2^-shift, 24 <= shift <= 149
   const u64 hi = __umul64hi(m, all), lo = m * all;  // hi < 2^24
   return shift < 64 ? (hi << (64 - shift)) | (lo >> shift) : hi >> min(shift - 64, 63);
+}
+
+// The entry of a vector whose mass holds the target, `run` the sum before the vector: written, and true, where the target is farther
+// than the margin from both ends of that mass.
+template <int N>
+__device__ __forceinline__ bool take(const double (&m)[N], double run, double target, double margin, int first, int32_t* out) {
+  double to_low = 0.0, to_high = 0.0;
+  int i = -1;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (m[j] > 0.0 && (i < 0 || run <= target)) {
+      i = j;
+      to_low = target - run;
+      to_high = m[j] - to_low;
+    }
+    run += m[j];
+  }
+  const bool sure = to_low > margin && to_high > margin;
+  if (sure) *out = first + i;
+  return sure;
 }
 
 // The draw of a row without a cut from the sums that weight_walk left: only the subsegment that holds the target is read again.
@@ -747,22 +771,8 @@ __device__ __forceinline__ bool draw_in_subsegment(const Slice<T, NT, kShared>& 
       const int who = __ffs(hit) - 1;
       const double before = __shfl_up_sync(0xffffffffu, inc, 1);
       bool sure = false;
-      if (lane == who) {
-        double run = lane > 0 ? before : 0.0, to_low = 0.0, to_high = 0.0;
-        int i = -1;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          if (m[j] > 0.0 && (i < 0 || run <= rest)) {
-            i = j;
-            to_low = rest - run;
-            to_high = m[j] - to_low;
-          }
-          run += m[j];
-        }
-        sure = to_low > margin && to_high > margin;
-        if (sure) *out = sl.first + v * N + i;
-      }
-      return __any_sync(0xffffffffu, sure);
+      if (lane == who) sure = take(m, lane > 0 ? before : 0.0, rest, margin, sl.first + v * N, out);
+      return __any_sync(0xffffffffu, sure) != 0;
     }
     rest = fmax(rest - __shfl_sync(0xffffffffu, inc, 31), 0.0);
   }
@@ -1392,7 +1402,9 @@ __device__ __forceinline__ uint4* slice_of(unsigned char* dyn, const SampleParam
 }
 
 // The draw of a row without a cut from max(p - q, 0), in double like weight_walk: masses of the subsegments, then the one that holds
-// the target again. false: no mass. Slot 33.
+// the target again. As in draw_all the sums decide only away from the ends of the token's mass: p of an entry differs from the
+// fixed-point one by 2^-45 of the top's p and by the relative difference of the two wholes, which makes twice sum_margin here, in
+// units of the whole. false (in all threads of the cluster): they do not, or hardly anything is left. Slots 33 and 35.
 template <typename T, int NT, bool kShared>
 __device__ bool draw_rest(const Slice<T, NT, kShared>& sl, const Walk& walk, float temperature, const float* q, int one_hot, float u,
                           int32_t* out, Shared& sh) {
@@ -1459,55 +1471,48 @@ __device__ bool draw_rest(const Slice<T, NT, kShared>& sl, const Walk& walk, flo
   mass = lane < (int)cluster_size() ? as_double(ld_remote64(remote(&sh.slot[33].a, lane))) : 0.0;
   same = 0.0;
   join(mass, same, inc, lane);
-  const double all = __shfl_sync(0xffffffffu, inc, 31);
-  if (!(all > 0.0)) return false;
-  if (warp != 0) return true;
-  double rest;
-  if (pick(inc, u > 0.f ? fmin((double)u, 1.0) * all : 0.0, rest) != (int)cluster_rank()) return true;
-  mass = lane < NT / 32 ? as_double(sh.warp_a[lane]) : 0.0;
-  join(mass, same, inc, lane);
-  const int w = pick(inc, rest, rest);
-  mass = lane < kSub ? as_double(sh.seg[w * kSub + lane]) : 0.0;
-  join(mass, same, inc, lane);
-  const int k = pick(inc, rest, rest), a = min(sl.begin(w) + k * sl.sub, sl.end(w)), b = min(a + sl.sub, sl.end(w));
-  int last = -1;
-  for (int v0 = a; v0 < b; v0 += 32) {
-    const int v = v0 + lane;
-    float f[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = -INFINITY;
-    if (v < b) sl.get(v, f);
-    double m[N], total = 0.0;
-    int mine = -1;
-    rest_of(f, sl.first + min(v, b - 1) * N, m);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      total += m[i];
-      if (m[i] > 0.0) mine = sl.first + v * N + i;
-    }
-    mass = total;
+  const double all = __shfl_sync(0xffffffffu, inc, 31), margin = 2.0 * sum_margin(walk, temperature, sl.limit) * inv;
+  if (!(all > margin)) return false;
+  // (warp 0 of the CTA that holds the target; the answer of the others is yes)
+  auto settle_token = [&]() {
+    double rest;
+    if (pick(inc, u > 0.f ? fmin((double)u, 1.0) * all : 0.0, rest) != (int)cluster_rank()) return true;
+    mass = lane < NT / 32 ? as_double(sh.warp_a[lane]) : 0.0;
     join(mass, same, inc, lane);
-    const unsigned hit = __ballot_sync(0xffffffffu, inc > rest);
-    if (hit) {
-      const int who = __ffs(hit) - 1;
-      const double before = __shfl_up_sync(0xffffffffu, inc, 1);
-      if (lane == who) {
-        double run = lane > 0 ? before : 0.0;
-        int i = -1;
+    const int w = pick(inc, rest, rest);
+    mass = lane < kSub ? as_double(sh.seg[w * kSub + lane]) : 0.0;
+    join(mass, same, inc, lane);
+    const int k = pick(inc, rest, rest), a = min(sl.begin(w) + k * sl.sub, sl.end(w)), b = min(a + sl.sub, sl.end(w));
+    for (int v0 = a; v0 < b; v0 += 32) {
+      const int v = v0 + lane;
+      float f[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          if (m[j] > 0.0 && (i < 0 || run <= rest)) i = j;
-          run += m[j];
-        }
-        *out = sl.first + v * N + i;
+      for (int i = 0; i < N; ++i) f[i] = -INFINITY;
+      if (v < b) sl.get(v, f);
+      double m[N], total = 0.0;
+      rest_of(f, sl.first + min(v, b - 1) * N, m);
+#pragma unroll
+      for (int i = 0; i < N; ++i) total += m[i];
+      mass = total;
+      join(mass, same, inc, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, inc > rest);
+      if (hit) {
+        const int who = __ffs(hit) - 1;
+        const double before = __shfl_up_sync(0xffffffffu, inc, 1);
+        bool sure = false;
+        if (lane == who) sure = take(m, lane > 0 ? before : 0.0, rest, margin, sl.first + v * N, out);
+        return __any_sync(0xffffffffu, sure) != 0;
       }
-      return true;
+      rest = fmax(rest - __shfl_sync(0xffffffffu, inc, 31), 0.0);
     }
-    last = max(last, __reduce_max_sync(0xffffffffu, mine));
-    rest = fmax(rest - __shfl_sync(0xffffffffu, inc, 31), 0.0);
+    return false;
+  };
+  if (warp == 0) {
+    const bool sure = settle_token();
+    if (lane == 0) sh.slot[35].a = sure ? 0 : 1;
   }
-  if (lane == 0) *out = max(last, 0);
-  return true;
+  cluster_sync();
+  return cluster_max(&sh.slot[35].a) == 0;
 }
 
 // The sum of weight_walk in units of the fixed-point weights, -1 where it does not hold.
@@ -1769,31 +1774,33 @@ __global__ void __launch_bounds__(NT, 1024 / NT) verify_draw_kernel(const Sample
     } else {
       const float top = settle(sl, walk.top);
       mass.s = row_scale(top, sl.how == kQuartered ? t * 0.25f : t);
-      const double known = cut || !last ? in_fixed_units(walk, mass.s) : -1.0;
-      const bool plain = !cut && !walk.far;  // sums in double will do
-      if (plain && !last) {
-        mass.kept.value = -INFINITY;
-        mass.kept.index = -1;
-        mass.kept.total = (u64)fmax(known, 1.0);
-      } else {
-        if (plain) done = draw_all(sl, walk, t, u, p.tokens + req, sh);
-        if (!done) mass.kept = settled_border(sl, mass.s, top_p, known, near, sh, mine);
-      }
-      if (said == kUnknown) {
-        const float l = rewritten(to_f32(row[x]), sl.how);
-        const double qx = q_row == nullptr ? 1.0 : (double)__ldg(q_row + x);
-        if (mass.kept.holds(l, x) && (double)__ldg(p.uniform + r) * qx < weight(l, mass.s) * (top_weight(mass.s) / (double)mass.kept.total)) {
+      // Sums in double decide where they are far enough from a border, else the row goes the exact way.
+      bool plain = !cut && !walk.far;
+      const float l = said == kUnknown ? rewritten(to_f32(row[x]), sl.how) : 0.f;
+      const double uq = said == kUnknown ? (double)__ldg(p.uniform + r) * (q_row == nullptr ? 1.0 : (double)__ldg(q_row + x)) : 0.0;
+      if (plain && said == kUnknown) {
+        const double w = weight(l, mass.s) * top_units(walk, t), bar = uq * walk.total;
+        plain = fabs(w - bar) > sum_margin(walk, t, p.vocab);
+        if (plain && bar < w) {
           cluster_sync();  // the others may still read this CTA's slots
           continue;
         }
       }
-      if (!done && plain && !last) done = draw_rest(sl, walk, t, q_row, q_row == nullptr ? x : -1, u, p.tokens + req, sh);
+      if (plain) done = last ? draw_all(sl, walk, t, u, p.tokens + req, sh) : draw_rest(sl, walk, t, q_row, q_row == nullptr ? x : -1, u, p.tokens + req, sh);
       if (!done) {
+        mass.kept = settled_border(sl, mass.s, top_p, cut ? in_fixed_units(walk, mass.s) : -1.0, near, sh, mine);
+        if (said == kUnknown && !plain) {
+          const u64 w = mass.kept.holds(l, x) ? raw_weight(l, mass.s, sh.table) - kRaw : 0;
+          if (uq < (double)w / (double)mass.kept.total) {
+            cluster_sync();
+            continue;
+          }
+        }
         mass.inv_z = 1.0 / (double)mass.kept.total;
-        mass.residual = !last && !plain;  // (plain: nothing is left above the draft's distribution, the target's own is drawn from)
+        mass.residual = !last;
         mass.minus = last ? nullptr : q_row;
         mass.one_hot = q_row == nullptr ? x : -1;
-        if (!draw(sl, mass, near, u, last && !cut, mine, 31, p.tokens + req, sh) && mass.residual) {
+        if (!draw(sl, mass, near, u, last && !cut, mine, 31, p.tokens + req, sh) && mass.residual) {  // nothing is left above the draft's
           mass.residual = false;
           draw(sl, mass, near, u, false, 0, 34, p.tokens + req, sh);
         }

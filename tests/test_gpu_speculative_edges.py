@@ -141,6 +141,42 @@ def test_masked_entries_have_no_weight_at_any_temperature(dtype, temperature, hi
                 assert (_last_row(row, rows, temperature, top_p, u) == want).all()
 
 
+# ---- verification --------------------------------------------------------------------------------------------------------------
+def _verify_one_draft(row, requests, draft, q, u, u_last, temperature=0.7, top_p=1.0):
+    """Requests with one draft each, all alike: (accepted, next token) of every one."""
+    x = row.to(DEV).expand(2 * requests, -1).contiguous()
+    tokens = torch.full((2 * requests,), draft, dtype=torch.int32, device=DEV)
+    uniform = torch.tensor([u, u_last], dtype=torch.float32, device=DEV).repeat(requests)
+    indptr = torch.arange(0, 2 * requests + 1, 2, dtype=torch.int32, device=DEV)
+    n, tok = dk.verify_draft(x, tokens, indptr, uniform, _full(requests, temperature), _full(requests, top_p),
+                             None if q is None else q.to(DEV).expand(2 * requests, -1).contiguous())
+    return n.cpu(), tok.cpu()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,value", [(1000, 5.0), (1024, 0.3125), (5000, -3.75), (32000, 7.5)])
+@pytest.mark.parametrize("requests", [1, 40, 299, 700])
+def test_residual_draws_at_exact_borders_do_not_depend_on_the_launch(dtype, vocab, value, requests):
+    """The target is flat, the draft has all its mass on the first half: what is left is the second half, evenly."""
+    q = torch.zeros(vocab)
+    q[: vocab // 2] = 2 / vocab
+    row = torch.full((vocab,), value, dtype=dtype)
+    for u in (0.125, 0.25, 0.5, 0.75):
+        n, tok = _verify_one_draft(row, requests, 3, q, 0.9, u)
+        assert (n == 0).all() and (tok == vocab // 2 + int(u * (vocab // 2))).all()
+
+
+@pytest.mark.parametrize("requests", [1, 40, 700])
+def test_a_draft_whose_test_meets_equality_is_rejected(requests):
+    """u q = p exactly is not u q < p; one step below it is accepted. The same under a nucleus that keeps every token."""
+    row, q = torch.full((4096,), 0.3125), torch.zeros(4096)
+    q[: 2048] = 2.0**-11
+    for top_p in (1.0, 1 - 2.0**-24):
+        for value in (row, row.to(torch.bfloat16)):
+            assert (_verify_one_draft(value, requests, 3, q, 0.5, 0.5, top_p=top_p)[0] == 0).all()
+            assert (_verify_one_draft(value, requests, 3, q, 0.5 - 2.0**-25, 0.5, top_p=top_p)[0] == 1).all()
+
+
 # ---- calls that are refused on the device --------------------------------------------------------------------------------------
 def test_verify_draft_with_an_indptr_that_is_not_monotone_reads_nothing_it_should_not():
     """Requests whose rows belong to no request of the search, drafts that are no tokens, and scratch full of old verdicts: the bad

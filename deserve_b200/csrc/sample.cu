@@ -1687,6 +1687,7 @@ __device__ int quick_walk(const Slice<T, NT, false>& sl, float temperature, floa
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (__any_sync(0xffffffffu, (z >> 32) != 0) || best == INFINITY || best < -1e38f) return -1;
+  if (((double)best - (double)lx) * c > 44.0) return -1;  // may be below what can be drawn: its fixed-point weight says
   const double wx = exp2(fmax((double)lx * c - e, -2000.0));
   double least = total, most = total;  // bounds of Z
   if (cut) {

@@ -177,6 +177,18 @@ def test_a_draft_whose_test_meets_equality_is_rejected(requests):
             assert (_verify_one_draft(value, requests, 3, q, 0.5 - 2.0**-25, 0.5, top_p=top_p)[0] == 1).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("top_p", [0.9, 1.0])
+def test_a_draft_that_cannot_be_drawn_is_rejected_by_every_random_number(dtype, top_p):
+    row = torch.full((900,), -40.0, dtype=dtype)
+    row[5] = row[700] = 0.0
+    for draft, accepted in ((8, 0), (700, 1), (5, 1)):
+        n, tok = _verify_one_draft(row, 2, draft, None, 0.0, 0.75, temperature=1.0, top_p=top_p)
+        assert (n == accepted).all() and (tok == 700).all()
+        n, tok = _verify_one_draft(row, 2, draft, torch.zeros(900), 0.3, 0.75, temperature=1.0, top_p=top_p)  # q(x) = 0
+        assert (n == accepted).all() and (tok == 700).all()
+
+
 # ---- calls that are refused on the device --------------------------------------------------------------------------------------
 def test_verify_draft_with_an_indptr_that_is_not_monotone_reads_nothing_it_should_not():
     """Requests whose rows belong to no request of the search, drafts that are no tokens, and scratch full of old verdicts: the bad

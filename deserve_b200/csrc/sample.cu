@@ -1151,6 +1151,7 @@ __device__ Kept find_kept(const Slice<T, NT, kShared>& sl, const RowScale& s, fl
   int put = 0;  // the cluster's entries, should they be few
   if (lane == 0 && near.n > 0) put = atomicAdd(&sh.n_list, near.n);
   put = __shfl_sync(0xffffffffu, put, 0);
+  __syncwarp();  // the entries were written by other lanes, and a shuffle orders no memory
   for (int i = lane; i < min(near.n, near.cap); i += 32)
     if (put + i < kList) sh.list[put + i] = rank_key<T>(list[i].l, list[i].i);
   Slot whole = cluster_total<NT>(warp_sum(sum), warp_sum(whole_mass), (u64)near.n + (near.n > near.cap ? 1ull << 40 : 0), sh, 2, before);

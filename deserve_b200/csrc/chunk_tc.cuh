@@ -330,7 +330,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
     int c0 = 0, c1 = D / 32;
     uint32_t oa = o_addr, ob = 0;
     if (dual) {
-      asm volatile("bar.sync %0, 128;\n" ::"r"(2 + x) : "memory");  // `poison` of the whole group
+      // `poison` of both groups: a value that the other one cleared first is not found by this one. (Parts without a hidden
+      // region look for none.)
+      if (hidden < it.tok_end) asm volatile("bar.sync 1, 256;\n" ::: "memory");
     } else {
       float2* ml = reinterpret_cast<float2*>(smem + (q_smem - base));  // q is no longer read
       ml[x * 128 + row] = make_float2(m_used, l);

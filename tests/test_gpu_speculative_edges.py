@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import deserve_b200 as dk
-from deserve_b200 import _lib
+from deserve_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -213,3 +213,41 @@ def test_verify_draft_with_an_indptr_that_is_not_monotone_reads_nothing_it_shoul
         assert (scratch <= 2).all() and following[1] == -1
         assert accepted.tolist() == [1, 0, 1]  # the last request gets to row 4, which the search gives to the first one
         assert ((following[[0, 2]] >= 0) & (following[[0, 2]] < vocab)).all()
+
+
+# ---- chunk attention -----------------------------------------------------------------------------------------------------------
+def _chunk_batch(seed, lens, new, hq, hkv, d, ps, dtype):
+    """Requests over a shuffled pool: (wrapper, q, pages, page ids, first new row of every request)."""
+    g = torch.Generator().manual_seed(seed)
+    n_pages = [-(-n // ps) for n in lens]
+    qo, kvp = (np.concatenate([[0], np.cumsum(v)]).astype(np.int32) for v in (new, n_pages))
+    ids = torch.randperm(int(kvp[-1]) + 3, generator=g)[: int(kvp[-1])].to(torch.int32).to(DEV)
+    pages = torch.randn(int(kvp[-1]) + 3, 2, ps, hkv, d, generator=g).to(dtype).to(DEV)
+    q = torch.randn(int(qo[-1]), hq, d, generator=g).to(dtype).to(DEV)
+    last = torch.tensor([(n - 1) % ps + 1 for n in lens], dtype=torch.int32, device=DEV)
+    w = ops.BatchChunkWithPagedKVCacheWrapper(torch.empty(64 << 20, dtype=torch.uint8, device=DEV))
+    w.begin_forward(torch.from_numpy(qo).to(DEV), torch.from_numpy(kvp).to(DEV), ids, last, hq, hkv, d, ps, dtype,
+                    qo_indptr_host=qo, kv_indptr_host=kvp)
+    return w, q, pages, ids, qo, kvp
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [INF, float("nan")])
+@pytest.mark.parametrize("at", [0, 9, 31, 32, 50, 62])
+def test_chunk_attention_with_two_q_tiles_finds_values_that_are_no_numbers(dtype, d, bad, at):
+    """64 new tokens of 4 heads each, two q tiles that share their V: a new token's V that is no number reaches the rows from its own
+    on, in both tiles, and no earlier one."""
+    lens, new = [64, 700, 1290], [64, 64, 64]
+    w, q, pages, ids, qo, kvp = _chunk_batch(at, lens, new, 8, 2, d, 16, dtype)
+    clean = w.forward(q, pages)
+    for i, n in enumerate(lens):
+        t = n - 64 + at
+        pages[int(ids[kvp[i] + t // 16]), 1, t % 16, :, 5] = bad
+    for _ in range(10):
+        got = w.forward(q, pages)
+        for i in range(len(lens)):
+            a = int(qo[i])
+            assert torch.equal(got[a: a + at], clean[a: a + at])
+            assert not torch.isfinite(got[a + at: a + 64, :, 5]).any()
+            assert torch.isfinite(got[a + at: a + 64, :, :5]).all() and torch.isfinite(got[a + at: a + 64, :, 6:]).all()

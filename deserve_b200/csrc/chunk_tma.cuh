@@ -13,47 +13,19 @@
 
 #include <cuda.h>
 
+#include "tcgen05.cuh"
+
 namespace dsv {
 namespace chunk_tma {
+
+using namespace ptx;
 
 constexpr int kConsumerWarps = 8;
 constexpr int kConsumerThreads = kConsumerWarps * 32;
 constexpr int kThreads = kConsumerThreads + 32;
 constexpr int kStages = 3;
-constexpr int kSpinLimit = 1 << 21;
 constexpr float kGrow = 8.f;  // log2 units
 
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
-}
-// Bounded wait: false (and a status code) when the phase never completes.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* status) {
-  for (int i = 0; i < kSpinLimit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (i > (1 << 16)) __nanosleep(64);  // back off only when the wait is clearly not a normal one
-  }
-  record_status(status, ST_WAIT_TIMEOUT);
-  return false;
-}
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
-                                            int c3, int c4) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n" ::
-          "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
-      : "memory");
-}
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
@@ -79,18 +51,6 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <>
 __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
@@ -105,11 +65,6 @@ template <typename T>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   return ((w & E) == E ? 0x0000ffffu : 0u) | (((w >> 16) & E) == E ? 0xffff0000u : 0u);
-}
-__device__ __forceinline__ float ex2(float x) {  // 2^x on the special-function unit; ex2(-inf) = 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
 }
 
 struct Split {
@@ -163,7 +118,8 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
   if (warp == kConsumerWarps) {
     const int32_t* idx = p.kv_indices + it.ip0;
     const int n_boxes = ng * bpg;  // boxes per tile and per K/V half (<= 16)
-    for (int tile = 0; tile < n_tiles; ++tile) {
+    int tile = 0;
+    for (; tile < n_tiles; ++tile) {
       const int s = tile % kStages;
       const int tok0 = it.tok_begin + tile * ttok + lane * bt;  // first token of this lane's box
       const bool mine = lane < n_boxes && tok0 < it.tok_end;
@@ -176,7 +132,7 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
         }
       }
       if (tile >= kStages) {
-        if (!mbar_wait(bar_empty + 8 * s, ((tile / kStages) - 1) & 1, p.status)) return;
+        if (!warp_wait(bar_empty + 8 * s, ((tile / kStages) - 1) & 1, p.status)) break;
       }
       const unsigned live = __ballot_sync(0xffffffffu, mine);
       if (lane == 0) mbar_expect_tx(bar_full + 8 * s, (uint32_t)(__popc(live) * 2 * box_bytes));
@@ -188,6 +144,8 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
         tma_load_5d(dst + HALF, &tmap, bar_full + 8 * s, 0, in_page, kv_group * hb, 0, 2 * page + 1);
       }
     }
+    // the CTA does not end before its copies, whatever became of a consumer's wait
+    for (int k = max(tile - kStages, 0); k < tile; ++k) warp_wait(bar_full + 8 * (k % kStages), (k / kStages) & 1, p.status);
     return;
   }
 
@@ -363,8 +321,8 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
   bool ok = true;
   for (int tile = 0; tile < n_tiles; ++tile) {
     const int s = tile % kStages;
-    if (!mbar_wait(bar_full + 8 * s, (tile / kStages) & 1, p.status)) {
-      ok = false;
+    if (!warp_wait(bar_full + 8 * s, (tile / kStages) & 1, p.status)) {
+      ok = false;  // (still passes the barriers below: warps whose waits succeeded meet there)
       break;
     }
     const int t0 = it.tok_begin + tile * ttok + 16 * sub;  // this warp's group of the stage
@@ -372,8 +330,6 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
     __syncwarp();
     if (lane == 0) mbar_arrive(bar_empty + 8 * s);  // this warp is done with the stage
   }
-  if (!ok) return;
-
   l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
   l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
   l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
@@ -396,6 +352,7 @@ chunk_tma_kernel(const __grid_constant__ CUtensorMap tmap, const ChunkParams p, 
   }
   asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumerThreads) : "memory");
 
+  if (!ok) return;
   // four consecutive elements of a row per thread
   const int quads = D / 4;
   for (int x = tid; x < hb * it.n_rows * quads; x += kConsumerThreads) {

@@ -57,6 +57,10 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* st
   record_status(status, ST_WAIT_TIMEOUT);
   return false;
 }
+// The same wait with one answer for the warp, so that its lanes stay together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* status) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
+}
 
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
                                             int c3, int c4) {
@@ -125,7 +129,8 @@ decode_tma_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p
     const int32_t* idx = p.kv_indices + ip0;
     const int n_boxes = wph * bpg;          // boxes per tile and per K/V half (<= 16)
     const int sub = lane / bpg, b = lane - sub * bpg;
-    for (int tile = 0; tile < n_tiles; ++tile) {
+    int tile = 0;
+    for (; tile < n_tiles; ++tile) {
       const int s = tile % kStages;
       const int tok0 = tok_begin + tile * ttok + 16 * sub + b * bt;  // first token of this lane's box
       const bool mine = lane < n_boxes && tok0 < tok_end;
@@ -138,7 +143,7 @@ decode_tma_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p
         }
       }
       if (tile >= kStages) {
-        if (!mbar_wait(bar_empty + 8 * s, ((tile / kStages) - 1) & 1, p.status)) return;
+        if (!warp_wait(bar_empty + 8 * s, ((tile / kStages) - 1) & 1, p.status)) break;
       }
       const unsigned live = __ballot_sync(0xffffffffu, mine);
       if (lane == 0) mbar_expect_tx(bar_full + 8 * s, (uint32_t)(__popc(live) * 2 * box_bytes));
@@ -150,6 +155,8 @@ decode_tma_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p
         tma_load_5d(dst + HALF, &tmap, bar_full + 8 * s, 0, in_page, kv_group * hb, 0, 2 * page + 1);
       }
     }
+    // the CTA does not end before its copies, whatever became of a consumer's wait
+    for (int k = max(tile - kStages, 0); k < tile; ++k) warp_wait(bar_full + 8 * (k % kStages), (k / kStages) & 1, p.status);
     return;
   }
 
@@ -196,10 +203,9 @@ decode_tma_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p
   bool ok = true;
   for (int tile = 0; tile < n_tiles; ++tile) {
     const int s = tile % kStages;
-    if (!mbar_wait(bar_full + 8 * s, (tile / kStages) & 1, p.status)) {
-      ok = false;
-      break;
-    }
+    // A lane whose wait gave up goes on without waiting and writes nothing in the end: it stays with its warp, whose other
+    // lanes may have been luckier, and passes the barriers below, where the other warps stand. (A vote here took 1 % of the time.)
+    ok = ok && mbar_wait(bar_full + 8 * s, (tile / kStages) & 1, p.status);
     const int wt0 = tok_begin + tile * ttok + 16 * sub;
     if (wt0 < tok_end) {  // warp-uniform
       const uint32_t kbase = smem_base + s * STAGE + group_off;
@@ -284,8 +290,6 @@ decode_tma_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p
     __syncwarp();
     if (lane == 0) mbar_arrive(bar_empty + 8 * s);  // this warp is done with the stage
   }
-  if (!ok) return;
-
   l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
   l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
   if (HI) {
@@ -314,6 +318,7 @@ decode_tma_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p
   }
   asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumerThreads) : "memory");
 
+  if (!ok) return;
   const int slot = item.w;
   for (int x = tid; x < hb * G * D; x += kConsumerThreads) {
     const int d = x % D, r = (x / D) % G, hl = x / (D * G);

@@ -85,6 +85,8 @@ _SIGNATURES = {
                                   c_float, c_int, c_void_p]),
     "dsv_chunk_plan": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64,
                                _p64, _p64]),
+    "dsv_chunk_plan_within": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p,
+                                      c_int64, _p64, _p64]),
     "dsv_paged_chunk_attention": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                                           c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                           c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p]),

@@ -373,15 +373,9 @@ cudaError_t launch_simple_d(const ChunkParams& p, int n_items, int tile_tokens, 
   return launch_simple<T, 256>(p, n_items, tile_tokens, st);
 }
 
-}  // namespace
-}  // namespace dsv
-
-extern "C" {
-
-int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int batch, int n_q_heads,
-                   int n_kv_heads, int head_dim, int page_size, int dtype, int sm_count, int32_t* plan_host,
-                   int64_t plan_capacity_i32, int64_t* plan_used_i32, int64_t* workspace_bytes) {
-  using namespace dsv;
+int chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int batch, int n_q_heads, int n_kv_heads, int head_dim,
+               int page_size, int dtype, int sm_count, int64_t workspace_capacity, int32_t* plan_host, int64_t plan_capacity_i32,
+               int64_t* plan_used_i32, int64_t* workspace_bytes) {
   DSV_REQUIRE(qo_indptr_host && kv_indptr_host && plan_host && plan_used_i32 && workspace_bytes,
               "chunk_plan: null pointer argument");
   DSV_REQUIRE(batch >= 0, "chunk_plan: negative batch");
@@ -443,18 +437,22 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
     const int c = (int)std::min<int64_t>(std::max<int64_t>(c64, min_chunk), std::max(min_chunk, max_pages));
     const int64_t k = count_items(c);
     if (k > most_items) return;
+    int64_t rows = 0, merged = 0;  // partial states, and the q rows that they belong to
+    if (k > (int64_t)tiles.size()) {
+      for (const Tile& t : tiles) {
+        const int64_t parts = std::max(1, (t.pages + c - 1) / c);
+        if (parts > 1) { rows += parts * t.nq; merged += t.nq; }
+      }
+      // a split that the caller has no room for is none (whole tiles need no workspace)
+      if (rows > workspace_capacity / ((int64_t)n_q_heads * (head_dim + 2) * (int64_t)sizeof(float)) ||
+          kPlanHeader + kItemInts * k + 4 * merged > plan_capacity_i32)
+        return;
+    }
     const int64_t ctas = k * ctas_per_item;
     const double longest = std::min(c, max_pages) * page_cost + overhead;
     double cost = ctas <= slots ? longest
                                 : std::max(longest, ((double)total_pages * ctas_per_item * page_cost + (double)ctas * overhead) / (double)slots) + 0.5 * longest;
-    if (k > (int64_t)tiles.size()) {
-      int64_t rows = 0;
-      for (const Tile& t : tiles) {
-        const int64_t parts = std::max(1, (t.pages + c - 1) / c);
-        if (parts > 1) rows += parts * t.nq;
-      }
-      cost += merge_cost + 2.0 * (double)rows * n_q_heads * (head_dim + 2) * sizeof(float) / sm_count;
-    }
+    if (rows > 0) cost += merge_cost + 2.0 * (double)rows * n_q_heads * (head_dim + 2) * sizeof(float) / sm_count;
     if (best < 0.0 || cost < best) { best = cost; chunk = c; }
   };
   if (!tiles.empty()) {
@@ -522,6 +520,28 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
     it[10] = it[11] = 0;
   }
   return DSV_OK;
+}
+
+}  // namespace
+}  // namespace dsv
+
+extern "C" {
+
+int dsv_chunk_plan_within(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int batch, int n_q_heads,
+                          int n_kv_heads, int head_dim, int page_size, int dtype, int sm_count,
+                          int64_t workspace_capacity, int32_t* plan_host, int64_t plan_capacity_i32,
+                          int64_t* plan_used_i32, int64_t* workspace_bytes) {
+  using namespace dsv;
+  DSV_REQUIRE(workspace_capacity >= 0, "chunk_plan: negative workspace_capacity");
+  return chunk_plan(qo_indptr_host, kv_indptr_host, batch, n_q_heads, n_kv_heads, head_dim, page_size, dtype, sm_count, workspace_capacity,
+                    plan_host, plan_capacity_i32, plan_used_i32, workspace_bytes);
+}
+
+int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int batch, int n_q_heads,
+                   int n_kv_heads, int head_dim, int page_size, int dtype, int sm_count, int32_t* plan_host,
+                   int64_t plan_capacity_i32, int64_t* plan_used_i32, int64_t* workspace_bytes) {
+  return dsv_chunk_plan_within(qo_indptr_host, kv_indptr_host, batch, n_q_heads, n_kv_heads, head_dim, page_size, dtype, sm_count,
+                               INT64_MAX, plan_host, plan_capacity_i32, plan_used_i32, workspace_bytes);
 }
 
 int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t* qo_indptr, const void* pages_layer,

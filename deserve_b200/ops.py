@@ -421,17 +421,18 @@ def chunk_plan_capacity(nnz: int, batch: int, sm_count: int = 148) -> int:
 
 def make_chunk_plan(qo_indptr_host: np.ndarray, kv_indptr_host: np.ndarray, n_q_heads: int, n_kv_heads: int,
                     head_dim: int, page_size: int, dtype: torch.dtype, sm_count: int,
-                    plan_out: np.ndarray) -> tuple[int, int]:
+                    plan_out: np.ndarray, workspace_bytes: int | None = None) -> tuple[int, int]:
     """Fill plan_out (int32) with the (request, q tile, page range) work items; returns (int32
-    entries used, device workspace bytes needed)."""
+    entries used, device workspace bytes needed). workspace_bytes: what there is for partial states; the plan
+    splits no further than they fit (None: as far as it likes)."""
     qo = np.ascontiguousarray(qo_indptr_host, dtype=np.int32)
     kv = np.ascontiguousarray(kv_indptr_host, dtype=np.int32)
     if len(qo) != len(kv) or len(qo) == 0:
         raise ValueError("chunk_plan: qo_indptr and kv_indptr must both have batch + 1 entries")
     used, ws = ctypes.c_int64(), ctypes.c_int64()
-    _lib.check(_lib.lib.dsv_chunk_plan(
+    _lib.check(_lib.lib.dsv_chunk_plan_within(
         qo.ctypes.data, kv.ctypes.data, len(qo) - 1, n_q_heads, n_kv_heads, head_dim, page_size, _lib.dtype_code(dtype),
-        sm_count, plan_out.ctypes.data, plan_out.size, ctypes.byref(used), ctypes.byref(ws)))
+        sm_count, (1 << 63) - 1 if workspace_bytes is None else workspace_bytes, plan_out.ctypes.data, plan_out.size, ctypes.byref(used), ctypes.byref(ws)))
     return used.value, ws.value
 
 
@@ -486,7 +487,7 @@ class BatchChunkWithPagedKVCacheWrapper:
     """begin_forward / forward / end_forward object of a step that feeds a few tokens per request (the
     last token and its drafts), beside the decode and prefill wrappers. `workspace_buffer` is a uint8
     device tensor owned by the caller: its head holds the device copy of the plan, the rest the split-KV
-    partial states. Two wrappers (or two captured graphs) that may run at the same time need two buffers."""
+    partial states (a batch is split no further than they fit). Two wrappers (or two captured graphs) that may run at the same time need two buffers."""
 
     _PLAN_BYTES = 1 << 20
 
@@ -520,14 +521,10 @@ class BatchChunkWithPagedKVCacheWrapper:
                     _i32_dev(paged_kv_indptr, "kv_indptr").data_ptr(), _i32_dev(paged_kv_last_page_len, "kv_last_page_len").data_ptr())
         cap = chunk_plan_capacity(int(qo_indptr_host[-1]), len(qo_indptr_host) - 1, self._sm_count)
         pinned, slot = _pinned_ring("chunk_plan").take(cap)
-        plan = pinned.numpy()
-        used, ws_bytes = make_chunk_plan(qo_indptr_host, kv_indptr_host, num_qo_heads, num_kv_heads, head_dim, page_size,
-                                         data_type if isinstance(data_type, torch.dtype) else torch.float16,
-                                         self._sm_count, plan)
-        if used * 4 > self._PLAN_BYTES:
-            raise _lib.DeserveKVError(f"chunk plan for {int(qo_indptr_host[-1])} tokens does not fit the workspace head")
-        if ws_bytes > self._ws.numel() - self._PLAN_BYTES:
-            raise _lib.DeserveKVError(f"workspace_buffer too small: split-KV partials need {ws_bytes} bytes")
+        plan = pinned.numpy()[: self._PLAN_BYTES // 4]  # what the workspace's head holds of it
+        used, _ = make_chunk_plan(qo_indptr_host, kv_indptr_host, num_qo_heads, num_kv_heads, head_dim, page_size,
+                                  data_type if isinstance(data_type, torch.dtype) else torch.float16,
+                                  self._sm_count, plan, self._ws.numel() - self._PLAN_BYTES)
         self._ws[: used * 4].view(torch.int32).copy_(pinned[:used], non_blocking=True)
         _pinned_ring("chunk_plan").done(slot)
         _COUNTERS["h2d_bytes"] += used * 4

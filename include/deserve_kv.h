@@ -280,6 +280,16 @@ int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
                    int64_t* plan_used_i32, int64_t* workspace_bytes);
 
 /*
+ * dsv_chunk_plan for a caller whose workspace for partial states holds workspace_capacity
+ * bytes: only splits whose states fit there, and whose plan fits plan_capacity_i32, are
+ * compared. Unsplit tiles need no workspace, so any capacity (0 too) has a plan.
+ */
+int dsv_chunk_plan_within(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int batch,
+                          int n_q_heads, int n_kv_heads, int head_dim, int page_size, int dtype,
+                          int sm_count, int64_t workspace_capacity, int32_t* plan_host,
+                          int64_t plan_capacity_i32, int64_t* plan_used_i32, int64_t* workspace_bytes);
+
+/*
  * Causal attention of a few new tokens per request (drafted tokens that are verified, a
  * short continuation) over one layer's pages, the kv axis split over the GPU. q row j (of
  * n_i) of request i sees kv positions <= len_i - n_i + j. It computes what

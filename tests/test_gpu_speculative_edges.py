@@ -251,3 +251,19 @@ def test_chunk_attention_with_two_q_tiles_finds_values_that_are_no_numbers(dtype
             assert torch.equal(got[a: a + at], clean[a: a + at])
             assert not torch.isfinite(got[a + at: a + 64, :, 5]).any()
             assert torch.isfinite(got[a + at: a + 64, :, :5]).all() and torch.isfinite(got[a + at: a + 64, :, 6:]).all()
+
+
+@pytest.mark.parametrize("dtype,hq", [(torch.float32, 8), (torch.bfloat16, 8), (torch.bfloat16, 32)])
+def test_chunk_attention_in_the_smallest_workspace(dtype, hq):
+    """2 MiB: the plan of a batch that would be cut finer elsewhere; the same outputs up to rounding (each is within eps / 2 of the value
+    plus eps / 2 of sum p |v| <= max |v| of the exact one, test_gpu_speculative.py)."""
+    w, q, pages, ids, qo, kvp = _chunk_batch(3, [40000, 30000], [16, 9], hq, 2, 128, 16, dtype)
+    want = w.forward(q, pages)
+    small = ops.BatchChunkWithPagedKVCacheWrapper(torch.empty(2 << 20, dtype=torch.uint8, device=DEV))
+    small.begin_forward(torch.from_numpy(qo).to(DEV), torch.from_numpy(kvp).to(DEV), ids,
+                        torch.tensor([16, 16], dtype=torch.int32, device=DEV), hq, 2, 128, 16, dtype, qo_indptr_host=qo,
+                        kv_indptr_host=kvp)
+    assert small._plan_host[10] < w._plan_host[10]
+    got = small.forward(q, pages)
+    eps = torch.finfo(dtype).eps if dtype != torch.float32 else 2.0**-17
+    assert ((got.float() - want.float()).abs() <= eps * (want.float().abs() + float(pages.abs().max()))).all()

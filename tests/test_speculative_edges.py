@@ -1,0 +1,51 @@
+"""The chunk planner and the engine's speculative bookkeeping at their edges. No GPU needed."""
+import numpy as np
+import pytest
+import torch
+
+import deserve_b200 as dk
+from deserve_b200 import _lib, ops
+
+
+def _plan(new, pages, hq=64, hkv=8, d=128, ps=16, dtype=torch.bfloat16, workspace_bytes=None, capacity=None):
+    qo, kv = (np.concatenate([[0], np.cumsum(v)]).astype(np.int32) for v in (new, pages))
+    plan = np.zeros(ops.chunk_plan_capacity(int(qo[-1]), len(new)) if capacity is None else capacity, dtype=np.int32)
+    used, ws = ops.make_chunk_plan(qo, kv, hq, hkv, d, ps, dtype, 148, plan, workspace_bytes)
+    return plan[:used], ws
+
+
+def _check_cover(plan, new, pages):
+    """Every (row, page) once: rows of an item see the pages [first, end) of their request."""
+    seen = [np.zeros((n, p), dtype=int) for n, p in zip(new, pages)]
+    for req, q0, nq, pb, pe, *_ in plan[16: 16 + 12 * plan[1]].reshape(-1, 12):
+        seen[req][q0: q0 + nq, pb:pe] += 1
+    for s, p in zip(seen, pages):
+        assert (s <= 1).all() and (s[-1] == 1).all()  # (pages behind a tile may be left out, the last row sees all)
+
+
+BIG = [([64] * 8, [131072 // 16] * 8), ([512] * 4, [2048] * 4), ([1024], [8192]), ([5], [4096]), ([3, 1, 40], [9000, 2, 600])]
+
+
+@pytest.mark.parametrize("new,pages", BIG)
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float32, 128), (torch.float16, 96)])
+@pytest.mark.parametrize("room", [127 << 20, 1 << 20, 5000, 0])
+def test_chunk_plan_splits_no_further_than_its_workspace(new, pages, dtype, d, room):
+    free, wanted = _plan(new, pages, dtype=dtype, d=d)
+    plan, ws = _plan(new, pages, dtype=dtype, d=d, workspace_bytes=room)
+    assert ws <= room and ws == plan[10] * 64 * (d + 2) * 4
+    _check_cover(plan, new, pages)
+    if wanted <= room:
+        assert np.array_equal(plan, free)
+
+
+def test_chunk_plan_splits_no_further_than_its_plan_holds():
+    new, pages = [40, 5], [4096, 3000]
+    free, _ = _plan(new, pages, dtype=torch.float32)
+    plan, ws = _plan(new, pages, dtype=torch.float32, workspace_bytes=0)
+    less, _ = _plan(new, pages, dtype=torch.float32, capacity=len(plan))  # unsplit tiles just fit
+    assert len(free) > len(plan) and ws == 0 and len(less) <= len(plan)
+    _check_cover(less, new, pages)
+    with pytest.raises(_lib.DeserveKVError, match="plan needs"):
+        _plan(new, pages, dtype=torch.float32, capacity=len(plan) - 1)
+    with pytest.raises(ValueError, match="workspace_capacity"):
+        _plan(new, pages, workspace_bytes=-1)

@@ -19,7 +19,7 @@ namespace {
 
 constexpr int32_t kChunkMagic = 0x44534331;  // "DSC1"
 // header: magic, items, merge rows, q tokens per tile, batch, offset of the items, offset of the merge
-// rows, q heads, kv heads, head_dim, partial rows, page size, dtype, nnz, kernel, most parts of a tile
+// rows, q heads, kv heads, head_dim, partial rows, page size, dtype, nnz, kernel (+ 4: some tile has many parts), entries of kv_indices
 constexpr int kPlanHeader = 16;
 // request, first q token, q tokens, first page | end page, partial row or -1, first q row, first entry of the page list |
 // pages of the request, first q token behind which the request's tokens lie (n_new - q0), 2 unused: all that a CTA needs but the last
@@ -335,7 +335,7 @@ int ilog2_exact(int x) {  // log2 of a power of two, -1 otherwise
   while ((1 << l) < x) ++l;
   return l;
 }
-enum : int { kSimple = 0, kMma = 1, kTc = 2 };  // kernel of a plan
+enum : int { kSimple = 0, kMma = 1, kTc = 2, kManyParts = 4 };  // kernel of a plan, and whether its merge takes eight warps a row
 // kv heads of a CTA of the mma.sync kernel
 int heads_per_cta(int n_kv_heads) {
   int hb = 8;
@@ -508,7 +508,7 @@ int chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int
   plan_host[4] = batch; plan_host[5] = kPlanHeader; plan_host[6] = (int32_t)(kPlanHeader + kItemInts * n_items);
   plan_host[7] = n_q_heads; plan_host[8] = n_kv_heads; plan_host[9] = head_dim; plan_host[10] = (int32_t)part_rows;
   plan_host[11] = page_size; plan_host[12] = dtype; plan_host[13] = batch > 0 ? qo_indptr_host[batch] : 0;
-  plan_host[14] = kind; plan_host[15] = (int32_t)most_parts;
+  plan_host[14] = kind + (most_parts > 8 ? kManyParts : 0); plan_host[15] = batch > 0 ? kv_indptr_host[batch] : 0;
   for (int64_t k = 0; k < n_items; ++k) {
     int32_t* it = plan_host + kPlanHeader + kItemInts * k;
     for (int j = 0; j < 6; ++j) it[j] = items[k].v[j];
@@ -594,7 +594,7 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
   cudaError_t e;
   const int ps_log2 = ilog2_exact(page_size);
   // a pool with gaps between its pages has no tensor map: the general kernel takes any plan
-  const int kind = page_stride == (int64_t)2 * page_size * n_kv_heads * head_dim ? plan_host[14] : kSimple;
+  const int kind = page_stride == (int64_t)2 * page_size * n_kv_heads * head_dim ? plan_host[14] & ~kManyParts : kSimple;
   DSV_REQUIRE(kind >= kSimple && kind <= kTc && (kind == kSimple || (ps_log2 >= 3 && dtype != DSV_F32 && (head_dim == 64 || head_dim == 128))),
               "chunk: corrupt plan");
   if (kind == kMma) {
@@ -621,7 +621,7 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
   if (merge_rows > 0) {
     const int4* rows = reinterpret_cast<const int4*>(plan_dev + plan_host[6]);
     const int units = merge_rows * n_q_heads;
-    const bool many = plan_host[15] > 8;
+    const bool many = (plan_host[14] & kManyParts) != 0;
     switch (dtype) {
       case DSV_F32: launch_merge<float>(rows, units, many, p, st); break;
       case DSV_F16: launch_merge<__half>(rows, units, many, p, st); break;

@@ -442,8 +442,9 @@ def paged_chunk_attention(q: torch.Tensor, qo_indptr: torch.Tensor, paged_kv_cac
                           out: torch.Tensor | None = None, sm_scale: float | None = None,
                           lse: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of a few new tokens per request over the paged cache, the kv axis split over the
-    GPU. Functional form: every buffer explicit. Rows behind the last request are left as they are; lse,
-    if given ([nnz, n_q_heads] fp32), receives the natural-log sum-exp of the scaled scores."""
+    GPU. Functional form: every buffer explicit; plan_host is what make_chunk_plan filled, plan_dev the entries it used, on the
+    device, and the plan has to be that of these qo_indptr and kv_indptr (the kernels read them from it). Rows behind the last
+    request are left as they are; lse, if given ([nnz, n_q_heads] fp32), receives the natural-log sum-exp of the scaled scores."""
     dev = _same_device("chunk attention", q, qo_indptr, paged_kv_cache, kv_indices, kv_indptr, kv_last_page_len, plan_dev,
                        workspace, out, lse)
     ps, hkv, d, page_stride = _pages_view(paged_kv_cache)
@@ -460,6 +461,12 @@ def paged_chunk_attention(q: torch.Tensor, qo_indptr: torch.Tensor, paged_kv_cac
         raise ValueError(f"chunk attention: lse must be a contiguous float32 tensor [{nnz}, {hq}]")
     if qo_indptr.shape[0] != batch + 1 or kv_indptr.shape[0] != batch + 1:
         raise ValueError("chunk attention: qo_indptr and kv_indptr must have batch + 1 entries")
+    if plan_host.dtype != np.int32 or plan_host.ndim != 1 or len(plan_host) < 16 or not plan_host.flags.c_contiguous:
+        raise ValueError("chunk attention: plan_host must be the int32 array that make_chunk_plan filled")
+    if kv_indices.shape[0] < int(plan_host[15]):
+        raise ValueError(f"chunk attention: {kv_indices.shape[0]} kv_indices, the plan covers {int(plan_host[15])}")
+    if plan_dev.numel() < int(plan_host[6]) + 4 * int(plan_host[2]):
+        raise ValueError(f"chunk attention: plan_dev holds {plan_dev.numel()} of the plan's {int(plan_host[6]) + 4 * int(plan_host[2])} entries")
     descriptors = (_i32_dev(qo_indptr, "qo_indptr").data_ptr(), _i32_dev(kv_indices, "kv_indices").data_ptr(),
                    _i32_dev(kv_indptr, "kv_indptr").data_ptr(), _i32_dev(kv_last_page_len, "kv_last_page_len").data_ptr())
     _launch_chunk(dev, q, qs, descriptors, paged_kv_cache, (ps, hkv, d, page_stride), out, os_, lse, plan_host,

@@ -300,7 +300,9 @@ int dsv_chunk_plan_within(const int32_t* qo_indptr_host, const int32_t* kv_indpt
  * qo_indptr[batch] are neither read nor written. out may not alias q. lse (optional, may
  * be NULL): [nnz, n_q_heads] natural-log sum-exp of the scaled scores. plan_host /
  * plan_dev: the same plan on the host (header) and on the device; workspace: device
- * scratch of the size that the plan reported. A replayed CUDA graph may change the
+ * scratch of the size that the plan reported. The row and page ranges of the requests are
+ * those of the plan: qo_indptr and kv_indptr must not be NULL but are not read, and
+ * kv_indices must hold the kv_indptr_host[batch] entries that were planned. A replayed CUDA graph may change the
  * contents of q, pages, kv_indices and kv_last_page_len, not the plan's page counts.
  */
 int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t* qo_indptr,

@@ -267,3 +267,31 @@ def test_chunk_attention_in_the_smallest_workspace(dtype, hq):
     got = small.forward(q, pages)
     eps = torch.finfo(dtype).eps if dtype != torch.float32 else 2.0**-17
     assert ((got.float() - want.float()).abs() <= eps * (want.float().abs() + float(pages.abs().max()))).all()
+
+
+@pytest.mark.parametrize("dtype,hq,lens,new", [(torch.bfloat16, 8, [5000, 33], [4, 3]), (torch.bfloat16, 8, [9000, 100], [40, 7]),
+                                               (torch.float32, 4, [3000, 1], [2, 1])])
+def test_functional_chunk_attention(dtype, hq, lens, new):
+    """Every buffer explicit: the outputs of the wrapper with the same plan; buffers that the plan outgrows are refused."""
+    hkv, d, ps = 2, 128, 16
+    w, q, pages, ids, qo, kvp = _chunk_batch(7, lens, new, hq, hkv, d, ps, dtype)
+    lse = torch.empty(q.shape[:2], device=DEV)
+    want = w.forward(q, pages, lse=lse)
+    plan = np.zeros(ops.chunk_plan_capacity(int(qo[-1]), len(new)), dtype=np.int32)
+    used, ws_bytes = ops.make_chunk_plan(qo, kvp, hq, hkv, d, ps, dtype, _lib.device_info()[0], plan, 63 << 20)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    last = i32([(n - 1) % ps + 1 for n in lens])
+    plan_dev, ws = torch.from_numpy(plan[:used]).to(DEV), torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=DEV)
+    out, got_lse = torch.empty_like(q), torch.empty_like(lse)
+    call = lambda **kw: dk.paged_chunk_attention(**{**dict(
+        q=q, qo_indptr=i32(qo), paged_kv_cache=pages, kv_indices=ids, kv_indptr=i32(kvp), kv_last_page_len=last, plan_host=plan,
+        plan_dev=plan_dev, workspace=ws, out=out, lse=got_lse), **kw})
+    assert call() is out and torch.equal(out, want) and torch.equal(got_lse, lse)
+    for kw, message in (({"kv_indices": ids[:-1]}, "kv_indices"), ({"plan_dev": plan_dev[:-1]}, "plan_dev"),
+                        ({"plan_host": plan.astype(np.int64)}, "plan_host"), ({"plan_host": plan[:8]}, "plan_host"),
+                        ({"out": out[:-1]}, "rows"), ({"lse": got_lse[:-1]}, "lse"), ({"kv_indptr": i32(kvp[:-1])}, "batch")):
+        with pytest.raises(ValueError, match=message):
+            call(**kw)
+    if ws_bytes:
+        with pytest.raises(_lib.DeserveKVError, match="workspace"):
+            call(workspace=None)

@@ -593,8 +593,9 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   const int ps_log2 = ilog2_exact(page_size);
-  // a pool with gaps between its pages has no tensor map: the general kernel takes any plan
-  const int kind = page_stride == (int64_t)2 * page_size * n_kv_heads * head_dim ? plan_host[14] & ~kManyParts : kSimple;
+  // a pool with gaps between its pages has no tensor map, and the tensor-core kernels scale a row's largest score, which has to stay
+  // its largest: the general kernel takes any plan and scales q
+  const int kind = page_stride == (int64_t)2 * page_size * n_kv_heads * head_dim && sm_scale > 0.f ? plan_host[14] & ~kManyParts : kSimple;
   DSV_REQUIRE(kind >= kSimple && kind <= kTc && (kind == kSimple || (ps_log2 >= 3 && dtype != DSV_F32 && (head_dim == 64 || head_dim == 128))),
               "chunk: corrupt plan");
   if (kind == kMma) {

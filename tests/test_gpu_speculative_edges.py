@@ -7,6 +7,7 @@ import torch
 
 import deserve_b200 as dk
 from deserve_b200 import _lib, ops
+from oracle import sampling as oracle
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -295,3 +296,20 @@ def test_functional_chunk_attention(dtype, hq, lens, new):
     if ws_bytes:
         with pytest.raises(_lib.DeserveKVError, match="workspace"):
             call(workspace=None)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[3, 1], [40, 17]])
+@pytest.mark.parametrize("scale", [0.0, -0.2, -3.0])
+def test_chunk_attention_with_a_scale_that_is_not_positive(dtype, new, scale):
+    """The definition holds for any scale. Tolerances as in test_gpu_speculative.py: a rounding of the result, one of each probability, fp32
+    scores of 128 products."""
+    w, q, pages, ids, qo, kvp = _chunk_batch(4, [900, 50], new, 8, 2, 128, 16, dtype)
+    lse = torch.empty(q.shape[:2], device=DEV)
+    out = w.forward(q, pages, sm_scale=scale, lse=lse)
+    want, want_lse, size, reach = oracle.chunk_attention(q, pages, qo, ids, kvp, [900, 50], scale)
+    eps = torch.finfo(dtype).eps if dtype != torch.float32 else 0.0
+    arith = 2 * 130 * 2.0**-24 * reach + 2.0**-18
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + size * (eps / 2 + arith[..., None])
+    assert ((out.double() - want).abs() <= tol).all()
+    assert ((lse.double() - want_lse).abs() <= arith + 2.0**-23 * want_lse.abs()).all()

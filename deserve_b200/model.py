@@ -68,7 +68,8 @@ class LlamaStage:
                  first: bool | None = None, last: bool | None = None, split_head: bool = False,
                  sample_seed: int | None = None):
         """sample_seed: requests with a temperature above 0 are sampled (temperature, top_p) with random
-        numbers of a generator of this seed; None: every request is greedy.
+        numbers of a generator of this seed; None: every request is greedy. Not with split_head, whose two
+        halves only exchange maxima.
         split_head: the output projection is cut in two halves of the vocabulary. The LAST stage
         applies the final norm, computes the logits of the lower half and their row maxima, and hands
         on the normed rows together with (max, argmax) of its half (`pack_partial`); the FIRST stage
@@ -77,6 +78,8 @@ class LlamaStage:
         the stage that owns the head (it reads 1 GB of output weights per microbatch step instead of
         2 GB) at the price of a 2 MiB instead of a 512-byte message on the link back to the first
         stage. The reference keeps the whole head on the last worker (layer_storage.py:219-253)."""
+        if split_head and sample_seed is not None:
+            raise ValueError("a split head is greedy: it has no sample_seed")
         self.model_args = args
         self.layer_begin, self.layer_end = layer_begin, layer_end
         self.need_tokenize = layer_begin == 0 if first is None else first

@@ -49,3 +49,14 @@ def test_chunk_plan_splits_no_further_than_its_plan_holds():
         _plan(new, pages, dtype=torch.float32, capacity=len(plan) - 1)
     with pytest.raises(ValueError, match="workspace_capacity"):
         _plan(new, pages, workspace_bytes=-1)
+
+
+# ---- stages and tasks ------------------------------------------------------------------------------------------------------------
+ARGS = dk.ModelArgs(dim=64, n_layers=2, n_heads=2, n_kv_heads=1, vocab_size=64, ffn_dim=64)
+
+
+def test_a_split_head_does_not_sample():
+    with pytest.raises(ValueError, match="split head is greedy"):
+        dk.LlamaStage(ARGS, 0, 2, "cpu", torch.float32, split_head=True, sample_seed=1)
+    assert dk.LlamaStage(ARGS, 0, 2, "cpu", torch.float32, sample_seed=1).generator is not None
+    assert dk.LlamaStage(ARGS, 0, 2, "cpu", torch.float32, split_head=True).generator is None

@@ -478,6 +478,8 @@ class BatchVerify(BatchExec):
     verify_ctx: Optional[FlashVerifyCtx] = None
 
     def prepare(self) -> None:
+        if getattr(self.layer_storage, "split_head", False):
+            raise ValueError("drafts are verified against whole rows of logits: a split head has none")
         for t in self.task_datas:
             if not t.is_prefill():
                 raise ValueError(f"task {t.task_id}: drafts are verified behind the whole prompt ({t.start_pos} of {t.initial_seqlen} "

@@ -60,3 +60,14 @@ def test_a_split_head_does_not_sample():
         dk.LlamaStage(ARGS, 0, 2, "cpu", torch.float32, split_head=True, sample_seed=1)
     assert dk.LlamaStage(ARGS, 0, 2, "cpu", torch.float32, sample_seed=1).generator is not None
     assert dk.LlamaStage(ARGS, 0, 2, "cpu", torch.float32, split_head=True).generator is None
+
+
+@pytest.mark.parametrize("layers", [(0, 1), (1, 2), (0, 2)])
+def test_a_split_head_does_not_verify(layers):
+    """Refused before the caches grow."""
+    stage = dk.LlamaStage(ARGS, *layers, "cpu", torch.float32, split_head=True)
+    task = dk.TaskData.empty("a", 0)
+    task.init(3)
+    batch = dk.BatchVerify(torch.zeros(3, dtype=torch.int32), stage, [task], [None])
+    with pytest.raises(ValueError, match="split head"):
+        batch.prepare()

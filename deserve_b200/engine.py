@@ -576,13 +576,15 @@ class MicroBatchProcessor:
 
     def commit(self, task_ids: list, accepted: list) -> list:
         """End of a speculative step: the tasks move on by their accepted drafts and the token drawn behind them. Returns the
-        tasks that are done by their token or length limits."""
+        tasks that are done by their token or length limits. A step may bring more tokens than a limit leaves: the task then
+        moves by as many as plain decoding would have made, the first of (accepted drafts, drawn token); start_pos tells."""
         done = []
         for task_id, n in zip(task_ids, accepted):
             task = self.task_data_manager.get(task_id)
-            task.step_verified(int(n))
             sp = task.sampling_params
-            sp.max_new_tokens -= int(n) + 1
+            n = max(0, min(int(n), sp.max_new_tokens - 1, sp.max_seq_len - task.start_pos - 1))
+            task.step_verified(n)
+            sp.max_new_tokens -= n + 1
             if sp.max_new_tokens <= 0 or task.start_pos >= sp.max_seq_len:
                 done.append(task_id)
         return done

@@ -71,3 +71,33 @@ def test_a_split_head_does_not_verify(layers):
     batch = dk.BatchVerify(torch.zeros(3, dtype=torch.int32), stage, [task], [None])
     with pytest.raises(ValueError, match="split head"):
         batch.prepare()
+
+
+@pytest.mark.parametrize("fed,accepted,max_new,max_len,start,moved,left", [
+    (5, 4, 100, 1000, 50, 5, 95),   # no limit near
+    (5, 4, 5, 1000, 50, 5, 0),      # the limit met exactly
+    (5, 4, 3, 1000, 50, 3, 0),      # two tokens too many
+    (5, 4, 1, 1000, 50, 1, 0),
+    (5, 2, 100, 52, 50, 2, 98),     # the length limit
+    (5, 4, 100, 51, 50, 1, 99),
+    (1, 0, 1, 1000, 50, 1, 0),      # no drafts
+])
+def test_commit_stops_at_the_limits_of_plain_decoding(fed, accepted, max_new, max_len, start, moved, left):
+    plain = dk.TaskData.empty("p", start, dk.SamplingParams(max_new_tokens=max_new, max_seq_len=max_len))
+    plain.start_pos, steps = start, 0
+    while steps < accepted + 1:  # token by token, as LlamaStage.sample counts
+        plain.init(1)
+        plain.step()
+        plain.sampling_params.max_new_tokens -= 1
+        steps += 1
+        if plain.sampling_params.max_new_tokens <= 0 or plain.start_pos >= max_len:
+            break
+    proc = dk.MicroBatchProcessor.__new__(dk.MicroBatchProcessor)
+    proc.task_data_manager = dk.TaskManager(16, 16)
+    task = dk.TaskData.empty("a", start, dk.SamplingParams(max_new_tokens=max_new, max_seq_len=max_len))
+    proc.task_data_manager.add(task)
+    task.start_pos = start
+    task.init(fed)
+    done = proc.commit(["a"], [accepted])
+    assert (task.start_pos, task.sampling_params.max_new_tokens) == (plain.start_pos, plain.sampling_params.max_new_tokens) == (start + moved, left)
+    assert done == (["a"] if left == 0 or start + moved >= max_len else [])

@@ -405,7 +405,8 @@ int chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int
   for (int i = 0; i < batch; ++i) {
     const int n = qo_indptr_host[i + 1] - qo_indptr_host[i], np = kv_indptr_host[i + 1] - kv_indptr_host[i];
     DSV_REQUIRE(n >= 0 && np >= 0, "chunk_plan: indptr not monotone at %d", i);
-    DSV_REQUIRE((int64_t)np * page_size < (1ll << 31), "chunk_plan: request %d is longer than 2^31 tokens", i);
+    // (positions are 32-bit in the kernels, which step past the end by up to a tile of 128 and a lane's box)
+    DSV_REQUIRE((int64_t)np * page_size <= (1ll << 31) - 1024, "chunk_plan: request %d is longer than 2^31 - 1024 tokens", i);
     for (int q0 = 0; q0 < n; q0 += tile) {
       const int nq = std::min(tile, n - q0);
       // pages that the tile's last token can see if the last page is full (the kernel knows its true length)

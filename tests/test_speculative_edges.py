@@ -51,6 +51,20 @@ def test_chunk_plan_splits_no_further_than_its_plan_holds():
         _plan(new, pages, workspace_bytes=-1)
 
 
+def test_chunk_plan_keeps_positions_within_32_bits():
+    """Kernels walk a request in steps of a tile: the step behind its last token has to be a 32-bit position too."""
+    for pages in ((1 << 27) - 1, (1 << 27) - 63):
+        with pytest.raises(ValueError, match="2\\^31"):
+            _plan([1], [pages])
+    plan, _ = _plan([1], [(1 << 27) - 64])
+    _check_cover_ends(plan, (1 << 27) - 64)
+
+
+def _check_cover_ends(plan, pages):
+    items = sorted(tuple(it[3:5]) for it in plan[16: 16 + 12 * plan[1]].reshape(-1, 12))
+    assert items[0][0] == 0 and items[-1][1] == pages and all(a[1] == b[0] for a, b in zip(items, items[1:]))
+
+
 # ---- stages and tasks ------------------------------------------------------------------------------------------------------------
 ARGS = dk.ModelArgs(dim=64, n_layers=2, n_heads=2, n_kv_heads=1, vocab_size=64, ffn_dim=64)
 

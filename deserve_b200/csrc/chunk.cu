@@ -9,6 +9,7 @@
 // (request, q tile, page range): the tile's tokens and the G q heads of a kv head are stacked into
 // rows (row = token * G + head), so one pass over a K/V tile serves all of them.
 #include <algorithm>
+#include <exception>
 #include <type_traits>
 #include <vector>
 
@@ -399,15 +400,22 @@ int chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int
 
   struct Tile { int req, q0, nq, pages; };
   std::vector<Tile> tiles;
-  int64_t total_pages = 0;
+  int64_t total_pages = 0, n_tiles = 0;
   int max_pages = 0;
+  bool fits = true;
   DSV_REQUIRE(qo_indptr_host[0] == 0 && kv_indptr_host[0] >= 0, "chunk_plan: indptr must begin at 0");
   for (int i = 0; i < batch; ++i) {
     const int n = qo_indptr_host[i + 1] - qo_indptr_host[i], np = kv_indptr_host[i + 1] - kv_indptr_host[i];
     DSV_REQUIRE(n >= 0 && np >= 0, "chunk_plan: indptr not monotone at %d", i);
     // (positions are 32-bit in the kernels, which step past the end by up to a tile of 128 and a lane's box)
     DSV_REQUIRE((int64_t)np * page_size <= (1ll << 31) - 1024, "chunk_plan: request %d is longer than 2^31 - 1024 tokens", i);
-    for (int q0 = 0; q0 < n; q0 += tile) {
+    // whole tiles are the least that a plan can have: one that the caller has no room for takes no memory either
+    n_tiles += (n + (int64_t)tile - 1) / tile;
+    if (kPlanHeader + kItemInts * n_tiles > plan_capacity_i32) {
+      fits = false;
+      continue;
+    }
+    for (int q0 = 0; q0 < n; q0 += std::min(tile, n - q0)) {
       const int nq = std::min(tile, n - q0);
       // pages that the tile's last token can see if the last page is full (the kernel knows its true length)
       const int64_t seen = (int64_t)np * page_size - n + q0 + nq;
@@ -416,6 +424,11 @@ int chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int
       total_pages += pages;
       max_pages = std::max(max_pages, pages);
     }
+  }
+  if (!fits) {
+    *plan_used_i32 = kPlanHeader + kItemInts * n_tiles;
+    *workspace_bytes = 0;
+    return fail(DSV_E_WORKSPACE, "chunk_plan: plan needs %lld int32, capacity %lld", (long long)*plan_used_i32, (long long)plan_capacity_i32);
   }
   // Part length: compared on a model of the launch. A CTA costs the bytes it streams plus a fixed
   // overhead (fill and drain of its ring, q), a launch that splits anything a merge and the partial
@@ -534,8 +547,12 @@ int dsv_chunk_plan_within(const int32_t* qo_indptr_host, const int32_t* kv_indpt
                           int64_t* plan_used_i32, int64_t* workspace_bytes) {
   using namespace dsv;
   DSV_REQUIRE(workspace_capacity >= 0, "chunk_plan: negative workspace_capacity");
-  return chunk_plan(qo_indptr_host, kv_indptr_host, batch, n_q_heads, n_kv_heads, head_dim, page_size, dtype, sm_count, workspace_capacity,
-                    plan_host, plan_capacity_i32, plan_used_i32, workspace_bytes);
+  try {
+    return chunk_plan(qo_indptr_host, kv_indptr_host, batch, n_q_heads, n_kv_heads, head_dim, page_size, dtype, sm_count, workspace_capacity,
+                      plan_host, plan_capacity_i32, plan_used_i32, workspace_bytes);
+  } catch (const std::exception& e) {  // no exception leaves a C entry
+    return fail(DSV_E_WORKSPACE, "chunk_plan: %s", e.what());
+  }
 }
 
 int dsv_chunk_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host, int batch, int n_q_heads,

@@ -65,6 +65,34 @@ def _check_cover_ends(plan, pages):
     assert items[0][0] == 0 and items[-1][1] == pages and all(a[1] == b[0] for a, b in zip(items, items[1:]))
 
 
+BEYOND_MEMORY = """
+import ctypes, resource
+import numpy as np
+from deserve_b200 import _lib
+size = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (size + (64 << 20),) * 2)
+qo, kv = np.array([0, 2**31 - 1], dtype=np.int32), np.array([0, 1], dtype=np.int32)
+plan, used, ws = np.zeros(4096, dtype=np.int32), ctypes.c_int64(), ctypes.c_int64()
+for capacity in (4096, 2**62):  # what there is, and more than the planner can have
+    rc = _lib.lib.dsv_chunk_plan(qo.ctypes.data, kv.ctypes.data, 1, 1, 1, 64, 16, _lib.dtype_code(__import__("torch").float32), 148,
+                                 plan.ctypes.data, capacity, ctypes.byref(used), ctypes.byref(ws))
+    assert rc == _lib.E_WORKSPACE, rc
+    print(_lib.last_error())
+"""
+
+
+def test_chunk_plan_beyond_memory_is_an_error_code():
+    """2^31 - 1 new tokens, 64 MiB left to the process: refused by the capacity, or by the allocation that fails; not the end of the
+    process."""
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", BEYOND_MEMORY], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    needs, alloc = r.stdout.splitlines()[-2:]
+    assert "plan needs" in needs and "alloc" in alloc
+
+
 # ---- stages and tasks ------------------------------------------------------------------------------------------------------------
 ARGS = dk.ModelArgs(dim=64, n_layers=2, n_heads=2, n_kv_heads=1, vocab_size=64, ffn_dim=64)
 

@@ -84,6 +84,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
                  bar_sfull = bars + 104, bar_pfull = bars + 120, bar_odone = bars + 136;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (bars - base) + 152);
   volatile int* poison = reinterpret_cast<volatile int*>(smem + (bars - base) + 156);
+  volatile int* gave_up = poison + 1;  // some wait ran out
 
   if (tid == 0) {
     mbar_init(bar_q, 1);
@@ -99,6 +100,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
       mbar_init(bar_odone + 8 * s, 1);
     }
     *poison = 0;
+    *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 8) {  // TMEM: all 512 columns (one CTA per SM)
@@ -112,6 +114,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  bool ok = true;   // every wait of this warp has ended
+  int issued = 0;   // tiles that a producer has asked for, or whether the issuer has issued anything
 
   if (warp == 8 || warp == 10) {
     // ================================ TMA producers: warp 8 = q + K ring, warp 10 = V ring =======
@@ -139,7 +143,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
     for (int tile = 0; tile < n_tiles; ++tile) {
       const int s = tile % n_stages, round = tile / n_stages;
       const int next = tile + 1 < n_tiles ? page_of(tile + 1) : -1;  // looked up ahead of the wait
-      if (round > 0 && !warp_wait(bar_empty + 8 * s, (round - 1) & 1, p.status)) break;
+      if (round > 0 && !warp_wait(bar_empty + 8 * s, (round - 1) & 1, p.status)) { ok = false; break; }
       const unsigned live = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0) mbar_expect_tx(bar_full + 8 * s, (uint32_t)(__popc(live) * DH * bt * 128));
       __syncwarp();
@@ -156,11 +160,13 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
         }
       }
       page = next;
+      issued = tile + 1;
     }
   } else if (warp == 9) {
     // ================================ MMA issuer (one thread) ===================================
     if (lane == 0 && units > 0) {
-      bool ok = mbar_wait(bar_q, 0, p.status);
+      ok = mbar_wait(bar_q, 0, p.status);
+      issued = ok ? 1 : 0;
       auto issue_qk = [&](int u) {  // S_x = Q K_tile^T; wait for the K tile on its first use
         const int x = u & 1, tile = dual ? u >> 1 : u, s = tile % k_stages;
         if (!dual || x == 0) {
@@ -216,7 +222,6 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
     const uint32_t s_addr = tmem + lane_base + x * COL_SET, o_addr = s_addr + COL_O;
     const float sc = p.scale_log2;
     float m_used = -INFINITY, l = 0.f;
-    bool ok = true;
     for (int i = 0; i < my_units; ++i) {
       if (!warp_wait(bar_sfull + 8 * x, i & 1, p.status)) { ok = false; break; }
       tc_fence_after();
@@ -412,8 +417,23 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant
   }
 
   // ---- teardown: everyone meets here, then the allocating warp frees TMEM ----------------------
+  if (!ok) *gave_up = 1;
   tc_fence_before();
   __syncthreads();
+  if (*gave_up) {  // a CTA that gave up still sees its copies and products end, within the same limits
+    if (warp == 8 || warp == 10) {
+      const int n_stages = warp == 10 ? kVStages : k_stages;
+      const uint32_t full = warp == 10 ? bar_vfull : bar_kfull;
+      for (int k = max(issued - n_stages, 0); k < issued; ++k) warp_wait(full + 8 * (k % n_stages), (k / n_stages) & 1, p.status);
+      if (warp == 8 && units > 0) warp_wait(bar_q, 0, p.status);
+    }
+    __syncthreads();
+    if (warp == 9 && lane == 0 && issued) {
+      tc_commit(bar_q);  // the barrier's second phase: all products issued so far
+      mbar_wait(bar_q, 1, p.status);
+    }
+    __syncthreads();
+  }
   if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");

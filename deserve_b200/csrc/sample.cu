@@ -1876,6 +1876,8 @@ int dsv_sample_top_p(const void* logits, int64_t row_stride, int rows, int vocab
   DSV_REQUIRE(logits && temperature && top_p && uniform && tokens, "sample_top_p: null pointer argument");
   DSV_REQUIRE(row_stride >= vocab && (probs == nullptr || probs_stride >= vocab), "sample_top_p: row stride smaller than a row");
   DSV_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (elem_size(dtype) - 1)) == 0, "sample_top_p: misaligned logits");
+  // a warp may write probabilities while another still looks for the token
+  DSV_REQUIRE(logits != (const void*)probs, "sample_top_p: probs must not be logits");
   SampleParams p = {};
   p.logits = logits; p.row_stride = row_stride; p.vocab = vocab; p.temperature = temperature; p.top_p = top_p;
   p.uniform = uniform; p.tokens = tokens; p.probs = probs; p.probs_stride = probs_stride;

@@ -654,8 +654,8 @@ def sample_top_p(logits: torch.Tensor, temperature: torch.Tensor, top_p: torch.T
     """int32 tokens drawn from every row of [rows, vocab] logits. temperature, top_p and uniform (in [0, 1),
     one random number per row) are float32 [rows]; a row with temperature <= 0 takes the argmax. The nucleus
     is the shortest prefix of the tokens by probability (lower index first among equals) whose mass exceeds
-    top_p; the draw walks it in index order. probs, if given ([rows, vocab] float32), receives the kept,
-    renormalised probabilities: what verify_draft takes as draft_probs."""
+    top_p; the draw walks it in index order. probs, if given ([rows, vocab] float32, not overlapping
+    logits), receives the kept, renormalised probabilities: what verify_draft takes as draft_probs."""
     dev = _same_device("sample_top_p", logits, temperature, top_p, uniform, probs, out)
     stride = _rows_of(logits, "sample_top_p: logits")
     rows, vocab = logits.shape

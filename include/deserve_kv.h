@@ -152,7 +152,7 @@ int dsv_greedy_sample(const void* logits, int64_t row_stride, int rows, int voca
  * (or NaN): the argmax, lowest index among equals. NaN and -inf entries are no tokens; a
  * row without any gives token 0. probs (optional, may be NULL): [rows, vocab] fp32, the
  * kept weights over their sum, 0 elsewhere (one at the argmax for a greedy row, all 0 for
- * a row without tokens). Weights and sums are 64-bit (weights below 2^-45 of the largest
+ * a row without tokens); they may not overlap logits. Weights and sums are 64-bit (weights below 2^-45 of the largest
  * cannot be drawn), so the token does not depend on the launch. vocab <= 2^18
  * (DSV_E_UNSUPPORTED above). Row strides in elements, any alignment of a row.
  */

@@ -93,6 +93,13 @@ def test_chunk_plan_beyond_memory_is_an_error_code():
     assert "plan needs" in needs and "alloc" in alloc
 
 
+def test_sample_top_p_does_not_write_probabilities_over_its_logits():
+    buf = np.zeros(256, dtype=np.float32)
+    at = buf.ctypes.data
+    assert _lib.lib.dsv_sample_top_p(at, 64, 2, 64, at, at, at, at, at, 64, _lib.dtype_code(torch.float32), None) == _lib.E_INVALID
+    assert "must not be logits" in _lib.last_error()
+
+
 # ---- stages and tasks ------------------------------------------------------------------------------------------------------------
 ARGS = dk.ModelArgs(dim=64, n_layers=2, n_heads=2, n_kv_heads=1, vocab_size=64, ffn_dim=64)
 

@@ -587,7 +587,7 @@ int dsv_paged_chunk_attention(const void* q, int64_t q_stride_tok, const int32_t
   const int64_t part_rows = plan_host[10];
   DSV_REQUIRE(n_items >= 0 && merge_rows >= 0 && part_rows >= 0 && plan_host[3] > 0, "chunk: corrupt plan");
   if (n_items == 0) return DSV_OK;
-  DSV_REQUIRE(kv_indices != nullptr, "chunk: null pointer argument");
+  DSV_REQUIRE(kv_indices != nullptr || plan_host[15] == 0, "chunk: null pointer argument");  // no request has a page: an empty list
   const int es = elem_size(dtype);
   DSV_REQUIRE(aligned16(q) && aligned16(pages_layer) && aligned16(out) && (q_stride_tok * es) % 16 == 0 &&
                   (out_stride_tok * es) % 16 == 0 && (page_stride * es) % 16 == 0,

@@ -225,7 +225,7 @@ def _chunk_batch(seed, lens, new, hq, hkv, d, ps, dtype):
     ids = torch.randperm(int(kvp[-1]) + 3, generator=g)[: int(kvp[-1])].to(torch.int32).to(DEV)
     pages = torch.randn(int(kvp[-1]) + 3, 2, ps, hkv, d, generator=g).to(dtype).to(DEV)
     q = torch.randn(int(qo[-1]), hq, d, generator=g).to(dtype).to(DEV)
-    last = torch.tensor([(n - 1) % ps + 1 for n in lens], dtype=torch.int32, device=DEV)
+    last = torch.tensor([(n - 1) % ps + 1 if n else 0 for n in lens], dtype=torch.int32, device=DEV)
     w = ops.BatchChunkWithPagedKVCacheWrapper(torch.empty(64 << 20, dtype=torch.uint8, device=DEV))
     w.begin_forward(torch.from_numpy(qo).to(DEV), torch.from_numpy(kvp).to(DEV), ids, last, hq, hkv, d, ps, dtype,
                     qo_indptr_host=qo, kv_indptr_host=kvp)
@@ -313,3 +313,29 @@ def test_chunk_attention_with_a_scale_that_is_not_positive(dtype, new, scale):
     tol = torch.finfo(dtype).eps / 2 * want.abs() + size * (eps / 2 + arith[..., None])
     assert ((out.double() - want).abs() <= tol).all()
     assert ((lse.double() - want_lse).abs() <= arith + 2.0**-23 * want_lse.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[3], [2, 0, 40]])
+def test_chunk_attention_of_a_batch_without_any_cache(dtype, new):
+    """No request has a page: every row sees nothing."""
+    w, q, pages, ids, qo, kvp = _chunk_batch(2, [0] * len(new), new, 8, 2, 128, 16, dtype)
+    assert ids.numel() == 0
+    out, lse = torch.full_like(q, 3.0), torch.full(q.shape[:2], 3.0, device=DEV)
+    w.forward(q, pages, out=out, lse=lse)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("dtype,hq", [(torch.float32, 8), (torch.bfloat16, 8), (torch.float16, 32)])
+def test_chunk_attention_reports_a_page_outside_the_pool(dtype, hq):
+    """... and reads page 0 in its place; the requests that do not hold it are as before."""
+    w, q, pages, ids, qo, kvp = _chunk_batch(5, [700, 90], [4, 3], hq, 2, 128, 16, dtype)
+    want = w.forward(q, pages)
+    for bad in (-1, len(pages), 2**31 - 1):
+        kept = int(ids[7])
+        ids[7] = bad
+        got = w.forward(q, pages)
+        torch.cuda.synchronize()
+        assert _lib.read_device_status() == 1
+        assert torch.equal(got[4:], want[4:]) and torch.isfinite(got).all()
+        ids[7] = kept

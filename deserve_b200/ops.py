@@ -532,8 +532,9 @@ class BatchChunkWithPagedKVCacheWrapper:
         used, _ = make_chunk_plan(qo_indptr_host, kv_indptr_host, num_qo_heads, num_kv_heads, head_dim, page_size,
                                   data_type if isinstance(data_type, torch.dtype) else torch.float16,
                                   self._sm_count, plan, self._ws.numel() - self._PLAN_BYTES)
-        self._ws[: used * 4].view(torch.int32).copy_(pinned[:used], non_blocking=True)
-        _pinned_ring("chunk_plan").done(slot)
+        with _on(dev):  # the event that frees the pinned buffer has to be one of the copy's stream
+            self._ws[: used * 4].view(torch.int32).copy_(pinned[:used], non_blocking=True)
+            _pinned_ring("chunk_plan").done(slot)
         _COUNTERS["h2d_bytes"] += used * 4
         self._plan_host = plan[:16].copy()  # the header is all that a call reads on the host
         self._desc = (dev, batch, num_qo_heads, num_kv_heads, head_dim, page_size, pointers)

@@ -15,11 +15,11 @@
 // full HBM speed (2850 cycles per SM), so even a few live rows are bound by the K/V traffic; warps without a
 // live row only pass the barriers. K and V arrive in boxes of 16 tokens x head_dim (4 KB for head_dim 128).
 //
-// Measured (bf16, 8 kv heads of 128): one request of 65,536 tokens, 5 of them new, 32 q heads: 54.6 us with the merge, 4.9 TB/s;
-// 128 requests of 512-4096 tokens, 1-8 new, 64 q heads (1.24 GB): 238 us, 5.2 TB/s. A 64 KB tile takes 1.58 us per SM in
+// Measured (bf16, 8 kv heads of 128): one request of 65,536 tokens, 5 of them new, 32 q heads: 55 us with the merge, 4.9 TB/s;
+// 128 requests of 512-4096 tokens, 1-8 new, 64 q heads (1.24 GB): 239 us, 5.2 TB/s. A 64 KB tile takes 1.58 us per SM in
 // the steady state (6 TB/s), the rest is each CTA's fill and drain, about 6 us; CTAs that stay and carry their rings over
 // several items were slower (60 and 264 us: their softmax warps spill). 16 requests of 3000-8192 tokens with 100-257 new ones
-// (206 GFLOP): 342 us, bound by the softmax between the products.
+// (206 GFLOP): 340-344 us, bound by the softmax between the products.
 #pragma once
 
 #include <cuda.h>

@@ -5,14 +5,17 @@
 // whole sum. With Z the sum of the kept weights, p_v = w_v / Z for kept v and 0 otherwise. A draw with
 // u in [0, 1) takes the first v in INDEX order whose running sum of p exceeds u times the whole.
 //
-// Which token a draw takes depends on ~1e5 borders per row: sums in fp32 would move some of them and the
+// Which token a draw takes depends on ~1e5 borders per row: rounded sums would move some of them and the
 // result would depend on how a row is cut among threads. Weights are therefore 64-bit fixed point
 // (units of 2^-44 of the largest weight, evaluated in double): integer sums are exact and associative,
 // so every cut of the row, and every order of the atomics, gives the same token. 2^18 entries of
-// weight one still fit 63 bits, hence the bound on the vocabulary.
+// weight one still fit 63 bits, hence the bound on the vocabulary. Sums in double (one walk, before the
+// largest logit is known) and in fp32 (drafts) decide only where the answer lies farther from a border
+// than they can differ from the integers; what comes closer, below 1 % of ordinary rows, goes the exact
+// way. So the token depends neither on the launch nor on which way a row went.
 //
-// A row is read from HBM once: a cluster of up to 8 CTAs keeps it in shared memory, or, with many rows, one
-// CTA finds it in L2 again. The largest logit, the weight sums, the top-p border and the draw each walk it
+// A row is read from HBM once: a cluster of up to 8 CTAs keeps it in shared memory, or, with many rows,
+// finds it in L2 again. The largest logit, the weight sums, the top-p border and the draw each walk it
 // there. Sums and histograms of a cluster's CTAs meet through distributed shared memory.
 //
 // The top-p border is found without sorting: a histogram of weight over 2048 bins of (max - l) / T gives
@@ -20,9 +23,11 @@
 // one token is left (two or three times).
 //
 // Bound by the arithmetic of the FP64 weights (about 28 instructions an entry; issue slots 64 % busy, the FP64 pipe 40 %), few rows by
-// the chain of exchanges (2 us each). Measured: 1 row of 128,256 bf16 logits 15 us, 128 rows 88 us, 1024 rows without a border 156 us
-// (1.7 TB/s); 64 rows of 32,003 fp32 with probabilities 34 us; verification of 128 requests with 0-7 drafts each (128,256,
-// bf16) 176 us, 52 of them the streaming decision (4.1 TB/s), the rest one exact draw per request.
+// the chain of exchanges (2 us each). Measured: 1 row of 128,256 bf16 logits 16 us, 128 rows 91 us, 1024 rows without a border 160 us
+// (1.6 TB/s); 64 rows of 32,003 fp32 with probabilities 34 us; verification of 128 requests with 0-7 drafts each (128,256,
+// bf16) 165 us, 52 of them the streaming decision (4.1 TB/s), the rest one draw per request. Slower: 1024 rows whose border lies in a
+// flat tail around zero 2.4 ms (count_border crosses the 16-bit values 2048 at a time, and most of them lie around zero); drafts at
+// temperatures of 0.1 and below, where the streaming decision leaves most of them open: 240-345 us for 128 requests.
 #include <algorithm>
 #include <type_traits>
 
@@ -240,7 +245,8 @@ __device__ __forceinline__ double top_weight(const RowScale& s) {
   return kOne * exp2(fma((double)s.top, s.c, s.magic - 6755399441055744.0) * 0.015625);
 }
 // Fixed-point weight behind kRaw (subtract it; sums may subtract it once per entry). With l c = N + r, |r| <= 1/2:
-// 2^((N - K) / 64) from a table of 2^(j / 64) and an exponent, e^(r ln 2 / 64) to the fourth power (its argument is
+// 2^((N - K) / 64) from a table of 2^(j / 64) and an exponent, e^(r ln 2 / 64) by its Taylor series to the fourth power (the table-driven
+// exponential of P. T. P. Tang, ACM TOMS 15, 1989) (its argument is
 // below 0.0055: the next term is under 2^-44). Eight FP64 instructions: 128,256 entries keep one SM's FP64 units
 // busy for 8 us, 1.5 times what its share of HBM takes to bring them in 16 bits.
 __device__ __forceinline__ u64 raw_weight(float l, const RowScale& s, const double* __restrict__ table) {
@@ -894,7 +900,6 @@ __device__ int hist_find(Shared& sh, int s, u64 limit, u64& before, u64& mass, F
   return (int)__shfl_sync(0xffffffffu, x, from);
 }
 
-// The kept tokens: those above `value`, and of those equal to it the ones up to index `index`.
 // A warp's entries within kWindow nats of the top, in index order. They are a small part of most rows, and where all of them
 // are held and the border lies among them, nothing behind them is looked at again.
 struct Entry {
@@ -909,6 +914,7 @@ struct Near {
   __device__ __forceinline__ Entry* mine() const { return all + (threadIdx.x >> 5) * cap; }
 };
 
+// The kept tokens: those above `value`, and of those equal to it the ones up to index `index`.
 struct Kept {
   float value;
   int index;

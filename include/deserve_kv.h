@@ -143,17 +143,19 @@ int dsv_greedy_sample(const void* logits, int64_t row_stride, int rows, int voca
 
 /*
  * Temperature / top-p sampling of every row of logits, the temperature > 0 branch of
- * deserve_worker/layer_storage.py:219-253 for a whole batch, with the random numbers
- * given. Row r has weights w_v = exp((l_v - max l) / temperature[r]); entries are ranked
- * by value, the lower index first among equals; v is kept when the weights ranked before
- * it sum to at most top_p[r] times the whole sum (top_p >= 1, or NaN: all are kept; the
+ * deserve_worker/layer_storage.py:199-277 (sample_top_p, 31-54) for a whole batch, with
+ * the random numbers given. Row r has weights w_v = exp((l_v - max l) / temperature[r]);
+ * entries are ranked by value, the lower index first among equals; v is kept when the
+ * weights ranked before it sum to at most top_p[r] times the whole sum (top_p >= 1, or NaN: all are kept; the
  * first entry always is). tokens[r] is the first kept v in INDEX order whose running sum
  * of kept weights exceeds uniform[r] (in [0, 1)) times the kept sum. temperature[r] <= 0
  * (or NaN): the argmax, lowest index among equals. NaN and -inf entries are no tokens; a
  * row without any gives token 0. probs (optional, may be NULL): [rows, vocab] fp32, the
  * kept weights over their sum, 0 elsewhere (one at the argmax for a greedy row, all 0 for
- * a row without tokens); they may not overlap logits. Weights and sums are 64-bit (weights below 2^-45 of the largest
- * cannot be drawn), so the token does not depend on the launch. vocab <= 2^18
+ * a row without tokens); they may not overlap logits. Weights and the sums that decide
+ * are 64-bit fixed point (weights below 2^-45 of the largest cannot be drawn), so the
+ * token does not depend on the launch, the number of rows in the call included; probabilities are fp32 and may
+ * differ in their last bits between launches. vocab <= 2^18
  * (DSV_E_UNSUPPORTED above). Row strides in elements, any alignment of a row.
  */
 int dsv_sample_top_p(const void* logits, int64_t row_stride, int rows, int vocab,
@@ -173,8 +175,11 @@ int dsv_sample_top_p(const void* logits, int64_t row_stride, int rows, int vocab
  * next_tokens[i] is drawn, with the uniform number of the request's LAST row, from
  * max(p - q, 0) of the first rejected row (from p where nothing is left) or from p of
  * the last row when every draft was accepted: first index in ascending order whose running
- * sum exceeds u times the whole. A request without rows gets accepted 0 and token -1; a
- * draft outside [0, vocab) is rejected. Rows behind indptr[batch] are not read.
+ * sum exceeds u times the whole. Neither answer depends on the launch. A request without
+ * rows gets accepted 0 and token -1; a draft outside [0, vocab), or one whose weight cannot
+ * be drawn, is rejected. An indptr that is not monotone, or goes past nnz, is recorded in
+ * the device status word (2); requests that end before they begin, or past nnz, get
+ * accepted 0 and token -1, the others' answers are then undefined. Rows behind indptr[batch] are not read.
  * workspace: device scratch of nnz bytes; may be NULL when nnz is 0.
  */
 int dsv_verify_draft(const void* logits, int64_t row_stride, int nnz, int vocab,
